@@ -541,6 +541,107 @@ typedef struct tb_dest_sample_io {
 } tb_dest_sample_io;
 int tb_dest_sample(tb_ctx* ctx, const tb_dest_sample_io* io, tb_stream stream);
 
+/* -- training operators of a transformer layer ------------------------------------------------------------------------------ */
+/* Forward and backward of what `TransformerCrossAttention` (src/models/modules/transformer.py:98-240), `Attention`
+ * (src/models/modules/attention.py:9-154) and `MLP` (src/models/modules/mlp.py:20-85) are made of: attention, layer norm, Linear with its
+ * epilogue.  They read no loaded weight (a context without tb_finalize_weights will do), take every tensor as it lies, keep nothing
+ * between calls and own no memory: scratch comes from the caller (`workspace`; *_workspace_bytes says how much, 0 = may be NULL), so calls
+ * on different streams, and captured graphs, are independent of each other as long as their buffers are.  Sums, softmax statistics
+ * and norms are fp32, results are rounded once; every result has the same bits in every run.  Buffers of one call must not overlap, except
+ * that inputs may share memory.  The device of the context is used and the calling thread's current device restored.
+ * dtype of a call's tensors: 0 = fp32, 1 = bf16 (the values of tb_config.operand_precision).  fp32 operands are multiplied as three bf16
+ * planes, six products (fp32's range, error as of an fp32 product); an infinite or NaN operand turns the results it enters into NaN. */
+
+/* Attention.  Query head h uses key / value head h / (n_head / n_kv_head).  Query i may attend to key j when key_valid[j], query_valid[i],
+ * not attn_mask[i][j] and, with `causal`, j <= i + n_key - n_query.  A query that may attend to nothing gets out = 0, lse = -inf and
+ * gradients 0.  Rows of invalid queries and keys are not looked at (they may hold anything, infinities and NaN too) and their
+ * gradients are 0; keys that only attn_mask or `causal` hide must hold finite values.  n_batch, n_query and n_key may be 0.
+ * Replaces: the products, masks and softmax of Attention.forward (attention.py:90-141) between its in- and out-projection. */
+typedef struct tb_attention_io {
+    int32_t dtype, n_batch, n_query, n_key, n_head, n_kv_head, head_dim; /* 1 <= head_dim <= 128; n_head a multiple of n_kv_head */
+    int32_t causal;
+    float scale;                  /* > 0, usually 1 / sqrt(head_dim) */
+    /* [n_batch, n_query | n_key, n_head | n_kv_head, head_dim], components adjacent; strides in elements over (batch, position, head) */
+    const void* q;
+    const void* k;
+    const void* v;
+    int64_t q_strides[3], k_strides[3], v_strides[3];
+    const uint8_t* query_valid;   /* [n_batch, n_query] or NULL = all */
+    const uint8_t* key_valid;     /* [n_batch, n_key] or NULL = all */
+    const uint8_t* attn_mask;     /* nonzero = may NOT attend (attention.py:90-99); keys adjacent, or NULL */
+    int64_t attn_mask_strides[2]; /* bytes over (batch, query); 0 over the batch = one mask for all */
+    void* out;                    /* tb_attention: written; tb_attention_backward: what tb_attention wrote */
+    int64_t out_strides[3];
+    float* lse;                   /* [n_batch, n_head, n_query], natural logarithm; as `out` */
+    /* tb_attention_backward only */
+    const void* d_out;
+    int64_t d_out_strides[3];
+    void* dq;                     /* written */
+    void* dk;
+    void* dv;
+    int64_t dq_strides[3], dk_strides[3], dv_strides[3];
+    void* workspace;              /* tb_attention_workspace_bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+} tb_attention_io;
+int tb_attention(tb_ctx* ctx, const tb_attention_io* io, tb_stream stream);
+int tb_attention_backward(tb_ctx* ctx, const tb_attention_io* io, tb_stream stream);
+/* from the sizes of `io` alone; -1 where they are not allowed */
+int64_t tb_attention_workspace_bytes(const tb_attention_io* io, int32_t backward);
+
+/* Layer norm of rows of n_col elements: y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(var + eps) (biased variance).
+ * Replaces: nn.LayerNorm (transformer.py:41-49, mlp.py:45-60).  n_row may be 0; 1 <= n_col <= 8192. */
+typedef struct tb_layer_norm_io {
+    int32_t dtype, n_col;
+    int64_t n_row;
+    float eps;                    /* tb_layer_norm only */
+    const void* x;                /* [n_row, n_col] */
+    const void* weight;           /* [n_col] or NULL = 1 */
+    const void* bias;             /* [n_col] or NULL = 0; tb_layer_norm only */
+    void* y;                      /* [n_row, n_col] written by tb_layer_norm */
+    float* mean;                  /* [n_row] written by tb_layer_norm, read by tb_layer_norm_backward */
+    float* rstd;
+    /* tb_layer_norm_backward only */
+    const void* d_out;            /* [n_row, n_col] */
+    void* dx;                     /* [n_row, n_col] or NULL = not wanted */
+    void* dweight;                /* [n_col] or NULL */
+    void* dbias;                  /* [n_col] or NULL */
+    void* workspace;              /* tb_layer_norm_workspace_bytes (backward), 16-byte aligned */
+    int64_t workspace_bytes;
+} tb_layer_norm_io;
+int tb_layer_norm(tb_ctx* ctx, const tb_layer_norm_io* io, tb_stream stream);
+int tb_layer_norm_backward(tb_ctx* ctx, const tb_layer_norm_io* io, tb_stream stream);
+int64_t tb_layer_norm_workspace_bytes(const tb_layer_norm_io* io, int32_t backward);
+
+/* Linear with its epilogue: a = act(x weight^T + bias), 0 in rows that are not valid, y = a + residual; act: 0 none, 1 ReLU.
+ * backward: dz = d_out [a > 0 for ReLU] in valid rows, 0 elsewhere; dx = dz weight, dweight = dz^T x, dbias = sum of dz over the rows (the
+ * residual's gradient is d_out itself).  Invalid rows of x are not looked at.  n_row may be 0; n_in, n_out >= 1.
+ * Replaces: the Linears, masks and residuals of attention.py:81-87,142-146, transformer.py:197-222, mlp.py:62-85. */
+typedef struct tb_linear_io {
+    int32_t dtype, n_in, n_out, activation;
+    int64_t n_row;
+    const void* x;                /* [n_row, n_in] */
+    const void* weight;           /* [n_out, n_in] */
+    const void* bias;             /* [n_out] or NULL; tb_linear only */
+    const uint8_t* row_valid;     /* [n_row] or NULL = all */
+    const void* residual;         /* [n_row, n_out] or NULL; tb_linear only */
+    void* y;                      /* [n_row, n_out] written by tb_linear */
+    /* a, [n_row, n_out]: tb_linear writes it unless NULL; tb_linear_backward reads it for ReLU (without a residual it is y) */
+    void* act;
+    /* tb_linear_backward only */
+    const void* d_out;            /* [n_row, n_out] */
+    void* dx;                     /* [n_row, n_in] or NULL = not wanted */
+    void* dweight;                /* [n_out, n_in] or NULL */
+    void* dbias;                  /* [n_out] or NULL */
+    void* workspace;              /* tb_linear_workspace_bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+} tb_linear_io;
+int tb_linear(tb_ctx* ctx, const tb_linear_io* io, tb_stream stream);
+int tb_linear_backward(tb_ctx* ctx, const tb_linear_io* io, tb_stream stream);
+int64_t tb_linear_workspace_bytes(const tb_linear_io* io, int32_t backward);
+
+/* sizeof() of tb_attention_io, tb_layer_norm_io, tb_linear_io as the library was compiled (see tb_struct_sizes) */
+void tb_operator_struct_sizes(int32_t out[3]);
+
 /* sizeof() of the structs of this header as the library was compiled: out[0..5] = tb_config, tb_rollout_io, tb_encode_io,
  * tb_rule_io, tb_post_io, tb_metric_io; out[6] = the pointer size; out[7..8] = tb_posterior_io, tb_train_io; out[9..10] = tb_step_override, tb_forward_io;
  * out[11..12] = tb_latent_sample_io, tb_dest_sample_io -- lets a binding check its mirror of the layouts before the first call (no GPU needed). */

@@ -1,0 +1,173 @@
+"""The training operators of a transformer layer in plain torch, 64 bits, on the CPU (test infrastructure): attention with its masks, layer
+norm and Linear with its epilogue, forward and backward from the formulas, and how far a result in fp32 or bf16 may be off -- element by
+element, from the roundings that the operators make.
+
+A rounding to a type is off by at most `U[type]` of the value (half a step).  The operators hold sums, softmax statistics and norms in
+fp32 and round where they say so: a result once, and for bf16 the probabilities and the scores' gradients once more, as operands of the
+next product.  fp32 operands go through three bf16 planes, which leaves out less than 2^-23 of a product."""
+from __future__ import annotations
+
+import math
+from typing import Dict, Optional
+
+import torch
+from torch import Tensor
+
+U = {torch.float32: 2.0**-24, torch.bfloat16: 2.0**-8}
+E = 2.0**-24  # one fp32 operation
+
+
+def hidden(b, lq, lk, query_valid=None, key_valid=None, attn_mask=None, causal=False) -> Tensor:
+    """[b, lq, lk], True where a query may not see a key."""
+    h = torch.zeros(b, lq, lk, dtype=torch.bool)
+    if query_valid is not None:
+        h |= ~query_valid.bool()[:, :, None]
+    if key_valid is not None:
+        h |= ~key_valid.bool()[:, None, :]
+    if attn_mask is not None:
+        h |= attn_mask.bool()
+    if causal:
+        h |= torch.arange(lk)[None, :] > torch.arange(lq)[:, None] + (lk - lq)
+    return h
+
+
+def attention(q, k, v, d_out=None, query_valid=None, key_valid=None, attn_mask=None, causal=False, scale=None) -> Dict[str, Tensor]:
+    """q [B, Lq, H, D], k, v [B, Lk, Hkv, D] (CPU, any type) -> out, lse, with `d_out` also dq, dk, dv (all fp64); and `<name>_bound` for
+    the type of q: how far each element may be off."""
+    t = q.dtype
+    u = U[t]
+    b, lq, h, d = q.shape
+    lk, hkv = k.shape[1:3]
+    scale = 1.0 / math.sqrt(d) if scale is None else scale
+
+    def on(x, valid):  # rows that are not valid are not looked at
+        x = x.double()
+        return x if valid is None else torch.where(valid.bool()[:, :, None, None], x, torch.zeros((), dtype=torch.float64))
+
+    q, k, v = on(q, query_valid), on(k, key_valid), on(v, key_valid)
+    rep = h // hkv
+    qh, kh, vh = q.transpose(1, 2), k.transpose(1, 2).repeat_interleave(rep, 1), v.transpose(1, 2).repeat_interleave(rep, 1)
+    hide = hidden(b, lq, lk, query_valid, key_valid, attn_mask, causal)[:, None]
+    s = (qh @ kh.transpose(-1, -2)) * scale
+    s_abs = (qh.abs() @ kh.abs().transpose(-1, -2)) * scale
+    if lk:
+        lse = torch.logsumexp(s.masked_fill(hide, -math.inf), -1)
+    else:
+        lse = torch.full((b, h, lq), -math.inf, dtype=torch.float64)
+    ref = torch.where(lse == -math.inf, torch.zeros_like(lse), lse)
+    p = torch.exp(s - ref[..., None]).masked_fill(hide, 0)
+    out = p @ vh
+    # a score: D + 4 roundings of the products' sizes, the planes' remainder, the steps in units of log 2 (its size and lse's); e^x turns an
+    # absolute error of x into a relative one; the exponential and the sum's few roundings
+    e_s = E * ((d + 8) * s_abs + 4 * (s.abs() + ref.abs()[..., None]) + 8)
+    e_s = e_s.masked_fill(hide, 0)
+    e_lse = (e_s * p).sum(-1) + E * (math.log2(lk + 2) + 8 + lk / 16) + 4 * E * ref.abs()
+    e_p = e_s + e_lse[..., None]
+    u_p = u if t == torch.bfloat16 else 4 * E  # a probability as an operand
+    n_k = E * (lk / 4 + 8)  # adding up lk terms (16 lanes, tiles of 32)
+    out_err = (p * (e_p + u_p + n_k)) @ vh.abs()
+    r = {"out": out.transpose(1, 2), "out_bound": (out_err + u * (out.abs() + out_err)).transpose(1, 2) + 1e-30, "lse": lse,
+         "lse_bound": e_lse + 4 * E * ref.abs() + 1e-30}
+    if d_out is None:
+        return r
+    g = on(d_out, query_valid).transpose(1, 2)
+    out_err = r["out_bound"].transpose(1, 2)
+    dp, dp_abs = g @ vh.transpose(-1, -2), g.abs() @ vh.abs().transpose(-1, -2)
+    delta = (g * out).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    # ds: the probability's error, the products' roundings, and D from the ROUNDED output
+    e_delta = (g.abs() * out_err).sum(-1, keepdim=True) + E * (d + 8) * (g.abs() * out.abs()).sum(-1, keepdim=True)
+    ds_err = ds.abs() * (e_p + 8 * E) + p * (E * (d + 8) * dp_abs + e_delta)
+    ds_err = ds_err + (u if t == torch.bfloat16 else 4 * E) * (ds.abs() + ds_err)
+    n_q = E * (lq * rep / 4 + 8)
+    dq = (ds @ kh) * scale
+    dq_err = ((ds_err + n_k * ds.abs()) @ kh.abs()) * scale
+    dk = (ds.transpose(-1, -2) @ qh) * scale
+    dk_err = ((ds_err + n_q * ds.abs()).transpose(-1, -2) @ qh.abs()) * scale
+    dv = p.transpose(-1, -2) @ g
+    dv_err = (p * (e_p + u_p + n_q)).transpose(-1, -2) @ g.abs()
+
+    def shared(x):  # the query heads of a key / value head add up
+        return x.view(b, hkv, rep, lk, d).sum(2)
+
+    for name, x, e in (("dq", dq, dq_err), ("dk", shared(dk), shared(dk_err)), ("dv", shared(dv), shared(dv_err))):
+        r[name] = x.transpose(1, 2)
+        r[name + "_bound"] = (e + u * (x.abs() + e)).transpose(1, 2) + 1e-30
+    return r
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, d_out=None) -> Dict[str, Tensor]:
+    """x [rows, C] (CPU) -> y, mean, rstd, with `d_out` also dx, dw, db (fp64), and their bounds for the type of x."""
+    u = U[x.dtype]
+    x = x.double()
+    n, c = x.shape
+    w = torch.ones(c, dtype=torch.float64) if weight is None else weight.double()
+    bb = torch.zeros(c, dtype=torch.float64) if bias is None else bias.double()
+    mean = x.mean(-1, keepdim=True)
+    var = ((x - mean) ** 2).mean(-1, keepdim=True)
+    rstd = 1.0 / torch.sqrt(var + eps)
+    h = (x - mean) * rstd
+    steps = c / 64 + 16  # a lane's terms, the lanes' tree, the few steps behind it
+    e_mean = E * steps * x.abs().mean(-1, keepdim=True)
+    # x - mean is off by e_mean + E |x - mean|; the variance by twice that, and its own sum
+    e_x = e_mean + E * (x - mean).abs()
+    e_var = 2 * ((x - mean).abs() * e_x).mean(-1, keepdim=True) + E * steps * var + e_mean**2
+    e_r = 0.5 * e_var * rstd**2 + 4 * E  # relative
+    e_h = rstd * e_x + h.abs() * (e_r + 2 * E)
+    y = h * w + bb
+    e_y = e_h * w.abs() + 2 * E * (h.abs() * w.abs() + bb.abs())
+    r = {"y": y, "y_bound": e_y + u * (y.abs() + e_y) + 1e-30, "mean": mean[:, 0], "mean_bound": e_mean[:, 0] + 1e-30, "rstd": rstd[:, 0],
+         "rstd_bound": (rstd * e_r)[:, 0]}
+    if d_out is None:
+        return r
+    g = d_out.double()
+    a = g * w
+    m1, m2 = a.mean(-1, keepdim=True), (a * h).mean(-1, keepdim=True)
+    dx = rstd * (a - m1 - h * m2)
+    e_m1 = E * steps * a.abs().mean(-1, keepdim=True)
+    e_m2 = E * steps * (a * h).abs().mean(-1, keepdim=True) + (a.abs() * e_h).mean(-1, keepdim=True)
+    e_dx = rstd * (3 * E * (a.abs() + m1.abs() + (h * m2).abs()) + e_m1 + h.abs() * e_m2 + e_h * m2.abs()) + dx.abs() * (e_r + E)
+    rows = n / 1024 + 64  # a lane's rows, the lanes and waves of a workgroup, the workgroups
+    e_dw = (g.abs() * e_h).sum(0) + E * rows * (g * h).abs().sum(0)
+    e_db = E * rows * g.abs().sum(0)
+    dw, db = (g * h).sum(0), g.sum(0)
+    for name, v, e in (("dx", dx, e_dx), ("dw", dw, e_dw), ("db", db, e_db)):
+        r[name], r[name + "_bound"] = v, e + u * (v.abs() + e) + 1e-30
+    return r
+
+
+def linear(x, weight, bias=None, relu=False, row_valid=None, residual=None) -> Dict[str, Tensor]:
+    """x [M, K], weight [N, K] (CPU) -> y, act (in front of the residual), and their bounds."""
+    u = U[x.dtype]
+    m, k = x.shape
+    x, w = _rows(x, row_valid), weight.double()
+    z, z_abs = x @ w.t(), x.abs() @ w.abs().t()
+    if bias is not None:
+        z, z_abs = z + bias.double(), z_abs + bias.double().abs()
+    e = E * (k / 4 + 16) * z_abs
+    a = z.clamp_min(0) if relu else z
+    if row_valid is not None:
+        off = ~row_valid.bool()[:, None]
+        a, e = a.masked_fill(off, 0), e.masked_fill(off, 0)
+    y = a if residual is None else a + residual.double()
+    return {"act": a, "act_bound": e + u * (a.abs() + e) + 1e-30, "y": y, "y_bound": e + E * y.abs() + u * (y.abs() + e) + 1e-30}
+
+
+def linear_backward(d_out, x, weight, act=None, row_valid=None) -> Dict[str, Tensor]:
+    """-> dx, dw, db and their bounds; `act`: ReLU's output or None."""
+    u = U[x.dtype]
+    (m, k), n = x.shape, weight.shape[0]
+    dz = d_out.double()
+    if act is not None:
+        dz = torch.where(act > 0, dz, torch.zeros_like(dz))
+    dz, x, w = _rows(dz, row_valid), _rows(x, row_valid), weight.double()
+    r = {}
+    for name, v, s, terms in (("dx", dz @ w, dz.abs() @ w.abs(), n), ("dw", dz.t() @ x, dz.abs().t() @ x.abs(), m), ("db", dz.sum(0), dz.abs().sum(0), m)):
+        e = E * (terms / 4 + 16) * s
+        r[name], r[name + "_bound"] = v, e + u * (v.abs() + e) + 1e-30
+    return r
+
+
+def _rows(x: Tensor, row_valid: Optional[Tensor]) -> Tensor:
+    x = x.double()
+    return x if row_valid is None else torch.where(row_valid.bool()[:, None], x, torch.zeros((), dtype=torch.float64))

@@ -1,0 +1,290 @@
+// Layer norm for training.  Per row of C elements: m = mean x, r = 1 / sqrt(mean (x - m)^2 + eps), h = (x - m) r, y = h g + b;
+//   backward: a = dy g,  dx = r (a - mean a - h mean(a h)),  dg = sum over rows of dy h,  db = sum over rows of dy.
+// HBM-bound: one pass over x (and dy) with the row in registers, in fp32; the variance is taken around the mean (two passes over
+// registers, not over memory).  A row is held by LPR lanes, each with NV chunks of 16 bytes: 8 lanes for a row of 64 bf16 up to a whole
+// workgroup for wide rows, so that every load is 16 bytes and no lane idles on short rows.
+// The weights' gradients are summed per lane over the rows of a workgroup, written once per workgroup and added up by a second kernel in
+// workgroup order: no atomics, the same bits every run.
+#include "tb_ops.hpp"
+
+#include "tb_ops_host.hpp"
+
+namespace tb {
+namespace op {
+
+namespace {
+
+constexpr int NT = 256;
+
+template <typename T>
+constexpr int VEC = 16 / sizeof(T);
+
+template <typename T>
+__device__ __forceinline__ void load_chunk(const T* p, int n, float (&x)[VEC<T>]) {
+    typedef T vec __attribute__((ext_vector_type(VEC<T>)));
+    vec v;
+    if (n >= VEC<T>) {
+        __builtin_memcpy(&v, p, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC<T>; ++j) v[j] = j < n ? p[j] : (T)0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < VEC<T>; ++j) x[j] = (float)v[j];
+}
+
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* p, int n, const float (&x)[VEC<T>]) {
+    typedef T vec __attribute__((ext_vector_type(VEC<T>)));
+    vec v;
+#pragma unroll
+    for (int j = 0; j < VEC<T>; ++j) v[j] = (T)x[j];
+    if (n >= VEC<T>) {
+        __builtin_memcpy(p, &v, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC<T>; ++j)
+            if (j < n) p[j] = v[j];
+    }
+}
+
+// sum over the LPR lanes that hold one row; every one of them gets it
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+#pragma unroll
+    for (int o = 1; o < (LPR < 64 ? LPR : 64); o <<= 1) v += __shfl_xor(v, o);
+    if constexpr (LPR > 64) {
+        __syncthreads();  // (red may still be read from the sum before)
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int w = 0; w < LPR / 64; ++w) v += red[w];
+    }
+    return v;
+}
+
+template <typename T, int LPR, int NV>
+__global__ __launch_bounds__(NT) void k_norm_fwd(const NormP p) {
+    constexpr int V = VEC<T>, RPB = NT / LPR;
+    __shared__ float red[4];
+    const int lr = threadIdx.x % LPR;
+    const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
+    const bool on = row < p.rows;
+    const T* x = (const T*)p.x + row * p.C;
+    float v[NV][V];
+    float s = 0.f;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+        const int col = (c * LPR + lr) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[c][j] = 0.f;
+        if (on && col < p.C) load_chunk<T>(x + col, p.C - col, v[c]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) s += v[c][j];
+    }
+    const float mean = row_sum<LPR>(s, red) / (float)p.C;
+    s = 0.f;
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            v[c][j] -= mean;
+            if ((c * LPR + lr) * V + j < p.C) s = __builtin_fmaf(v[c][j], v[c][j], s);
+        }
+    const float rstd = 1.f / sqrtf(row_sum<LPR>(s, red) / (float)p.C + p.eps);
+    if (!on) return;
+    T* y = (T*)p.y + row * p.C;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+        const int col = (c * LPR + lr) * V;
+        if (col >= p.C) continue;
+        float g[V], b[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) g[j] = 1.f, b[j] = 0.f;
+        if (p.weight) load_chunk<T>((const T*)p.weight + col, p.C - col, g);
+        if (p.bias) load_chunk<T>((const T*)p.bias + col, p.C - col, b);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[c][j] = __builtin_fmaf(v[c][j] * rstd, g[j], b[j]);
+        store_chunk<T>(y + col, p.C - col, v[c]);
+    }
+    if (lr == 0) {
+        p.mean[row] = mean;
+        p.rstd[row] = rstd;
+    }
+}
+
+template <typename T, int LPR, int NV>
+__global__ __launch_bounds__(NT) void k_norm_bwd(const NormP p) {
+    constexpr int V = VEC<T>, RPB = NT / LPR;
+    __shared__ float red[4];
+    __shared__ float part[LPR > 64 ? 1 : 2 * 4 * LPR * V];
+    const int lr = threadIdx.x % LPR;
+    float g[NV][V], dg[NV][V], db[NV][V];
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+        const int col = (c * LPR + lr) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) g[c][j] = 1.f, dg[c][j] = db[c][j] = 0.f;
+        if (p.weight && col < p.C) load_chunk<T>((const T*)p.weight + col, p.C - col, g[c]);
+    }
+    const float inv = 1.f / (float)p.C;
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < p.rows; r0 += (int64_t)gridDim.x * RPB) {  // (workgroup-uniform trip count: row_sum may hold barriers)
+        const int64_t row = r0 + threadIdx.x / LPR;
+        const bool on = row < p.rows;
+        const float mean = on ? p.mean[row] : 0.f, rstd = on ? p.rstd[row] : 0.f;
+        float h[NV][V], a[NV][V], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            const int col = (c * LPR + lr) * V;
+#pragma unroll
+            for (int j = 0; j < V; ++j) h[c][j] = a[c][j] = 0.f;
+            if (on && col < p.C) {
+                load_chunk<T>((const T*)p.x + row * p.C + col, p.C - col, h[c]);
+                load_chunk<T>((const T*)p.d_out + row * p.C + col, p.C - col, a[c]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < NV; ++c)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                h[c][j] = (h[c][j] - mean) * rstd;
+                db[c][j] += a[c][j];
+                dg[c][j] = __builtin_fmaf(a[c][j], h[c][j], dg[c][j]);
+                a[c][j] *= g[c][j];  // (columns past C hold dy = 0: they add nothing)
+                s1 += a[c][j];
+                s2 = __builtin_fmaf(a[c][j], h[c][j], s2);
+            }
+        s1 = row_sum<LPR>(s1, red) * inv;
+        s2 = row_sum<LPR>(s2, red) * inv;
+        if (on && p.dx) {
+#pragma unroll
+            for (int c = 0; c < NV; ++c) {
+                const int col = (c * LPR + lr) * V;
+                if (col >= p.C) continue;
+#pragma unroll
+                for (int j = 0; j < V; ++j) a[c][j] = rstd * (a[c][j] - s1 - h[c][j] * s2);
+                store_chunk<T>((T*)p.dx + row * p.C + col, p.C - col, a[c]);
+            }
+        }
+    }
+    if (!p.part) return;
+    float* pg = p.part + (int64_t)blockIdx.x * 2 * p.C;
+    if constexpr (LPR > 64) {
+#pragma unroll
+        for (int c = 0; c < NV; ++c)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int col = (c * LPR + lr) * V + j;
+                if (col < p.C) {
+                    pg[col] = dg[c][j];
+                    pg[p.C + col] = db[c][j];
+                }
+            }
+    } else {
+        const int wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                float u = dg[c][j], w = db[c][j];
+#pragma unroll
+                for (int o = LPR; o < 64; o <<= 1) {
+                    u += __shfl_xor(u, o);
+                    w += __shfl_xor(w, o);
+                }
+                if ((threadIdx.x & 63) < LPR) {
+                    part[(wave * LPR + lr) * V + j] = u;
+                    part[((4 + wave) * LPR + lr) * V + j] = w;
+                }
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < 2 * LPR * V; i += NT) {
+                const int which = i / (LPR * V), k = i % (LPR * V), col = c * LPR * V + k;
+                if (col < p.C) {
+                    float s = 0.f;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) s += part[(which * 4 + w) * LPR * V + k];
+                    pg[which * p.C + col] = s;
+                }
+            }
+        }
+    }
+}
+
+// dg, db = sum over the workgroups' parts [n][2 C]; 32 columns x 32 rows a workgroup
+template <typename T>
+__global__ __launch_bounds__(1024) void k_norm_sum(const float* part, int n, int C, T* dw, T* db) {
+    __shared__ float s[32][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, col = blockIdx.x * 32 + tx;
+    float v = 0.f;
+    if (col < 2 * C)
+        for (int r = ty; r < n; r += 32) v += part[(int64_t)r * 2 * C + col];
+    s[ty][tx] = v;
+    __syncthreads();
+    if (ty == 0 && col < 2 * C) {
+        v = 0.f;
+#pragma unroll
+        for (int r = 0; r < 32; ++r) v += s[r][tx];
+        T* d = col < C ? dw : db;
+        if (d) d[col < C ? col : col - C] = (T)v;
+    }
+}
+
+typedef void (*Kernel)(NormP);
+struct Shape {
+    Kernel fwd, bwd;
+    int rows;  // per workgroup and step
+};
+template <typename T, int LPR, int NV>
+Shape shape() {
+    return {k_norm_fwd<T, LPR, NV>, k_norm_bwd<T, LPR, NV>, NT / LPR};
+}
+template <typename T>
+Shape choose(int C) {
+    const int n = (C + VEC<T> - 1) / VEC<T>;  // 16-byte chunks of a row
+    if (n <= 8) return shape<T, 8, 1>();
+    if (n <= 16) return shape<T, 16, 1>();
+    if (n <= 32) return shape<T, 32, 1>();
+    if (n <= 64) return shape<T, 64, 1>();
+    if (n <= 128) return shape<T, 64, 2>();
+    if (n <= 256) return shape<T, 64, 4>();
+    if (n <= 512) return shape<T, 256, 2>();
+    if (sizeof(T) == 2 || n <= 1024) return shape<T, 256, 4>();
+    return shape<T, 256, 8>();  // (C <= 8192: a lane's share of a wider row would not fit its registers)
+}
+Shape choose(const NormP& p) { return p.dtype == 1 ? choose<bf16>(p.C) : choose<float>(p.C); }
+int bwd_blocks(const NormP& p) {
+    const int64_t n = (p.rows + choose(p).rows - 1) / choose(p).rows;
+    return (int)(n < 1024 ? n : 1024);
+}
+
+}  // namespace
+
+int64_t norm_workspace(const NormP& p) { return 4 * (int64_t)bwd_blocks(p) * 2 * p.C; }
+
+const char* run_norm(const NormP& p, hipStream_t s) {
+    const Shape h = choose(p);
+    const int64_t blocks = (p.rows + h.rows - 1) / h.rows;
+    if (blocks > 0x7fffffff) return "too many rows";
+    if (blocks) h.fwd<<<dim3((unsigned)blocks), dim3(NT), 0, s>>>(p);
+    return nullptr;
+}
+
+const char* run_norm_backward(NormP p, float* ws, hipStream_t s) {
+    const int n = bwd_blocks(p);
+    p.part = p.dw || p.db ? ws : nullptr;
+    if (n) choose(p).bwd<<<dim3(n), dim3(NT), 0, s>>>(p);
+    if (p.dw || p.db) {  // (no rows: zeros)
+        const dim3 grid((unsigned)((2 * p.C + 31) / 32));
+        if (p.dtype == 1)
+            k_norm_sum<bf16><<<grid, dim3(1024), 0, s>>>(ws, n, p.C, (bf16*)p.dw, (bf16*)p.db);
+        else
+            k_norm_sum<float><<<grid, dim3(1024), 0, s>>>(ws, n, p.C, (float*)p.dw, (float*)p.db);
+    }
+    return nullptr;
+}
+
+}  // namespace op
+}  // namespace tb

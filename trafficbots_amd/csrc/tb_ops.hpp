@@ -1,0 +1,220 @@
+// Shared device code of the training operators (attention, layer norm, Linear): element types, the matrix product of one tile and how
+// an fp32 operand is carried through the bf16 matrix instruction.
+//
+// Operand types.  bf16 operands go into v_mfma_f32_16x16x32_bf16 as they are.  An fp32 operand is carried as THREE bf16 planes,
+// x = b0 + b1 + b2 with b0 = bf16(x), b1 = bf16(x - b0), b2 = bf16(x - b0 - b1) (8 + 8 + 8 significant bits and fp32's exponent range), and a
+// product as the six terms a0 b0 + a0 b1 + a1 b0 + a1 b1 + a0 b2 + a2 b0; what is left out is below 2^-24 |a b|.  Six bf16 instructions
+// take 6 x 16 cycles for a 16 x 16 x 32 tile, the fp32 instruction (16x16x4) eight times 32: 2.7 times less matrix time for the same
+// accuracy, and unlike the fp16 pairs of the rollout kernels no value range to check.  An infinite or NaN fp32 operand makes every
+// result it enters NaN (b1 = inf - inf).
+//
+// Layouts of v_mfma_f32_16x16x32 (lane = 16 g + i): A: row i, k = 8 g + 0..7;  B: column i, k = 8 g + 0..7;  C / D: column i, rows 4 g + 0..3.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace tb {
+namespace op {
+
+typedef __bf16 bf16;
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+template <typename T>
+struct Planes;
+template <>
+struct Planes<bf16> {
+    static constexpr int N = 1;
+};
+template <>
+struct Planes<float> {
+    static constexpr int N = 3;
+};
+
+// one lane's share of an operand of the tile product: 8 values along the contraction, in 1 or 3 planes
+template <int NP>
+struct Frag {
+    bf16x8 p[NP];
+};
+
+template <int NP>
+__device__ __forceinline__ f32x4 mma(const Frag<NP>& a, const Frag<NP>& b, f32x4 c) {
+    if constexpr (NP == 3) {  // small terms first
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[2], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[2], b.p[0], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[1], b.p[1], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[1], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[1], b.p[0], c, 0, 0, 0);
+    }
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[0], c, 0, 0, 0);
+}
+
+// eight fp32 values -> planes (v_cvt_pk_bf16_f32 rounds to nearest even)
+template <int NP>
+__device__ __forceinline__ void to_planes(const float (&x)[8], bf16x8 (&p)[NP]) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        f32x2 r = {x[j], x[j + 1]};
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const bf16x2 h = __builtin_convertvector(r, bf16x2);
+            p[n][j] = h[0];
+            p[n][j + 1] = h[1];
+            if (n + 1 < NP) {
+                r[0] -= (float)h[0];
+                r[1] -= (float)h[1];
+            }
+        }
+    }
+}
+
+// ---- global memory: 8 consecutive elements of a row, the first `n` of them inside it (n >= 8: all).  Rows may start at any element:
+// gfx950 loads 16 bytes from any address, so odd widths and strides take the same path as aligned ones.
+struct Raw8f {
+    float x[8];
+};
+__device__ __forceinline__ void load8(const float* p, int n, float (&x)[8]) {
+    if (n >= 8) {
+        __builtin_memcpy(x, p, 32);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = j < n ? p[j] : 0.f;
+    }
+}
+__device__ __forceinline__ void load8(const bf16* p, int n, float (&x)[8]) {
+    bf16x8 v;
+    if (n >= 8) {
+        __builtin_memcpy(&v, p, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : (bf16)0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = (float)v[j];
+}
+
+// the same 8 elements as they are held between the load and the LDS write of a staged tile: fp32 or packed bf16
+template <typename T>
+struct Held;
+template <>
+struct Held<float> {
+    float x[8];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = 0.f;
+    }
+    __device__ __forceinline__ void load(const float* p, int n) { load8(p, n, x); }
+    __device__ __forceinline__ float get(int j) const { return x[j]; }
+    __device__ __forceinline__ void set(int j, float v) { x[j] = v; }
+    __device__ __forceinline__ void planes(bf16x8 (&p)[3]) const { to_planes<3>(x, p); }
+};
+template <>
+struct Held<bf16> {
+    bf16x8 v;
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (bf16)0.f;
+    }
+    __device__ __forceinline__ void load(const bf16* p, int n) {
+        if (n >= 8) {
+            __builtin_memcpy(&v, p, 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : (bf16)0.f;
+        }
+    }
+    __device__ __forceinline__ float get(int j) const { return (float)v[j]; }
+    __device__ __forceinline__ void set(int j, float f) { v[j] = (bf16)f; }
+    __device__ __forceinline__ void planes(bf16x8 (&p)[1]) const { p[0] = v; }
+};
+
+// 4 consecutive results of a row, the first `n` of them inside it
+__device__ __forceinline__ void store4(float* p, int n, f32x4 v) {
+    if (n >= 4) {
+        __builtin_memcpy(p, &v, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < n) p[j] = v[j];
+    }
+}
+__device__ __forceinline__ void store4(bf16* p, int n, f32x4 v) {
+    const bf16x4 h = __builtin_convertvector(v, bf16x4);
+    if (n >= 4) {
+        __builtin_memcpy(p, &h, 8);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < n) p[j] = h[j];
+    }
+}
+
+// ---- LDS tiles: `NP` planes of [rows][W + 8] bf16.  The 16-byte pad spreads the rows of a 16-byte read over all 64 banks
+// (row strides 80 / 144 / 272 bytes) and keeps them aligned.
+constexpr int LDS_PAD = 8;
+
+// A / B operand whose rows (columns) are the tile's rows and whose contraction runs along them
+template <int NP, int LD>
+__device__ __forceinline__ void frag_rows(const bf16* t, size_t plane, int row0, int k0, int lane, Frag<NP>& f) {
+    const bf16* a = t + (size_t)(row0 + (lane & 15)) * LD + k0 + 8 * (lane >> 4);
+#pragma unroll
+    for (int n = 0; n < NP; ++n) f.p[n] = *reinterpret_cast<const bf16x8*>(a + n * plane);
+}
+
+// A / B operand whose rows (columns) are the tile's COLUMNS c0 .. c0 + 15 and whose contraction runs down the tile's rows:
+// k slots 8 g + 0..3 = tile rows ra + 0..3, 8 g + 4..7 = tile rows rb + 0..3 (ra, rb of this lane's group g).  ds_read_b64_tr_b16: lane i of
+// a 16-lane group hands in row i / 4, columns 4 (i % 4) .. + 3 and receives column i of the group's four rows.
+template <int NP, int LD>
+__device__ __forceinline__ void frag_cols(const bf16* t, size_t plane, int ra, int rb, int c0, int lane, Frag<NP>& f) {
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const int i = lane & 15;
+    const bf16* a = t + (size_t)(ra + (i >> 2)) * LD + c0 + 4 * (i & 3);
+    const bf16* b = t + (size_t)(rb + (i >> 2)) * LD + c0 + 4 * (i & 3);
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + n * plane));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(b + n * plane));
+        const bf16x4 l4 = __builtin_bit_cast(bf16x4, lo), h4 = __builtin_bit_cast(bf16x4, hi);
+        f.p[n] = __builtin_shufflevector(l4, h4, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+}
+
+// all-reduce over the four 16-lane rows of a wave (lanes i, i + 16, i + 32, i + 48) with gfx950's row swaps.  Both registers are
+// read-write operands of the asm: the instruction swaps rows between them in place.  The s_nop's cover the wait states of a VALU write
+// in front of the swap and of the swap in front of a VALU read, which hipcc does not add inside an asm statement.
+__device__ __forceinline__ void swap16(float v, float& lo, float& hi) {
+    float a = v, b = v;
+    asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+    lo = a;
+    hi = b;
+}
+__device__ __forceinline__ void swap32(float v, float& lo, float& hi) {
+    float a = v, b = v;
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+    lo = a;
+    hi = b;
+}
+__device__ __forceinline__ float max_over_groups(float v) {
+    float x, y;
+    swap16(v, x, y);
+    v = fmaxf(x, y);
+    swap32(v, x, y);
+    return fmaxf(x, y);
+}
+__device__ __forceinline__ float sum_over_groups(float v) {
+    float x, y;
+    swap16(v, x, y);
+    v = x + y;
+    swap32(v, x, y);
+    return x + y;
+}
+
+}  // namespace op
+}  // namespace tb

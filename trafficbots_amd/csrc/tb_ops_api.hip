@@ -1,0 +1,200 @@
+// C entry points of the training operators (include/trafficbots_hip.h): arguments checked on the host, then the kernels' launches.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+
+#include "tb_internal.hpp"
+#include "tb_ops_host.hpp"
+
+namespace {
+
+using tb::op::AttnP;
+using tb::op::LinearP;
+using tb::op::NormP;
+
+// the context's device for the time of a call
+struct OnDevice {
+    int prev = -1;
+    hipError_t err;
+    explicit OnDevice(int device) {
+        err = hipGetDevice(&prev);
+        if (err == hipSuccess && prev != device)
+            err = hipSetDevice(device);
+        else
+            prev = -1;
+    }
+    ~OnDevice() {
+        if (prev >= 0) (void)hipSetDevice(prev);
+    }
+};
+
+constexpr int32_t MAX_LEN = 1 << 30;
+
+const char* sizes(const tb_attention_io& io) {
+    if (io.dtype != 0 && io.dtype != 1) return "dtype must be 0 (fp32) or 1 (bf16)";
+    if (io.n_batch < 0 || io.n_query < 0 || io.n_key < 0) return "negative length";
+    if (io.n_query > MAX_LEN || io.n_key > MAX_LEN) return "more than 2^30 queries or keys";
+    if (io.n_head < 1 || io.n_kv_head < 1 || io.n_head % io.n_kv_head) return "n_head must be a positive multiple of n_kv_head";
+    if ((int64_t)io.n_batch * io.n_head > MAX_LEN) return "more than 2^30 heads in the batch";
+    if (io.head_dim < 1 || io.head_dim > 128) return "head_dim must be 1 .. 128";
+    return nullptr;
+}
+const char* sizes(const tb_layer_norm_io& io) {
+    if (io.dtype != 0 && io.dtype != 1) return "dtype must be 0 (fp32) or 1 (bf16)";
+    if (io.n_row < 0 || io.n_row > ((int64_t)1 << 31)) return "n_row must be 0 .. 2^31";
+    if (io.n_col < 1 || io.n_col > 8192) return "n_col must be 1 .. 8192";
+    return nullptr;
+}
+const char* sizes(const tb_linear_io& io) {
+    if (io.dtype != 0 && io.dtype != 1) return "dtype must be 0 (fp32) or 1 (bf16)";
+    if (io.n_row < 0 || io.n_row > ((int64_t)1 << 31)) return "n_row must be 0 .. 2^31";
+    if (io.n_in < 1 || io.n_out < 1 || io.n_in > (1 << 24) || io.n_out > (1 << 24)) return "n_in and n_out must be 1 .. 2^24";
+    if (io.activation != 0 && io.activation != 1) return "activation must be 0 (none) or 1 (ReLU)";
+    return nullptr;
+}
+
+void copy3(int64_t (&dst)[3], const int64_t (&src)[3]) {
+    for (int i = 0; i < 3; ++i) dst[i] = src[i];
+}
+AttnP params(const tb_attention_io& io) {
+    AttnP p = {};
+    p.dtype = io.dtype;
+    p.B = io.n_batch, p.Lq = io.n_query, p.Lk = io.n_key, p.H = io.n_head, p.Hkv = io.n_kv_head, p.G = io.n_head / io.n_kv_head, p.D = io.head_dim;
+    p.causal = io.causal != 0;
+    p.scale = io.scale;
+    p.scale2 = (float)((double)io.scale * 1.4426950408889634);
+    p.q = io.q, p.k = io.k, p.v = io.v, p.out = io.out, p.lse = io.lse, p.d_out = io.d_out, p.dq = io.dq, p.dk = io.dk, p.dv = io.dv;
+    copy3(p.qs, io.q_strides), copy3(p.ks, io.k_strides), copy3(p.vs, io.v_strides), copy3(p.os, io.out_strides), copy3(p.dos, io.d_out_strides);
+    copy3(p.dqs, io.dq_strides), copy3(p.dks, io.dk_strides), copy3(p.dvs, io.dv_strides);
+    p.query_valid = io.query_valid, p.key_valid = io.key_valid, p.mask = io.attn_mask;
+    p.mask_s[0] = io.attn_mask_strides[0], p.mask_s[1] = io.attn_mask_strides[1];
+    return p;
+}
+NormP params(const tb_layer_norm_io& io) {
+    NormP p = {};
+    p.dtype = io.dtype, p.rows = io.n_row, p.C = io.n_col, p.eps = io.eps;
+    p.x = io.x, p.weight = io.weight, p.bias = io.bias, p.d_out = io.d_out, p.y = io.y, p.dx = io.dx, p.dw = io.dweight, p.db = io.dbias;
+    p.mean = io.mean, p.rstd = io.rstd;
+    return p;
+}
+LinearP params(const tb_linear_io& io) {
+    LinearP p = {};
+    p.dtype = io.dtype, p.M = io.n_row, p.N = io.n_out, p.K = io.n_in, p.relu = io.activation == 1;
+    p.x = io.x, p.weight = io.weight, p.bias = io.bias, p.residual = io.residual, p.row_valid = io.row_valid, p.y = io.y;
+    p.d_out = io.d_out, p.dx = io.dx, p.dw = io.dweight, p.db = io.dbias;
+    return p;
+}
+
+template <typename IO>
+const char* scratch(const IO& io, int64_t need) {
+    if (need > 0 && (!io.workspace || io.workspace_bytes < need)) return "workspace missing or smaller than *_workspace_bytes says";
+    if (need > 0 && ((uintptr_t)io.workspace & 15)) return "workspace must be 16-byte aligned";
+    return nullptr;
+}
+
+// runs `body` (an error text or nullptr) on the context's device and turns what went wrong into the library's error
+template <typename F>
+int call(tb_ctx* ctx, const char* name, F&& body) noexcept {
+    try {
+        OnDevice dev(ctx->device);
+        if (dev.err != hipSuccess) return tb_fail(ctx, "%s: %s", name, hipGetErrorString(dev.err));
+        if (const char* e = body()) return tb_fail(ctx, "%s: %s", name, e);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return tb_fail(ctx, "%s: %s", name, hipGetErrorString(e));
+        return 0;
+    } catch (...) {
+        return 1;
+    }
+}
+
+const char* attention_pointers(const tb_attention_io& io, bool backward) {
+    const bool q = io.n_batch && io.n_query, k = io.n_batch && io.n_key;
+    if (!(io.scale > 0.f) || std::isinf(io.scale)) return "scale must be positive and finite";
+    if ((q && (!io.q || !io.out || !io.lse)) || (k && (!io.k || !io.v))) return "a required buffer pointer is NULL";
+    if (backward && ((q && (!io.d_out || !io.dq)) || (k && (!io.dk || !io.dv)))) return "a required buffer pointer is NULL";
+    return nullptr;
+}
+
+}  // namespace
+
+extern "C" void tb_operator_struct_sizes(int32_t out[3]) {
+    out[0] = (int32_t)sizeof(tb_attention_io);
+    out[1] = (int32_t)sizeof(tb_layer_norm_io);
+    out[2] = (int32_t)sizeof(tb_linear_io);
+}
+
+extern "C" int64_t tb_attention_workspace_bytes(const tb_attention_io* io, int32_t backward) {
+    return !io || sizes(*io) ? -1 : tb::op::attention_workspace(params(*io), backward != 0);
+}
+extern "C" int64_t tb_layer_norm_workspace_bytes(const tb_layer_norm_io* io, int32_t backward) {
+    return !io || sizes(*io) ? -1 : backward ? tb::op::norm_workspace(params(*io)) : 0;
+}
+extern "C" int64_t tb_linear_workspace_bytes(const tb_linear_io* io, int32_t backward) {
+    return !io || sizes(*io) ? -1 : backward ? tb::op::linear_workspace(params(*io)) : 0;
+}
+
+extern "C" int tb_attention(tb_ctx* ctx, const tb_attention_io* io, tb_stream stream) {
+    if (!ctx || !io) return 1;
+    return call(ctx, "tb_attention", [&]() -> const char* {
+        if (const char* e = sizes(*io)) return e;
+        if (const char* e = attention_pointers(*io, false)) return e;
+        const AttnP p = params(*io);
+        if (const char* e = scratch(*io, tb::op::attention_workspace(p, false))) return e;
+        return tb::op::run_attention(p, (float*)io->workspace, (hipStream_t)stream);
+    });
+}
+extern "C" int tb_attention_backward(tb_ctx* ctx, const tb_attention_io* io, tb_stream stream) {
+    if (!ctx || !io) return 1;
+    return call(ctx, "tb_attention_backward", [&]() -> const char* {
+        if (const char* e = sizes(*io)) return e;
+        if (const char* e = attention_pointers(*io, true)) return e;
+        const AttnP p = params(*io);
+        if (const char* e = scratch(*io, tb::op::attention_workspace(p, true))) return e;
+        return tb::op::run_attention_backward(p, (float*)io->workspace, (hipStream_t)stream);
+    });
+}
+
+extern "C" int tb_layer_norm(tb_ctx* ctx, const tb_layer_norm_io* io, tb_stream stream) {
+    if (!ctx || !io) return 1;
+    return call(ctx, "tb_layer_norm", [&]() -> const char* {
+        if (const char* e = sizes(*io)) return e;
+        if (!(io->eps >= 0.f)) return "eps must not be negative";
+        if (io->n_row && (!io->x || !io->y || !io->mean || !io->rstd)) return "a required buffer pointer is NULL";
+        return tb::op::run_norm(params(*io), (hipStream_t)stream);
+    });
+}
+extern "C" int tb_layer_norm_backward(tb_ctx* ctx, const tb_layer_norm_io* io, tb_stream stream) {
+    if (!ctx || !io) return 1;
+    return call(ctx, "tb_layer_norm_backward", [&]() -> const char* {
+        if (const char* e = sizes(*io)) return e;
+        if (io->n_row && (!io->x || !io->d_out || !io->mean || !io->rstd)) return "a required buffer pointer is NULL";
+        const NormP p = params(*io);
+        if (io->dweight || io->dbias)
+            if (const char* e = scratch(*io, tb::op::norm_workspace(p))) return e;
+        return tb::op::run_norm_backward(p, (float*)io->workspace, (hipStream_t)stream);
+    });
+}
+
+extern "C" int tb_linear(tb_ctx* ctx, const tb_linear_io* io, tb_stream stream) {
+    if (!ctx || !io) return 1;
+    return call(ctx, "tb_linear", [&]() -> const char* {
+        if (const char* e = sizes(*io)) return e;
+        if (!io->weight || (io->n_row && (!io->x || !io->y))) return "a required buffer pointer is NULL";
+        LinearP p = params(*io);
+        p.act_out = io->act;
+        return tb::op::run_linear(p, (hipStream_t)stream);
+    });
+}
+extern "C" int tb_linear_backward(tb_ctx* ctx, const tb_linear_io* io, tb_stream stream) {
+    if (!ctx || !io) return 1;
+    return call(ctx, "tb_linear_backward", [&]() -> const char* {
+        if (const char* e = sizes(*io)) return e;
+        if ((io->dx && !io->weight) || (io->n_row && (!io->d_out || (io->dweight && !io->x)))) return "a required buffer pointer is NULL";
+        if (io->activation == 1 && io->n_row && !io->act) return "ReLU's gradient needs act (what tb_linear wrote there)";
+        LinearP p = params(*io);
+        p.act = io->activation == 1 ? io->act : nullptr;
+        if (io->dweight || io->dbias)
+            if (const char* e = scratch(*io, tb::op::linear_workspace(p))) return e;
+        return tb::op::run_linear_backward(p, (float*)io->workspace, (hipStream_t)stream);
+    });
+}

@@ -1,0 +1,59 @@
+// Launch parameters of the training operators, shared by the kernels' files and the C entry points (tb_ops_api.hip).
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace tb {
+namespace op {
+
+struct AttnP {
+    int dtype;  // 0 fp32, 1 bf16
+    int B, Lq, Lk, H, Hkv, G, D, causal;
+    float scale, scale2;  // scale2 = scale * log2(e): the softmax works in powers of two
+    const void *q, *k, *v, *d_out;
+    int64_t qs[3], ks[3], vs[3], os[3], dos[3], dqs[3], dks[3], dvs[3];  // elements over (batch, position, head)
+    const uint8_t *query_valid, *key_valid, *mask;
+    int64_t mask_s[2];  // bytes over (batch, query)
+    void *out, *dq, *dk, *dv;
+    float *lse, *delta;
+    // of one launch
+    int n_col_tile, n_split, split_len, xcd;
+    float *part, *part_lse;
+};
+int64_t attention_workspace(const AttnP& p, bool backward);
+const char* run_attention(AttnP p, float* ws, hipStream_t s);
+const char* run_attention_backward(AttnP p, float* ws, hipStream_t s);
+
+struct NormP {
+    int dtype;  // 0 fp32, 1 bf16
+    int64_t rows;
+    int C;
+    float eps;
+    const void *x, *weight, *bias, *d_out;
+    void *y, *dx, *dw, *db;
+    float *mean, *rstd;
+    float* part;  // of one launch: [workgroups][2 C]
+};
+int64_t norm_workspace(const NormP& p);
+const char* run_norm(const NormP& p, hipStream_t s);
+const char* run_norm_backward(NormP p, float* ws, hipStream_t s);
+
+struct LinearP {
+    int dtype;  // 0 fp32, 1 bf16
+    int64_t M;
+    int N, K, relu;
+    const void *x, *weight, *bias, *residual, *act, *d_out;
+    const uint8_t* row_valid;
+    void *y, *act_out, *dx, *dw, *db;
+    // of one launch
+    int n_rt, n_split;
+    int64_t n_ct, split_len;
+    float* part;  // [n_split][N][K], then [n_split][N]
+};
+int64_t linear_workspace(const LinearP& p);
+const char* run_linear(const LinearP& p, hipStream_t s);
+const char* run_linear_backward(LinearP p, float* ws, hipStream_t s);
+
+}  // namespace op
+}  // namespace tb

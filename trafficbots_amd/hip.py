@@ -165,12 +165,46 @@ class TbTrainIO(C.Structure):
     ]
 
 
+class TbAttentionIO(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("n_batch", C.c_int32), ("n_query", C.c_int32), ("n_key", C.c_int32), ("n_head", C.c_int32),
+        ("n_kv_head", C.c_int32), ("head_dim", C.c_int32), ("causal", C.c_int32), ("scale", C.c_float),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("q_strides", C.c_int64 * 3), ("k_strides", C.c_int64 * 3), ("v_strides", C.c_int64 * 3),
+        ("query_valid", C.c_void_p), ("key_valid", C.c_void_p), ("attn_mask", C.c_void_p), ("attn_mask_strides", C.c_int64 * 2),
+        ("out", C.c_void_p), ("out_strides", C.c_int64 * 3), ("lse", C.c_void_p),
+        ("d_out", C.c_void_p), ("d_out_strides", C.c_int64 * 3), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p),
+        ("dq_strides", C.c_int64 * 3), ("dk_strides", C.c_int64 * 3), ("dv_strides", C.c_int64 * 3),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
+class TbLayerNormIO(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("n_col", C.c_int32), ("n_row", C.c_int64), ("eps", C.c_float),
+        ("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("y", C.c_void_p), ("mean", C.c_void_p), ("rstd", C.c_void_p),
+        ("d_out", C.c_void_p), ("dx", C.c_void_p), ("dweight", C.c_void_p), ("dbias", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
+class TbLinearIO(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("n_in", C.c_int32), ("n_out", C.c_int32), ("activation", C.c_int32), ("n_row", C.c_int64),
+        ("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("row_valid", C.c_void_p), ("residual", C.c_void_p),
+        ("y", C.c_void_p), ("act", C.c_void_p), ("d_out", C.c_void_p), ("dx", C.c_void_p), ("dweight", C.c_void_p), ("dbias", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
 EXPORTS = (
     "tb_create", "tb_destroy", "tb_last_error", "tb_version", "tb_load_weight", "tb_finalize_weights",
     "tb_rollout", "tb_rollout_begin", "tb_rollout_step", "tb_rollout_step_ex", "tb_check_status", "tb_rollout_state", "tb_encode_scene", "tb_set_timing", "tb_get_timing",
     "tb_rule_checks", "tb_post_process", "tb_metric_partials", "tb_struct_sizes", "tb_encode_posterior", "tb_train_partials",
     "tb_forward", "tb_graph_stats", "tb_latent_sample", "tb_dest_sample", "tb_precision_state", "tb_precision_note", "tb_precision_restore",
     "tb_host_onehot_index",
+    "tb_attention", "tb_attention_backward", "tb_attention_workspace_bytes", "tb_layer_norm", "tb_layer_norm_backward",
+    "tb_layer_norm_workspace_bytes", "tb_linear", "tb_linear_backward", "tb_linear_workspace_bytes", "tb_operator_struct_sizes",
 )
 
 _lib: Optional[C.CDLL] = None
@@ -294,6 +328,18 @@ def load() -> C.CDLL:
     lib.tb_forward.restype = C.c_int
     if list(sizes) != mine:
         raise RuntimeError(f"trafficbots_amd: ctypes struct layouts {mine} do not match the library's {list(sizes)} (stale build?)")
+    sizes = (C.c_int32 * 3)()
+    lib.tb_operator_struct_sizes.argtypes = [C.POINTER(C.c_int32)]
+    lib.tb_operator_struct_sizes.restype = None
+    lib.tb_operator_struct_sizes(sizes)
+    mine = [C.sizeof(x) for x in (TbAttentionIO, TbLayerNormIO, TbLinearIO)]
+    if list(sizes) != mine:
+        raise RuntimeError(f"trafficbots_amd: ctypes struct layouts {mine} do not match the library's {list(sizes)} (stale build?)")
+    for name, io in (("tb_attention", TbAttentionIO), ("tb_layer_norm", TbLayerNormIO), ("tb_linear", TbLinearIO)):
+        for f in (getattr(lib, name), getattr(lib, name + "_backward")):
+            f.argtypes, f.restype = [C.c_void_p, C.POINTER(io), C.c_void_p], C.c_int
+        f = getattr(lib, name + "_workspace_bytes")
+        f.argtypes, f.restype = [C.POINTER(io), C.c_int32], C.c_int64
     lib.tb_precision_state.argtypes = [C.c_void_p, C.POINTER(C.c_int32)]
     lib.tb_precision_state.restype = C.c_int
     lib.tb_precision_note.argtypes = [C.c_void_p]

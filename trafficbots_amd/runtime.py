@@ -880,6 +880,214 @@ class HipEngine:
                                       hip.ptr(st["hidden"], hip.c_f32p), self._stream()), "tb_rollout_state")
         return st
 
+    # -------------------------------------------------------------------------------- training operators of a transformer layer
+    def _dtype(self, what: str, *tensors: Optional[Tensor]) -> int:
+        """0 fp32, 1 bf16 (`tb_*_io.dtype`): all tensors of a call share one type and live on this engine's device."""
+        t0 = tensors[0].dtype
+        if t0 not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"{what}: float32 or bfloat16 expected, got {t0}")
+        for t in tensors:
+            if t is None:
+                continue
+            if t.dtype != t0:
+                raise ValueError(f"{what}: all tensors must have one type, got {t0} and {t.dtype}")
+            if t.device != self.device:
+                raise ValueError(f"{what}: tensor on {t.device}, the engine's device is {self.device}")
+        return int(t0 == torch.bfloat16)
+
+    def _mask(self, what: str, name: str, m: Optional[Tensor], *shapes) -> Optional[Tensor]:
+        """A bool / uint8 mask of one of the shapes, as uint8."""
+        if m is None:
+            return None
+        if tuple(m.shape) not in shapes:
+            raise ValueError(f"{what}: {name} has shape {tuple(m.shape)}, expected {' or '.join(str(s) for s in shapes)}")
+        if m.dtype not in (torch.bool, torch.uint8):
+            raise ValueError(f"{what}: {name} must be bool or uint8, got {m.dtype}")
+        if m.device != self.device:
+            raise ValueError(f"{what}: {name} on {m.device}, the engine's device is {self.device}")
+        return m.view(torch.uint8) if m.dtype == torch.bool else m
+
+    def _scratch(self, n_bytes: int) -> Optional[Tensor]:
+        return torch.empty(n_bytes, device=self.device, dtype=torch.uint8) if n_bytes > 0 else None
+
+    def _attention_io(self, what: str, q: Tensor, k: Tensor, v: Tensor, query_valid, key_valid, attn_mask, causal: bool, scale, *more: Tensor):
+        for name, t in (("q", q), ("k", k), ("v", v)):
+            if t.dim() != 4:
+                raise ValueError(f"{what}: {name} must be [batch, length, heads, head_dim], got {tuple(t.shape)}")
+        b, lq, h, d = q.shape
+        lk, hkv = k.shape[1], k.shape[2]
+        if tuple(k.shape) != (b, lk, hkv, d) or k.shape != v.shape:
+            raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+        io = hip.TbAttentionIO()
+        io.dtype = self._dtype(what, q, k, v, *more)
+        io.n_batch, io.n_query, io.n_key, io.n_head, io.n_kv_head, io.head_dim = b, lq, lk, h, hkv, d
+        io.causal, io.scale = int(bool(causal)), 1.0 / d**0.5 if scale is None else float(scale)
+        qv, kv = self._mask(what, "query_valid", query_valid, (b, lq)), self._mask(what, "key_valid", key_valid, (b, lk))
+        qv, kv = (None if m is None else m.contiguous() for m in (qv, kv))
+        am = self._mask(what, "attn_mask", attn_mask, (lq, lk), (b, lq, lk))
+        if am is not None:
+            if lk > 1 and am.stride(-1) != 1:
+                am = am.contiguous()
+            io.attn_mask_strides[0] = am.stride(0) if am.dim() == 3 else 0
+            io.attn_mask_strides[1] = am.stride(-2)
+        io.query_valid, io.key_valid, io.attn_mask = (None if m is None else m.data_ptr() for m in (qv, kv, am))
+        keep = [qv, kv, am]
+        for name, t in (("q", q), ("k", k), ("v", v)):
+            keep.append(self._strided(io, name, t))
+        return io, keep
+
+    @staticmethod
+    def _strided(io, name: str, t: Tensor) -> Tensor:
+        """A [batch, length, heads, head_dim] tensor where it lies; only the components must be adjacent."""
+        if t.shape[3] > 1 and t.stride(3) != 1:
+            t = t.contiguous()
+        setattr(io, name, t.data_ptr())
+        st = getattr(io, name + "_strides")
+        st[0], st[1], st[2] = t.stride(0), t.stride(1), t.stride(2)
+        return t
+
+    def attention(self, q: Tensor, k: Tensor, v: Tensor, query_valid: Optional[Tensor] = None, key_valid: Optional[Tensor] = None,
+                  attn_mask: Optional[Tensor] = None, causal: bool = False, scale: Optional[float] = None) -> Tuple[Tensor, Tensor]:
+        """`tb_attention`: attention of q [B, Lq, H, D] over k, v [B, Lk, Hkv, D] (H a multiple of Hkv, D <= 128; fp32 or bf16; strided
+        tensors are read where they lie).  `query_valid` [B, Lq] / `key_valid` [B, Lk]: what their zeros mark is not looked at.
+        `attn_mask` [Lq, Lk] or [B, Lq, Lk]: True = may NOT attend (`attention.py:90-99`).  `causal`: key j for queries i >= j + Lq - Lk.
+        `scale` defaults to 1 / sqrt(D).  Returns (out [B, Lq, H, D], lse [B, H, Lq] fp32); a query without a key gets 0 and -inf."""
+        io, keep = self._attention_io("attention", q, k, v, query_valid, key_valid, attn_mask, causal, scale)
+        out = torch.empty(q.shape, device=self.device, dtype=q.dtype)
+        lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], device=self.device, dtype=torch.float32)
+        keep.append(self._strided(io, "out", out))
+        io.lse = lse.data_ptr()
+        self._run("tb_attention", io, False)
+        return out, lse
+
+    def attention_backward(self, d_out: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, query_valid: Optional[Tensor] = None,
+                           key_valid: Optional[Tensor] = None, attn_mask: Optional[Tensor] = None, causal: bool = False,
+                           scale: Optional[float] = None) -> Tuple[Tensor, Tensor, Tensor]:
+        """`tb_attention_backward`: (dq, dk, dv) from `d_out` [B, Lq, H, D] and what :meth:`attention` returned for the same arguments.  The
+        gradients of key / value heads that several query heads share are summed over those."""
+        io, keep = self._attention_io("attention_backward", q, k, v, query_valid, key_valid, attn_mask, causal, scale, d_out, out)
+        if d_out.shape != q.shape or out.shape != q.shape:
+            raise ValueError(f"attention_backward: d_out {tuple(d_out.shape)} and out {tuple(out.shape)} must have q's shape {tuple(q.shape)}")
+        lse = self._f32("attention_backward", "lse", lse, (q.shape[0], q.shape[2], q.shape[1]))
+        dq, dk, dv = (torch.empty(t.shape, device=self.device, dtype=t.dtype) for t in (q, k, v))
+        for name, t in (("out", out), ("d_out", d_out), ("dq", dq), ("dk", dk), ("dv", dv)):
+            keep.append(self._strided(io, name, t))
+        io.lse = lse.data_ptr()
+        self._run("tb_attention_backward", io, True)
+        return dq, dk, dv
+
+    def _f32(self, what: str, name: str, t: Tensor, shape) -> Tensor:
+        if tuple(t.shape) != tuple(shape) or t.dtype != torch.float32 or t.device != self.device:
+            raise ValueError(f"{what}: {name} must be float32 {tuple(shape)} on {self.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        return t.contiguous()
+
+    def _run(self, name: str, io, backward: bool) -> None:
+        """One call of a training operator on the current stream; its scratch lives on that stream, in torch's allocator."""
+        need = getattr(self.lib, name.replace("_backward", "") + "_workspace_bytes")(C.byref(io), int(backward))
+        ws = self._scratch(need)
+        if ws is not None:
+            io.workspace, io.workspace_bytes = ws.data_ptr(), need
+        self._check(getattr(self.lib, name)(self._ctx, C.byref(io), self._stream()), name)
+
+    def layer_norm(self, x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5
+                   ) -> Tuple[Tensor, Tensor, Tensor]:
+        """`tb_layer_norm` over the last axis of x [..., C] (C <= 8192; fp32 or bf16): (y [..., C], mean [...], rstd [...], both fp32)."""
+        io, x, keep = self._norm_io("layer_norm", x, weight, bias)
+        y = torch.empty(x.shape, device=self.device, dtype=x.dtype)
+        mean, rstd = (torch.empty(x.shape[:-1], device=self.device, dtype=torch.float32) for _ in range(2))
+        io.eps, io.y, io.mean, io.rstd = float(eps), y.data_ptr(), mean.data_ptr(), rstd.data_ptr()
+        self._run("tb_layer_norm", io, False)
+        return y, mean, rstd
+
+    def layer_norm_backward(self, d_out: Tensor, x: Tensor, weight: Optional[Tensor], mean: Tensor, rstd: Tensor, want_dx: bool = True,
+                            want_dweight: bool = True) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
+        """`tb_layer_norm_backward`: (dx, dweight, dbias) from `d_out` and what :meth:`layer_norm` returned."""
+        what = "layer_norm_backward"
+        io, x, keep = self._norm_io(what, x, weight, None, d_out)
+        if d_out.shape != x.shape:
+            raise ValueError(f"{what}: d_out {tuple(d_out.shape)} must have x's shape {tuple(x.shape)}")
+        d_out = d_out.contiguous()
+        mean, rstd = self._f32(what, "mean", mean, x.shape[:-1]), self._f32(what, "rstd", rstd, x.shape[:-1])
+        dx = torch.empty(x.shape, device=self.device, dtype=x.dtype) if want_dx else None
+        dw, db = (torch.empty(x.shape[-1], device=self.device, dtype=x.dtype) if want_dweight else None for _ in range(2))
+        io.d_out, io.mean, io.rstd = d_out.data_ptr(), mean.data_ptr(), rstd.data_ptr()
+        io.dx, io.dweight, io.dbias = (None if t is None else t.data_ptr() for t in (dx, dw, db))
+        self._run("tb_layer_norm_backward", io, True)
+        return dx, dw, db
+
+    def _norm_io(self, what: str, x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], *more: Tensor):
+        io = hip.TbLayerNormIO()
+        io.dtype = self._dtype(what, x, weight, bias, *more)
+        if x.dim() < 1:
+            raise ValueError(f"{what}: x has no axis")
+        for name, t in (("weight", weight), ("bias", bias)):
+            if t is not None and tuple(t.shape) != (x.shape[-1],):
+                raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected ({x.shape[-1]},)")
+        x, weight, bias = (None if t is None else t.contiguous() for t in (x, weight, bias))
+        io.n_col = x.shape[-1]
+        io.n_row = x.numel() // max(1, io.n_col)
+        io.x, io.weight, io.bias = (None if t is None else t.data_ptr() for t in (x, weight, bias))
+        return io, x, [weight, bias]
+
+    def linear(self, x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: Optional[str] = None, row_valid: Optional[Tensor] = None,
+               residual: Optional[Tensor] = None, want_act: bool = False):
+        """`tb_linear`: act(x weight^T + bias), 0 where `row_valid` is 0, + residual, for x [..., n_in], weight [n_out, n_in], row_valid
+        [...], residual [..., n_out] (fp32 or bf16); `activation` None or "relu".  Returns y [..., n_out]; with `want_act` (y, a), a = what
+        :meth:`linear_backward` needs for ReLU: the value in front of the residual (y itself where there is none)."""
+        what = "linear"
+        io, x, keep = self._linear_io(what, x, weight, bias, activation, row_valid, residual)
+        shape = tuple(x.shape[:-1]) + (weight.shape[0],)
+        if residual is not None:
+            if tuple(residual.shape) != shape:
+                raise ValueError(f"{what}: residual has shape {tuple(residual.shape)}, expected {shape}")
+            residual = residual.contiguous()
+            io.residual = residual.data_ptr()
+        y = torch.empty(shape, device=self.device, dtype=x.dtype)
+        io.y = y.data_ptr()
+        act = y
+        if want_act and residual is not None:
+            act = torch.empty(shape, device=self.device, dtype=x.dtype)
+            io.act = act.data_ptr()
+        self._run("tb_linear", io, False)
+        return (y, act) if want_act else y
+
+    def linear_backward(self, d_out: Tensor, x: Tensor, weight: Tensor, act: Optional[Tensor] = None, row_valid: Optional[Tensor] = None,
+                        want_dx: bool = True, want_dweight: bool = True, want_dbias: bool = True
+                        ) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
+        """`tb_linear_backward`: (dx, dweight, dbias) from `d_out` [..., n_out]; `act`: ReLU's output as :meth:`linear` returned it, None for a
+        call without activation.  The residual's gradient is `d_out`."""
+        what = "linear_backward"
+        io, x, keep = self._linear_io(what, x, weight, None, None if act is None else "relu", row_valid, d_out, act)
+        shape = tuple(x.shape[:-1]) + (weight.shape[0],)
+        for name, t in (("d_out", d_out), ("act", act)):
+            if t is not None and tuple(t.shape) != shape:
+                raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {shape}")
+        d_out, act = d_out.contiguous(), None if act is None else act.contiguous()
+        dx = torch.empty(x.shape, device=self.device, dtype=x.dtype) if want_dx else None
+        dw = torch.empty(weight.shape, device=self.device, dtype=x.dtype) if want_dweight else None
+        db = torch.empty(weight.shape[0], device=self.device, dtype=x.dtype) if want_dbias else None
+        io.d_out, io.act = d_out.data_ptr(), None if act is None else act.data_ptr()
+        io.dx, io.dweight, io.dbias = (None if t is None else t.data_ptr() for t in (dx, dw, db))
+        self._run("tb_linear_backward", io, True)
+        return dx, dw, db
+
+    def _linear_io(self, what: str, x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: Optional[str], row_valid: Optional[Tensor],
+                   *more: Optional[Tensor]):
+        if activation not in (None, "relu"):
+            raise ValueError(f"{what}: activation must be None or 'relu', got {activation!r}")
+        io = hip.TbLinearIO()
+        io.dtype = self._dtype(what, x, weight, bias, *more)
+        if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+            raise ValueError(f"{what}: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit together")
+        if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+            raise ValueError(f"{what}: bias has shape {tuple(bias.shape)}, expected ({weight.shape[0]},)")
+        rv = self._mask(what, "row_valid", row_valid, tuple(x.shape[:-1]))
+        x, weight, bias, rv = (None if t is None else t.contiguous() for t in (x, weight, bias, rv))
+        io.n_in, io.n_out, io.activation = weight.shape[1], weight.shape[0], int(activation == "relu")
+        io.n_row = x.numel() // max(1, io.n_in)
+        io.x, io.weight, io.bias, io.row_valid = (None if t is None else t.data_ptr() for t in (x, weight, bias, rv))
+        return io, x, [weight, bias, rv]
+
     # -------------------------------------------------------------------------------- timing
     def set_timing(self, enable: bool) -> None:
         self._check(self.lib.tb_set_timing(self._ctx, int(enable)), "tb_set_timing")
