@@ -6,4 +6,12 @@ sfx="$1"; shift
 SRC=$(python3 -c "import sys; sys.path.insert(0, '../..'); import __graft_entry__ as g; print(' '.join(g.SOURCES))")
 # flags: toolchain.json (TB_DROP_FLAGS="-amdgpu-sched-strategy=max-ilp" etc. remove entries for A/B builds)
 FLAGS=$(python3 -c "import sys; sys.path.insert(0, '../..'); import __graft_entry__ as g; print(' '.join(g.FLAGS))")
-/opt/rocm/bin/hipcc $FLAGS -shared "$@" -o ../lib/libtrafficbots_hip${sfx}.so $SRC
+OBJ=""
+mkdir -p "build$sfx"
+for f in $SRC; do
+  UNIT=$(python3 -c "import sys; sys.path.insert(0, '../..'); import __graft_entry__ as g; print(' '.join(g.unit_flags('$f')))")
+  /opt/rocm/bin/hipcc $FLAGS $UNIT "$@" -c "$f" -o "build$sfx/${f%.hip}.o" &
+  OBJ="$OBJ build$sfx/${f%.hip}.o"
+done
+for j in $(jobs -p); do wait $j; done
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -fPIC -shared -o ../lib/libtrafficbots_hip${sfx}.so $OBJ
