@@ -558,7 +558,7 @@ int tb_dest_sample(tb_ctx* ctx, const tb_dest_sample_io* io, tb_stream stream);
  * gradients are 0; keys that only attn_mask or `causal` hide must hold finite values.  n_batch, n_query and n_key may be 0.
  * Replaces: the products, masks and softmax of Attention.forward (attention.py:90-141) between its in- and out-projection. */
 typedef struct tb_attention_io {
-    int32_t dtype, n_batch, n_query, n_key, n_head, n_kv_head, head_dim; /* 1 <= head_dim <= 128; n_head a multiple of n_kv_head */
+    int32_t dtype, n_batch, n_query, n_key, n_head, n_kv_head, head_dim; /* 8 <= head_dim <= 128; n_head a multiple of n_kv_head */
     int32_t causal;
     float scale;                  /* > 0, usually 1 / sqrt(head_dim) */
     /* [n_batch, n_query | n_key, n_head | n_kv_head, head_dim], components adjacent; strides in elements over (batch, position, head) */

@@ -61,7 +61,7 @@ def test_workspace_sizes_refuse_what_the_operators_refuse():
     assert attention(n_query=1, n_key=1 << 16)[0] > 0  # one query over a long cache: the walk is split
     assert attention(n_query=0) == (0, 0) and attention(n_batch=0) == (0, 0) and attention(n_key=0)[0] == 0
     for bad in (dict(dtype=2), dict(dtype=-1), dict(n_batch=-1), dict(n_query=-1), dict(n_key=-1), dict(n_head=0), dict(n_kv_head=0), dict(n_kv_head=3),
-                dict(n_head=2, n_kv_head=4), dict(head_dim=0), dict(head_dim=129), dict(n_query=(1 << 30) + 1), dict(n_batch=1 << 29)):
+                dict(n_head=2, n_kv_head=4), dict(head_dim=7), dict(head_dim=129), dict(n_query=(1 << 30) + 1), dict(n_batch=1 << 29)):
         assert attention(**bad) == (-1, -1), bad
 
     def norm(**kw):
@@ -238,8 +238,8 @@ def _check_attention(eng, q, k, v, do, kw, ref=None):
 @gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("b,lq,lk,h,hkv,d", [
-    (1, 1, 1, 1, 1, 1), (2, 1, 33, 4, 4, 32), (3, 20, 20, 4, 4, 32), (2, 64, 256, 4, 4, 32), (2, 61, 61, 4, 2, 32), (1, 130, 67, 8, 2, 64),
-    (2, 17, 300, 3, 1, 40), (1, 33, 31, 2, 2, 128), (1, 200, 200, 4, 1, 72), (2, 65, 129, 2, 2, 7), (1, 16, 32, 2, 1, 96), (1, 257, 15, 1, 1, 100),
+    (1, 1, 1, 1, 1, 8), (2, 1, 33, 4, 4, 32), (3, 20, 20, 4, 4, 32), (2, 64, 256, 4, 4, 32), (2, 61, 61, 4, 2, 32), (1, 130, 67, 8, 2, 64),
+    (2, 17, 300, 3, 1, 40), (1, 33, 31, 2, 2, 128), (1, 200, 200, 4, 1, 72), (2, 65, 129, 2, 2, 9), (1, 16, 32, 2, 1, 96), (1, 257, 15, 1, 1, 100),
 ])
 def test_attention_sizes(eng, dtype, b, lq, lk, h, hkv, d):
     _check_attention(eng, *_attention_inputs(b, lq, lk, h, hkv, d, dtype, seed=lq + lk))
@@ -636,7 +636,8 @@ def test_the_current_device_and_the_library_errors(eng):
     from trafficbots_amd import hip
 
     io = hip.TbAttentionIO()
-    io.n_batch = io.n_query = io.n_key = io.n_head = io.n_kv_head = io.head_dim = 1
+    io.n_batch = io.n_query = io.n_key = io.n_head = io.n_kv_head = 1
+    io.head_dim = 8
     io.scale = 1.0
     assert eng.lib.tb_attention(eng._ctx, C.byref(io), None) != 0 and b"NULL" in eng.lib.tb_last_error(eng._ctx)
     io.n_key, io.n_head, io.n_kv_head = 1 << 16, 1, 1

@@ -20,62 +20,80 @@ namespace {
 
 constexpr float NEG_INF = -__builtin_inff();
 
-// workgroup -> (row of the (batch, head) list, tile of the columns x split).  Workgroups go to the eight XCDs round robin; with
-// `xcd` all tiles of one (batch, head) land on the same XCD, whose L2 then holds its keys and values once.
-__device__ __forceinline__ bool decode(unsigned id, int n_inner, int n_bh, int xcd, int& bh, int& inner) {
-    if (xcd) {
-        const unsigned lo = id & 7u, r = id >> 3;
-        inner = (int)(r % (unsigned)n_inner);
-        bh = (int)(r / (unsigned)n_inner) * 8 + (int)lo;
-    } else {
-        inner = (int)(id % (unsigned)n_inner);
-        bh = (int)(id / (unsigned)n_inner);
+// Workgroup -> (row of the (batch, head) list, split, column tile).  Workgroups go to the eight XCDs round robin.  By default each XCD takes a
+// contiguous part of the list, the tiles of one (batch, head) next to each other, so that its L2 holds their keys and values once.
+// `tile_major` (causal with few heads: the walks' lengths differ and all of them are in flight at once): the longest walks of every
+// (batch, head) first, and a (batch, head) still meets one XCD if their number is a multiple of eight.
+__device__ __forceinline__ bool decode(const AttnP& p, int n_bh, int& bh, int& split, int& tile) {
+    const unsigned id = blockIdx.x;
+    if (p.tile_major) {
+        const unsigned n = (unsigned)n_bh * p.n_split, c = id % n;
+        tile = (int)(id / n);
+        bh = (int)(c % (unsigned)n_bh);
+        split = (int)(c / (unsigned)n_bh);
+        return true;
     }
-    return bh < n_bh;
+    const unsigned n_inner = (unsigned)p.n_col_tile * p.n_split, total = n_inner * (unsigned)n_bh, per = (total + 7) / 8, t = (id & 7u) * per + (id >> 3);
+    const unsigned inner = t % n_inner;
+    bh = (int)(t / n_inner);
+    split = (int)(inner / (unsigned)p.n_col_tile);
+    tile = (int)(inner % (unsigned)p.n_col_tile);
+    return (id >> 3) < per && t < total;
 }
 
 // A tile of KT rows x D columns on its way from global memory to LDS: every thread holds PT chunks of 8 elements.
 template <typename T, int DP, int NT, int KT>
 struct Stage {
-    static constexpr int NP = Planes<T>::N, CH = DP / 8, PT = (KT * CH + NT - 1) / NT, LD = DP + LDS_PAD;
+    static constexpr int NP = Planes<T>::N, CH = DP / 8, PT = KT * CH / NT, LD = DP + LDS_PAD;
+    static_assert(KT * CH % NT == 0, "whole chunks per thread");
     Held<T> r[PT];
-    // rows row0 .. row0 + KT - 1 of `base` (row stride `ld`); a row outside [0, end) or marked invalid becomes zero, whatever it holds
-    __device__ __forceinline__ void load(const T* base, int64_t ld, const uint8_t* valid, int row0, int end, int D, int tid) {
+    uint8_t ok[PT];
+    int rows;
+    // rows row0 .. row0 + KT - 1 (row0 < end) of `base` (row stride `ld`); a row from `end` on or marked invalid becomes zero, whatever it holds
+    __device__ __forceinline__ void load(const AttnP& p, const T* base, int64_t ld, const Valid& valid, int row0, int end, int tid) {
 #pragma unroll
         for (int c = 0; c < PT; ++c) {
-            const int idx = tid + c * NT, row = row0 + idx / CH, col = (idx % CH) * 8;
-            r[c].zero();
-            if (idx < KT * CH && row < end && col < D) {
-                r[c].load(base + (int64_t)row * ld + col, D - col);
-                if (valid && !valid[row]) r[c].zero();
-            }
+            const int idx = tid + c * NT, rc = min(row0 + idx / CH, end - 1);
+            r[c].load(base + (int64_t)rc * ld + chunk_start((idx % CH) * 8, p.D));
+            ok[c] = valid[rc];
         }
+        rows = end - row0;
     }
-    __device__ __forceinline__ void store(bf16* lds, int tid) const {
+    // into LDS, and (unless null) `bias` = 0 for the rows that are there, -inf for the others
+    __device__ __forceinline__ void store(const AttnP& p, bf16* lds, float* bias, int tid) {
 #pragma unroll
         for (int c = 0; c < PT; ++c) {
-            const int idx = tid + c * NT;
-            if (KT * CH % NT == 0 || idx < KT * CH) {
-                bf16x8 pl[NP];
-                r[c].planes(pl);
+            const int idx = tid + c * NT, col = (idx % CH) * 8;
+            const bool on = ok[c] && idx / CH < rows;
+            if (p.ragged) r[c].fit(col - chunk_start(col, p.D));
+            r[c].keep(on && col < p.D);
+            bf16x8 pl[NP];
+            r[c].planes(pl);
 #pragma unroll
-                for (int n = 0; n < NP; ++n) *reinterpret_cast<bf16x8*>(lds + (size_t)n * KT * LD + (idx / CH) * LD + (idx % CH) * 8) = pl[n];
-            }
+            for (int n = 0; n < NP; ++n) *reinterpret_cast<bf16x8*>(lds + (size_t)n * KT * LD + (idx / CH) * LD + col) = pl[n];
+            if (bias && col == 0) bias[idx / CH] = on ? 0.f : NEG_INF;
         }
     }
 };
 
-// B operand of 16 columns: column i = row `row` of a [., D] matrix in global memory (zero where not `on`)
+// B operand of 16 columns: column i = row `row` of a [., D] matrix in global memory (a row that is there), zero where not `on`
 template <typename T, int KC>
-__device__ __forceinline__ void load_columns(const T* row, bool on, int D, int lane, Frag<Planes<T>::N> (&f)[KC]) {
+__device__ __forceinline__ void load_columns(const AttnP& p, const T* row, bool on, int lane, Held<T> (&h)[KC]) {
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc) h[kc].load(row + chunk_start(kc * 32 + 8 * (lane >> 4), p.D));
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc) {
-        Held<T> h;
-        h.zero();
         const int col = kc * 32 + 8 * (lane >> 4);
-        if (on && col < D) h.load(row + col, D - col);
-        h.planes(f[kc].p);
+        if (p.ragged) h[kc].fit(col - chunk_start(col, p.D));
+        h[kc].keep(on && col < p.D);
     }
+}
+template <typename T, int KC>
+__device__ __forceinline__ void load_columns(const AttnP& p, const T* row, bool on, int lane, Frag<Planes<T>::N> (&f)[KC]) {
+    Held<T> h[KC];
+    load_columns<T, KC>(p, row, on, lane, h);
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc) h[kc].planes(f[kc].p);
 }
 
 // two 16-row accumulator tiles -> the B operand of the second product (k slots 8 g + 0..3 from the first tile, 4..7 from the second)
@@ -85,6 +103,87 @@ __device__ __forceinline__ void as_operand(const f32x4& a, const f32x4& b, Frag<
     to_planes<NP>(x, f.p);
 }
 
+// scores of rows j .. j + 3 of one column: hidden behind the last visible row, or by a mask (rows from `end` on are hidden already)
+__device__ __forceinline__ void hide_later(f32x4& s, int j, int last) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (j + e > last) s[e] = NEG_INF;
+}
+__device__ __forceinline__ void hide_masked(f32x4& s, const uint8_t* mask, int j, int end) {  // (all loads first: one wait)
+    uint8_t m[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[e] = mask[min(j + e, end - 1)];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (m[e]) s[e] = NEG_INF;
+}
+
+// the same with queries as rows: hidden in front of the first query that sees the column's key, or by the key's column of a mask
+__device__ __forceinline__ void hide_earlier(f32x4& s, int i, int first) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (i + e < first) s[e] = NEG_INF;
+}
+__device__ __forceinline__ void hide_masked_rows(f32x4& s, const uint8_t* mask, int64_t ld, int i, int end) {
+    uint8_t m[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[e] = mask[(int64_t)min(i + e, end - 1) * ld];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (m[e]) s[e] = NEG_INF;
+}
+
+// One step of the running softmax of a column: scores s (not yet scaled; -inf where hidden) become probabilities relative to the running
+// maximum m.  m stays unscaled and 2^(scale2 s - scale2 m) is one fma in front of the exponential.  The accumulators are rescaled only
+// when the maximum of some column of the wave moved: after the first tiles it rarely does.
+template <int KN, int DN>
+__device__ __forceinline__ void soften(f32x4 (&s)[KN], float& m, float& l, f32x4 (&acc)[DN], float scale2) {
+    float mx = NEG_INF;
+#pragma unroll
+    for (int t = 0; t < KN; ++t) mx = fmaxf(fmaxf(mx, fmaxf(s[t][0], s[t][1])), fmaxf(s[t][2], s[t][3]));
+    mx = fmaxf(m, max_over_groups(mx));
+    if (__any(mx > m)) {
+        const float alpha = __builtin_amdgcn_exp2f((m - (mx == NEG_INF ? 0.f : mx)) * scale2);
+        m = mx;
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < DN; ++d) acc[d] *= alpha;
+    }
+    const float ref = m == NEG_INF ? 0.f : -(m * scale2);  // nothing to see yet: 2^(-inf) = 0
+#pragma unroll
+    for (int t = 0; t < KN; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            s[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], scale2, ref));
+            l += s[t][e];
+        }
+}
+
+// a column's result: o = acc / sum, lse = scale2 m + log2(sum) (in powers of two), or this split's part of them
+template <typename T, int DN>
+__device__ __forceinline__ void finish(const AttnP& p, const f32x4 (&acc)[DN], float m, float sum, int b, int h, int q, int split, int g) {
+    const bool valid = !p.query_valid || p.query_valid[(int64_t)b * p.Lq + q];
+    const bool on = valid && (sum > 0.f || sum != sum);  // (a NaN row stays NaN)
+    const float inv = on ? 1.f / sum : 0.f, lse2 = on ? m * p.scale2 + __builtin_amdgcn_logf(sum) : NEG_INF;
+    const int64_t rows = (int64_t)p.B * p.H * p.Lq, row = ((int64_t)b * p.H + h) * p.Lq + q;
+#pragma unroll
+    for (int d = 0; d < DN; ++d) {
+        const int col = d * 16 + 4 * g;
+        if (col >= p.D) continue;
+        const f32x4 o = on ? acc[d] * inv : (f32x4){0.f, 0.f, 0.f, 0.f};
+        if (p.n_split > 1)
+            store4(p.part + (split * rows + row) * p.D + col, p.D - col, o);
+        else
+            store4((T*)p.out + b * p.os[0] + q * p.os[1] + h * p.os[2] + col, p.D - col, o);
+    }
+    if (g == 0) {
+        if (p.n_split > 1)
+            p.part_lse[split * rows + row] = lse2;
+        else
+            p.lse[row] = lse2 * LN2;
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ forward
 template <typename T, int DP, int NW, int NQ, int KT>
 __global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AttnP p) {
@@ -92,23 +191,25 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AttnP p) {
     __shared__ __attribute__((aligned(16))) bf16 lk[NP * KT * LD];
     __shared__ __attribute__((aligned(16))) bf16 lv[NP * KT * LD];
     __shared__ __attribute__((aligned(16))) float lb[KT];
-    int bh, inner;
-    if (!decode(blockIdx.x, p.n_col_tile * p.n_split, p.B * p.H, p.xcd, bh, inner)) return;
-    const int split = inner / p.n_col_tile, qt = p.n_col_tile - 1 - inner % p.n_col_tile;  // (causal: the longest walks first)
+    int bh, split, tile;
+    if (!decode(p, p.B * p.H, bh, split, tile)) return;
+    const int qt = p.n_col_tile - 1 - tile;  // (causal: the longest walks first)
     const int b = bh / p.H, h = bh % p.H, hk = h / p.G;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i16 = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, g = lane >> 4;
+    const Valid qvalid(p.query_valid, (int64_t)b * p.Lq);
     const int qb = qt * QT, q0 = qb + wave * 16 * NQ, off = p.Lk - p.Lq;
     const T* kp = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
     const T* vp = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
-    const uint8_t* kvalid = p.key_valid ? p.key_valid + (int64_t)b * p.Lk : nullptr;
+    const Valid kvalid(p.key_valid, (int64_t)b * p.Lk);
 
     Frag<NP> qf[NQ][KC];
     int qi[NQ];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         qi[n] = q0 + n * 16 + i16;
-        const bool on = qi[n] < p.Lq && (!p.query_valid || p.query_valid[(int64_t)b * p.Lq + qi[n]]);
-        load_columns<T, KC>((const T*)p.q + b * p.qs[0] + (int64_t)(on ? qi[n] : 0) * p.qs[1] + h * p.qs[2], on, p.D, lane, qf[n]);
+        const int qc = min(qi[n], p.Lq - 1);
+        const bool on = qvalid[qc] && qi[n] < p.Lq;
+        load_columns<T, KC>(p, (const T*)p.q + b * p.qs[0] + (int64_t)qc * p.qs[1] + h * p.qs[2], on, lane, qf[n]);
     }
     f32x4 acc[NQ][DN];
     float m[NQ], l[NQ];
@@ -124,18 +225,17 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AttnP p) {
 
     Stage<T, DP, NT, KT> sk, sv;
     if (j0 < jend) {
-        sk.load(kp, p.ks[1], kvalid, j0, jend, p.D, tid);
-        sv.load(vp, p.vs[1], kvalid, j0, jend, p.D, tid);
+        sk.load(p, kp, p.ks[1], kvalid, j0, jend, tid);
+        sv.load(p, vp, p.vs[1], kvalid, j0, jend, tid);
     }
     for (; j0 < jend; j0 += KT) {
         __syncthreads();
-        sk.store(lk, tid);
-        sv.store(lv, tid);
-        if (tid < KT) lb[tid] = (j0 + tid < jend && (!kvalid || kvalid[j0 + tid])) ? 0.f : NEG_INF;
+        sk.store(p, lk, lb, tid);
+        sv.store(p, lv, nullptr, tid);
         __syncthreads();
         if (j0 + KT < jend) {
-            sk.load(kp, p.ks[1], kvalid, j0 + KT, jend, p.D, tid);
-            sv.load(vp, p.vs[1], kvalid, j0 + KT, jend, p.D, tid);
+            sk.load(p, kp, p.ks[1], kvalid, j0 + KT, jend, tid);
+            sv.load(p, vp, p.vs[1], kvalid, j0 + KT, jend, tid);
         }
         f32x4 s[NQ][KN];
 #pragma unroll
@@ -150,42 +250,20 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AttnP p) {
                 for (int n = 0; n < NQ; ++n) s[n][t] = mma<NP>(a, qf[n][kc], s[n][t]);
             }
         }
-        const bool biased = kvalid || j0 + KT > jend, diagonal = p.causal && j0 + KT - 1 > q0 + off;
+        const bool biased = p.key_valid || j0 + KT > jend, diagonal = p.causal && j0 + KT - 1 > q0 + off;
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
-            float mx = NEG_INF;
 #pragma unroll
             for (int t = 0; t < KN; ++t) {
-                s[n][t] *= p.scale2;
                 if (biased) s[n][t] += *reinterpret_cast<const f32x4*>(lb + t * 16 + 4 * g);
-                if (diagonal) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (j0 + t * 16 + 4 * g + e > qi[n] + off) s[n][t][e] = NEG_INF;
-                }
-                if (p.mask && qi[n] < p.Lq) {
-                    const uint8_t* mr = p.mask + b * p.mask_s[0] + (int64_t)qi[n] * p.mask_s[1] + j0 + t * 16 + 4 * g;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (j0 + t * 16 + 4 * g + e < jend && mr[e]) s[n][t][e] = NEG_INF;
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[n][t][e]);
+                if (diagonal) hide_later(s[n][t], j0 + t * 16 + 4 * g, qi[n] + off);
             }
-            mx = fmaxf(m[n], max_over_groups(mx));
-            const float ref = mx == NEG_INF ? 0.f : mx;  // nothing to see yet: exp2(-inf - 0) = 0
-            const float alpha = __builtin_amdgcn_exp2f(m[n] - ref);
-            m[n] = mx;
-            l[n] *= alpha;
+            if (p.mask) {
+                const uint8_t* mask = p.mask + b * p.mask_s[0] + (int64_t)min(qi[n], p.Lq - 1) * p.mask_s[1];
 #pragma unroll
-            for (int d = 0; d < DN; ++d) acc[n][d] *= alpha;
-#pragma unroll
-            for (int t = 0; t < KN; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[n][t][e] = __builtin_amdgcn_exp2f(s[n][t][e] - ref);
-                    l[n] += s[n][t][e];
-                }
+                for (int t = 0; t < KN; ++t) hide_masked(s[n][t], mask, j0 + t * 16 + 4 * g, jend);
+            }
+            soften<KN, DN>(s[n], m[n], l[n], acc[n], p.scale2);
         }
 #pragma unroll
         for (int t = 0; t < KN; t += 2) {
@@ -204,29 +282,7 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AttnP p) {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         const float sum = sum_over_groups(l[n]);
-        if (qi[n] >= p.Lq) continue;
-        const bool on = sum > 0.f || sum != sum;  // (a NaN row stays NaN)
-        const bool valid = !p.query_valid || p.query_valid[(int64_t)b * p.Lq + qi[n]];
-        const float inv = on && valid ? 1.f / sum : 0.f;
-        const float lse2 = on && valid ? m[n] + __builtin_amdgcn_logf(sum) : NEG_INF;
-        const int64_t row = (int64_t)bh * p.Lq + qi[n];
-#pragma unroll
-        for (int d = 0; d < DN; ++d) {
-            const int col = d * 16 + 4 * g;
-            f32x4 o = acc[n][d] * inv;
-            if (!(on && valid)) o = (f32x4){0.f, 0.f, 0.f, 0.f};
-            if (col >= p.D) continue;
-            if (p.n_split > 1)
-                store4(p.part + ((int64_t)split * p.B * p.H * p.Lq + row) * p.D + col, p.D - col, o);
-            else
-                store4((T*)p.out + b * p.os[0] + qi[n] * p.os[1] + h * p.os[2] + col, p.D - col, o);
-        }
-        if (g == 0) {
-            if (p.n_split > 1)
-                p.part_lse[(int64_t)split * p.B * p.H * p.Lq + row] = lse2;
-            else
-                p.lse[row] = lse2 * LN2;
-        }
+        if (qi[n] < p.Lq) finish<T, DN>(p, acc[n], m[n], sum, b, h, qi[n], split, g);
     }
 }
 
@@ -257,6 +313,383 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnP p) {
     if (col == 0) p.lse[row] = on ? (ref + __builtin_amdgcn_logf(sum)) * LN2 : NEG_INF;
 }
 
+// ------------------------------------------------------------------------------------------------ few columns: private walks
+// With at most 32 columns a workgroup has nothing to share: each wave walks 32 rows at a time on its own.  The rows it needs as A operand it
+// loads straight into that layout; only what the second product reads down its rows goes through LDS, a region of the wave's own, so
+// there is no barrier in the walk.  One wave takes one problem; with `wpp` = 4 (a single query over a long cache) the four waves of a
+// workgroup share the walk of one problem and join at its end.
+__device__ __forceinline__ void wave_fence() {  // orders the wave's own LDS accesses across its lanes
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// which of a lane's two rows (one of each 16-row tile) are there and valid
+struct Rows32 {
+    uint8_t valid[2];
+    int left;
+    __device__ __forceinline__ bool on(int t, int lane) const { return valid[t] && t * 16 + (lane & 15) < left; }
+};
+// rows row0 .. row0 + 31 (row0 < end) of a [., D] matrix for two 16-row tiles
+template <typename T, int KC>
+__device__ __forceinline__ void load_rows32(const AttnP& p, const T* base, int64_t ld, const Valid& valid, int row0, int end, int lane, Held<T> (&h)[2][KC], Rows32& ok) {
+    ok.left = end - row0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int rc = min(row0 + t * 16 + (lane & 15), end - 1);
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) h[t][kc].load(base + (int64_t)rc * ld + chunk_start(kc * 32 + 8 * (lane >> 4), p.D));
+        ok.valid[t] = valid[rc];
+    }
+}
+template <typename T, int KC>
+__device__ __forceinline__ void keep_rows32(const AttnP& p, Held<T> (&h)[2][KC], const Rows32& ok, int lane) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) {
+            const int col = kc * 32 + 8 * (lane >> 4);
+            if (p.ragged) h[t][kc].fit(col - chunk_start(col, p.D));
+            h[t][kc].keep(ok.on(t, lane) && col < p.D);
+        }
+}
+template <typename T, int KC>
+__device__ __forceinline__ void as_frags(const Held<T> (&h)[2][KC], Frag<Planes<T>::N> (&f)[2][KC]) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) h[t][kc].planes(f[t][kc].p);
+}
+// ... into the wave's LDS region, [planes][32][LD]
+template <int NP, int KC, int LD>
+__device__ __forceinline__ void rows32_to_lds(const Frag<NP> (&f)[2][KC], bf16* lds, int lane) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc)
+#pragma unroll
+            for (int n = 0; n < NP; ++n) *reinterpret_cast<bf16x8*>(lds + n * 32 * LD + (t * 16 + (lane & 15)) * LD + kc * 32 + 8 * (lane >> 4)) = f[t][kc].p[n];
+}
+// -inf where one of rows 16 t + 4 g + e is not there
+__device__ __forceinline__ void row_bias(const Rows32& ok, int lane, f32x4 (&bias)[2]) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const unsigned on = (unsigned)__ballot(ok.on(t, lane)) >> (4 * (lane >> 4));  // (every group of 16 lanes holds the tile's 16 rows)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bias[t][e] = on >> e & 1 ? 0.f : NEG_INF;
+    }
+}
+
+template <typename T, int DP, int NQ>
+__global__ __launch_bounds__(256) void k_attn_fwd_few(const AttnP p) {
+    constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, LD = DP + LDS_PAD;
+    constexpr int JOIN = 2 * 16 * NQ * DP * 2;  // (in bf16 elements) two waves' accumulators
+    constexpr int REGION = 4 * NP * 32 * LD > JOIN ? 4 * NP * 32 * LD : JOIN;
+    __shared__ __attribute__((aligned(16))) bf16 region[REGION];
+    __shared__ float ml[2][4][16 * NQ];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, g = lane >> 4;
+    const int part = p.wpp > 1 ? wave : 0;
+    const int64_t id = p.wpp > 1 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+    const int n_bh = p.B * p.H, split = (int)(id / n_bh), bh = (int)(id % n_bh);
+    if (split >= p.n_split) return;  // (wpp > 1: the grid has no such workgroup)
+    const int b = bh / p.H, h = bh % p.H, hk = h / p.G, off = p.Lk - p.Lq;
+    const T* kp = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
+    const T* vp = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
+    const Valid kvalid(p.key_valid, (int64_t)b * p.Lk);
+    bf16* lv = region + wave * NP * 32 * LD;
+    const Valid qvalid(p.query_valid, (int64_t)b * p.Lq);
+
+    Frag<NP> qf[NQ][KC];
+    f32x4 acc[NQ][DN];
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int q = n * 16 + i16, qc = min(q, p.Lq - 1);
+        const bool on = qvalid[qc] && q < p.Lq;
+        load_columns<T, KC>(p, (const T*)p.q + b * p.qs[0] + (int64_t)qc * p.qs[1] + h * p.qs[2], on, lane, qf[n]);
+        m[n] = NEG_INF;
+        l[n] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DN; ++d) acc[n][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+    const int first = split * p.split_len;
+    int jend = min(p.Lk, first + p.split_len);
+    if (p.causal) jend = min(jend, p.Lq + off);
+    const int step = 32 * p.wpp;
+    Held<T> rk[2][KC], rv[2][KC];
+    Rows32 ok;
+    int j0 = first + part * 32;
+    if (j0 < jend) {
+        load_rows32<T, KC>(p, kp, p.ks[1], kvalid, j0, jend, lane, rk, ok);
+        load_rows32<T, KC>(p, vp, p.vs[1], kvalid, j0, jend, lane, rv, ok);
+    }
+    for (; j0 < jend; j0 += step) {
+        Frag<NP> kf[2][KC], vf[2][KC];
+        f32x4 bias[2];
+        row_bias(ok, lane, bias);
+        keep_rows32<T, KC>(p, rk, ok, lane);
+        keep_rows32<T, KC>(p, rv, ok, lane);
+        as_frags<T, KC>(rk, kf);
+        as_frags<T, KC>(rv, vf);
+        wave_fence();
+        rows32_to_lds<NP, KC, LD>(vf, lv, lane);
+        wave_fence();
+        if (j0 + step < jend) {
+            load_rows32<T, KC>(p, kp, p.ks[1], kvalid, j0 + step, jend, lane, rk, ok);
+            load_rows32<T, KC>(p, vp, p.vs[1], kvalid, j0 + step, jend, lane, rv, ok);
+        }
+        Frag<NP> pf[NQ];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            f32x4 s[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                s[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kc = 0; kc < KC; ++kc) s[t] = mma<NP>(kf[t][kc], qf[n][kc], s[t]);
+                s[t] += bias[t];
+                if (p.causal) hide_later(s[t], j0 + t * 16 + 4 * g, n * 16 + i16 + off);
+            }
+            if (p.mask) {
+                const uint8_t* mask = p.mask + b * p.mask_s[0] + (int64_t)min(n * 16 + i16, p.Lq - 1) * p.mask_s[1];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) hide_masked(s[t], mask, j0 + t * 16 + 4 * g, jend);
+            }
+            soften<2, DN>(s, m[n], l[n], acc[n], p.scale2);
+            as_operand<NP>(s[0], s[1], pf[n]);
+        }
+#pragma unroll
+        for (int d = 0; d < DN; ++d) {
+            Frag<NP> a;
+            frag_cols<NP, LD>(lv, (size_t)32 * LD, 4 * g, 16 + 4 * g, d * 16, lane, a);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) acc[n][d] = mma<NP>(a, pf[n], acc[n][d]);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) l[n] = sum_over_groups(l[n]);
+    if (p.wpp > 1) {  // (workgroup-uniform) a common maximum, then the four waves' sums: 2, 3 into 0, 1, then 1 into 0
+        float* red = reinterpret_cast<float*>(region);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+            if (g == 0) {
+                ml[0][wave][n * 16 + i16] = m[n];
+                ml[1][wave][n * 16 + i16] = l[n];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            float mx = NEG_INF, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) mx = fmaxf(mx, ml[0][w][n * 16 + i16]);
+            const float ref = mx == NEG_INF ? 0.f : mx;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) sum = __builtin_fmaf(ml[1][w][n * 16 + i16], __builtin_amdgcn_exp2f((ml[0][w][n * 16 + i16] - ref) * p.scale2), sum);
+            const float alpha = __builtin_amdgcn_exp2f((m[n] - ref) * p.scale2);
+            m[n] = mx;
+            l[n] = sum;
+#pragma unroll
+            for (int d = 0; d < DN; ++d) acc[n][d] *= alpha;
+        }
+#pragma unroll
+        for (int half = 2; half >= 1; half >>= 1) {
+            if (wave >= half && wave < 2 * half) {
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int d = 0; d < DN; ++d) *reinterpret_cast<f32x4*>(red + ((((wave - half) * NQ + n) * DN + d) * 64 + lane) * 4) = acc[n][d];
+            }
+            __syncthreads();
+            if (wave < half) {
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int d = 0; d < DN; ++d) acc[n][d] += *reinterpret_cast<const f32x4*>(red + (((wave * NQ + n) * DN + d) * 64 + lane) * 4);
+            }
+            __syncthreads();
+        }
+        if (wave) return;
+    }
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int q = n * 16 + i16;
+        if (q < p.Lq) finish<T, DN>(p, acc[n], m[n], l[n], b, h, q, split, g);
+    }
+}
+
+// Backward of a whole problem with at most 32 queries and 32 keys: one wave per key / value head, everything loaded once.  Queries as columns
+// give dq; the scores once more with keys as columns give dk and dv.  The same registers serve as A and as B operand (both layouts
+// hold 8 components of one row).  K, dO and Q pass one after the other through the wave's LDS region to be read down their rows.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void k_attn_bwd_small(const AttnP p) {
+    constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, LD = DP + LDS_PAD;
+    __shared__ __attribute__((aligned(16))) bf16 region[4 * NP * 32 * LD];
+    __shared__ __attribute__((aligned(16))) float rowv[4][2][32];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i16 = lane & 15, g = lane >> 4;
+    const int64_t id = (int64_t)blockIdx.x * 4 + wave;
+    if (id >= (int64_t)p.B * p.Hkv) return;  // (no barrier below)
+    const int b = (int)(id / p.Hkv), hk = (int)(id % p.Hkv), off = p.Lk - p.Lq;
+    const Valid kvalid(p.key_valid, (int64_t)b * p.Lk);
+    const Valid qvalid(p.query_valid, (int64_t)b * p.Lq);
+    bf16* lds = region + wave * NP * 32 * LD;
+    float* nlse_r = rowv[wave][0];
+    float* delta_r = rowv[wave][1];
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+
+    Frag<NP> kf[2][KC], vf[2][KC];
+    Rows32 kok;
+    {
+        Held<T> a[2][KC], v[2][KC];
+        load_rows32<T, KC>(p, (const T*)p.k + b * p.ks[0] + hk * p.ks[2], p.ks[1], kvalid, 0, p.Lk, lane, a, kok);
+        load_rows32<T, KC>(p, (const T*)p.v + b * p.vs[0] + hk * p.vs[2], p.vs[1], kvalid, 0, p.Lk, lane, v, kok);
+        keep_rows32<T, KC>(p, a, kok, lane);
+        keep_rows32<T, KC>(p, v, kok, lane);
+        as_frags<T, KC>(a, kf);
+        as_frags<T, KC>(v, vf);
+    }
+    f32x4 bias[2], dk[2][DN], dv[2][DN];
+    row_bias(kok, lane, bias);
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int d = 0; d < DN; ++d) dk[n][d] = dv[n][d] = zero;
+    for (int h = hk * p.G; h < (hk + 1) * p.G; ++h) {
+        Frag<NP> qf[2][KC], gf[2][KC];
+        float nlse[2], delta[2];
+        {
+            Held<T> q[2][KC], go[2][KC], o[2][KC];
+            Rows32 ok;
+            float lse[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) lse[n] = p.lse[((int64_t)b * p.H + h) * p.Lq + min(n * 16 + i16, p.Lq - 1)];
+            load_rows32<T, KC>(p, (const T*)p.q + b * p.qs[0] + h * p.qs[2], p.qs[1], qvalid, 0, p.Lq, lane, q, ok);
+            load_rows32<T, KC>(p, (const T*)p.d_out + b * p.dos[0] + h * p.dos[2], p.dos[1], qvalid, 0, p.Lq, lane, go, ok);
+            load_rows32<T, KC>(p, (const T*)p.out + b * p.os[0] + h * p.os[2], p.os[1], qvalid, 0, p.Lq, lane, o, ok);
+            keep_rows32<T, KC>(p, q, ok, lane);
+            keep_rows32<T, KC>(p, go, ok, lane);
+            keep_rows32<T, KC>(p, o, ok, lane);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                float dot = 0.f;
+#pragma unroll
+                for (int kc = 0; kc < KC; ++kc)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) dot = __builtin_fmaf(go[n][kc].get(e), o[n][kc].get(e), dot);
+                delta[n] = sum_over_groups(dot);
+                nlse[n] = !ok.on(n, lane) || lse[n] == NEG_INF ? NEG_INF : -lse[n] * LOG2E;
+            }
+            as_frags<T, KC>(q, qf);
+            as_frags<T, KC>(go, gf);
+        }
+        wave_fence();
+        rows32_to_lds<NP, KC, LD>(kf, lds, lane);
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+            if (g == 0) {
+                nlse_r[n * 16 + i16] = nlse[n];
+                delta_r[n * 16 + i16] = delta[n];
+            }
+        wave_fence();
+        {  // queries as columns: dq
+            Frag<NP> df[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                f32x4 ds[2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    f32x4 s = zero, dp = zero;
+#pragma unroll
+                    for (int kc = 0; kc < KC; ++kc) {
+                        s = mma<NP>(kf[t][kc], qf[n][kc], s);
+                        dp = mma<NP>(vf[t][kc], gf[n][kc], dp);
+                    }
+                    const int q = n * 16 + i16, j = t * 16 + 4 * g;
+                    f32x4 x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(s[e], p.scale2, nlse[n]) + bias[t][e];
+                    if (p.causal) hide_later(x, j, q + off);
+                    if (p.mask) hide_masked(x, p.mask + b * p.mask_s[0] + (int64_t)min(q, p.Lq - 1) * p.mask_s[1], j, p.Lk);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) ds[t][e] = __builtin_amdgcn_exp2f(x[e]) * (dp[e] - delta[n]);
+                }
+                as_operand<NP>(ds[0], ds[1], df[n]);
+            }
+#pragma unroll
+            for (int d = 0; d < DN; ++d) {
+                Frag<NP> a;
+                frag_cols<NP, LD>(lds, (size_t)32 * LD, 4 * g, 16 + 4 * g, d * 16, lane, a);
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const int q = n * 16 + i16, col = d * 16 + 4 * g;
+                    const f32x4 o = mma<NP>(a, df[n], zero) * p.scale;
+                    if (q < p.Lq && col < p.D) store4((T*)p.dq + b * p.dqs[0] + q * p.dqs[1] + h * p.dqs[2] + col, p.D - col, o);
+                }
+            }
+        }
+        // keys as columns: dk, dv
+        Frag<NP> pf[2], df[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            f32x4 pr[2], ds[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                f32x4 s = zero, dp = zero;
+#pragma unroll
+                for (int kc = 0; kc < KC; ++kc) {
+                    s = mma<NP>(qf[t][kc], kf[n][kc], s);
+                    dp = mma<NP>(gf[t][kc], vf[n][kc], dp);
+                }
+                const int key = n * 16 + i16, i = t * 16 + 4 * g;
+                const f32x4 nl = *reinterpret_cast<const f32x4*>(nlse_r + i), de = *reinterpret_cast<const f32x4*>(delta_r + i);
+                f32x4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(s[e], p.scale2, nl[e]);
+                if (p.causal) hide_earlier(x, i, key - off);
+                if (p.mask) hide_masked_rows(x, p.mask + b * p.mask_s[0] + min(key, p.Lk - 1), p.mask_s[1], i, p.Lq);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    pr[t][e] = __builtin_amdgcn_exp2f(x[e]);
+                    ds[t][e] = pr[t][e] * (dp[e] - de[e]);
+                }
+            }
+            as_operand<NP>(pr[0], pr[1], pf[n]);
+            as_operand<NP>(ds[0], ds[1], df[n]);
+        }
+        wave_fence();
+        rows32_to_lds<NP, KC, LD>(gf, lds, lane);
+        wave_fence();
+#pragma unroll
+        for (int d = 0; d < DN; ++d) {
+            Frag<NP> a;
+            frag_cols<NP, LD>(lds, (size_t)32 * LD, 4 * g, 16 + 4 * g, d * 16, lane, a);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) dv[n][d] = mma<NP>(a, pf[n], dv[n][d]);
+        }
+        wave_fence();
+        rows32_to_lds<NP, KC, LD>(qf, lds, lane);
+        wave_fence();
+#pragma unroll
+        for (int d = 0; d < DN; ++d) {
+            Frag<NP> a;
+            frag_cols<NP, LD>(lds, (size_t)32 * LD, 4 * g, 16 + 4 * g, d * 16, lane, a);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) dk[n][d] = mma<NP>(a, df[n], dk[n][d]);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const int key = n * 16 + i16;
+        if (key >= p.Lk) continue;
+        const bool on = kok.on(n, lane);
+#pragma unroll
+        for (int d = 0; d < DN; ++d) {
+            const int col = d * 16 + 4 * g;
+            if (col >= p.D) continue;
+            store4((T*)p.dk + b * p.dks[0] + key * p.dks[1] + hk * p.dks[2] + col, p.D - col, on ? dk[n][d] * p.scale : zero);
+            store4((T*)p.dv + b * p.dvs[0] + key * p.dvs[1] + hk * p.dvs[2] + col, p.D - col, on ? dv[n][d] : zero);
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ backward: dq
 template <typename T, int DP, int NW, int NQ, int KT>
 __global__ __launch_bounds__(64 * NW) void k_attn_dq(const AttnP p) {
@@ -264,15 +697,16 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(const AttnP p) {
     __shared__ __attribute__((aligned(16))) bf16 lk[NP * KT * LD];
     __shared__ __attribute__((aligned(16))) bf16 lv[NP * KT * LD];
     __shared__ __attribute__((aligned(16))) float lb[KT];
-    int bh, inner;
-    if (!decode(blockIdx.x, p.n_col_tile * p.n_split, p.B * p.H, p.xcd, bh, inner)) return;
-    const int split = inner / p.n_col_tile, qt = p.n_col_tile - 1 - inner % p.n_col_tile;
+    int bh, split, tile;
+    if (!decode(p, p.B * p.H, bh, split, tile)) return;
+    const int qt = p.n_col_tile - 1 - tile;
     const int b = bh / p.H, h = bh % p.H, hk = h / p.G;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i16 = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, g = lane >> 4;
+    const Valid qvalid(p.query_valid, (int64_t)b * p.Lq);
     const int qb = qt * QT, q0 = qb + wave * 16 * NQ, off = p.Lk - p.Lq;
     const T* kp = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
     const T* vp = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
-    const uint8_t* kvalid = p.key_valid ? p.key_valid + (int64_t)b * p.Lk : nullptr;
+    const Valid kvalid(p.key_valid, (int64_t)b * p.Lk);
 
     Frag<NP> qf[NQ][KC], gf[NQ][KC];
     int qi[NQ];
@@ -281,27 +715,23 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(const AttnP p) {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         qi[n] = q0 + n * 16 + i16;
-        const bool in = qi[n] < p.Lq, on = in && (!p.query_valid || p.query_valid[(int64_t)b * p.Lq + qi[n]]);
-        const int64_t qr = on ? qi[n] : 0, row = (int64_t)bh * p.Lq + qi[n];
-        const T* dop = (const T*)p.d_out + b * p.dos[0] + qr * p.dos[1] + h * p.dos[2];
-        load_columns<T, KC>((const T*)p.q + b * p.qs[0] + qr * p.qs[1] + h * p.qs[2], on, p.D, lane, qf[n]);
-        load_columns<T, KC>(dop, on, p.D, lane, gf[n]);
-        const T* op = (const T*)p.out + b * p.os[0] + qr * p.os[1] + h * p.os[2];
+        const bool in = qi[n] < p.Lq;
+        const int64_t qc = in ? qi[n] : p.Lq - 1, row = (int64_t)bh * p.Lq + qc;
+        const bool on = qvalid[qc] && in;
+        const float lse = p.lse[row];
+        load_columns<T, KC>(p, (const T*)p.q + b * p.qs[0] + qc * p.qs[1] + h * p.qs[2], on, lane, qf[n]);
+        Held<T> go[KC], o[KC];
+        load_columns<T, KC>(p, (const T*)p.d_out + b * p.dos[0] + qc * p.dos[1] + h * p.dos[2], on, lane, go);
+        load_columns<T, KC>(p, (const T*)p.out + b * p.os[0] + qc * p.os[1] + h * p.os[2], on, lane, o);
         float dot = 0.f;
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) {
-            const int col = kc * 32 + 8 * g;
-            if (on && col < p.D) {
-                float x[8], y[8];
-                load8(dop + col, p.D - col, x);
-                load8(op + col, p.D - col, y);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) dot = __builtin_fmaf(x[e], y[e], dot);
-            }
+            for (int e = 0; e < 8; ++e) dot = __builtin_fmaf(go[kc].get(e), o[kc].get(e), dot);
+            go[kc].planes(gf[n][kc].p);
         }
         delta[n] = sum_over_groups(dot);
-        const float lse = on ? p.lse[row] : NEG_INF;
-        nlse[n] = lse == NEG_INF ? NEG_INF : -lse * LOG2E;  // an empty row: p = 2^(-inf) = 0
+        nlse[n] = !on || lse == NEG_INF ? NEG_INF : -lse * LOG2E;  // an empty row: p = 2^(-inf) = 0
         if (in && g == 0 && split == 0) p.delta[row] = delta[n];
 #pragma unroll
         for (int d = 0; d < DN; ++d) acc[n][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -310,20 +740,19 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(const AttnP p) {
     if (p.causal) jend = min(jend, min(p.Lq, qb + QT) + off);
     Stage<T, DP, NT, KT> sk, sv;
     if (j0 < jend) {
-        sk.load(kp, p.ks[1], kvalid, j0, jend, p.D, tid);
-        sv.load(vp, p.vs[1], kvalid, j0, jend, p.D, tid);
+        sk.load(p, kp, p.ks[1], kvalid, j0, jend, tid);
+        sv.load(p, vp, p.vs[1], kvalid, j0, jend, tid);
     }
     for (; j0 < jend; j0 += KT) {
         __syncthreads();
-        sk.store(lk, tid);
-        sv.store(lv, tid);
-        if (tid < KT) lb[tid] = (j0 + tid < jend && (!kvalid || kvalid[j0 + tid])) ? 0.f : NEG_INF;
+        sk.store(p, lk, lb, tid);
+        sv.store(p, lv, nullptr, tid);
         __syncthreads();
         if (j0 + KT < jend) {
-            sk.load(kp, p.ks[1], kvalid, j0 + KT, jend, p.D, tid);
-            sv.load(vp, p.vs[1], kvalid, j0 + KT, jend, p.D, tid);
+            sk.load(p, kp, p.ks[1], kvalid, j0 + KT, jend, tid);
+            sv.load(p, vp, p.vs[1], kvalid, j0 + KT, jend, tid);
         }
-        const bool biased = kvalid || j0 + KT > jend, diagonal = p.causal && j0 + KT - 1 > q0 + off;
+        const bool biased = p.key_valid || j0 + KT > jend, diagonal = p.causal && j0 + KT - 1 > q0 + off;
 #pragma unroll
         for (int t2 = 0; t2 < KN; t2 += 2) {
             f32x4 ds[NQ][2];
@@ -350,17 +779,8 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(const AttnP p) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(s[n][e], p.scale2, nlse[n]);
                     if (biased) x += *reinterpret_cast<const f32x4*>(lb + t * 16 + 4 * g);
-                    if (diagonal) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (j0 + t * 16 + 4 * g + e > qi[n] + off) x[e] = NEG_INF;
-                    }
-                    if (p.mask && qi[n] < p.Lq) {
-                        const uint8_t* mr = p.mask + b * p.mask_s[0] + (int64_t)qi[n] * p.mask_s[1] + j0 + t * 16 + 4 * g;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (j0 + t * 16 + 4 * g + e < jend && mr[e]) x[e] = NEG_INF;
-                    }
+                    if (diagonal) hide_later(x, j0 + t * 16 + 4 * g, qi[n] + off);
+                    if (p.mask) hide_masked(x, p.mask + b * p.mask_s[0] + (int64_t)min(qi[n], p.Lq - 1) * p.mask_s[1], j0 + t * 16 + 4 * g, jend);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) ds[n][u][e] = __builtin_amdgcn_exp2f(x[e]) * (dp[n][e] - delta[n]);
                 }
@@ -403,13 +823,14 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AttnP p) {
     __shared__ __attribute__((aligned(16))) bf16 lg[NP * KT * LD];
     __shared__ __attribute__((aligned(16))) float ll[KT];
     __shared__ __attribute__((aligned(16))) float ld[KT];
-    int bh, inner;
-    if (!decode(blockIdx.x, p.n_col_tile * p.n_split, p.B * p.Hkv, p.xcd, bh, inner)) return;
-    const int split = inner / p.n_col_tile, kt = inner % p.n_col_tile;  // (causal: the first keys have the longest walks)
+    int bh, split, tile;
+    if (!decode(p, p.B * p.Hkv, bh, split, tile)) return;
+    const int kt = tile;  // (causal: the first keys have the longest walks)
     const int b = bh / p.Hkv, hk = bh % p.Hkv;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i16 = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, g = lane >> 4;
+    const Valid kvalid(p.key_valid, (int64_t)b * p.Lk);
     const int kb = kt * CT, k0 = kb + wave * 16 * NQ, off = p.Lk - p.Lq;
-    const uint8_t* qvalid = p.query_valid ? p.query_valid + (int64_t)b * p.Lq : nullptr;
+    const Valid qvalid(p.query_valid, (int64_t)b * p.Lq);
 
     Frag<NP> kf[NQ][KC], vf[NQ][KC];
     int ki[NQ];
@@ -418,10 +839,10 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AttnP p) {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         ki[n] = k0 + n * 16 + i16;
-        on[n] = ki[n] < p.Lk && (!p.key_valid || p.key_valid[(int64_t)b * p.Lk + ki[n]]);
-        const int64_t kr = on[n] ? ki[n] : 0;
-        load_columns<T, KC>((const T*)p.k + b * p.ks[0] + kr * p.ks[1] + hk * p.ks[2], on[n], p.D, lane, kf[n]);
-        load_columns<T, KC>((const T*)p.v + b * p.vs[0] + kr * p.vs[1] + hk * p.vs[2], on[n], p.D, lane, vf[n]);
+        const int64_t kc = min(ki[n], p.Lk - 1);
+        on[n] = kvalid[kc] && ki[n] < p.Lk;
+        load_columns<T, KC>(p, (const T*)p.k + b * p.ks[0] + kc * p.ks[1] + hk * p.ks[2], on[n], lane, kf[n]);
+        load_columns<T, KC>(p, (const T*)p.v + b * p.vs[0] + kc * p.vs[1] + hk * p.vs[2], on[n], lane, vf[n]);
 #pragma unroll
         for (int d = 0; d < DN; ++d) dk[n][d] = dv[n][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
@@ -433,26 +854,28 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AttnP p) {
 
     Stage<T, DP, NT, KT> sq, sg;
     float r_lse = 0.f, r_delta = 0.f;
+    uint8_t r_valid = 0;
+    bool r_in = false;
     auto load = [&](int step) {
         const int h = hk * p.G + step / per_head, q0 = (first + step % per_head) * KT;
-        sq.load((const T*)p.q + b * p.qs[0] + h * p.qs[2], p.qs[1], qvalid, q0, p.Lq, p.D, tid);
-        sg.load((const T*)p.d_out + b * p.dos[0] + h * p.dos[2], p.dos[1], qvalid, q0, p.Lq, p.D, tid);
-        if (tid < KT) {
-            const bool in = q0 + tid < p.Lq && (!qvalid || qvalid[q0 + tid]);
-            const int64_t row = ((int64_t)b * p.H + h) * p.Lq + q0 + tid;
-            const float lse = in ? p.lse[row] : NEG_INF;
-            r_lse = lse == NEG_INF ? NEG_INF : -lse * LOG2E;
-            r_delta = in ? p.delta[row] : 0.f;
-        }
+        sq.load(p, (const T*)p.q + b * p.qs[0] + h * p.qs[2], p.qs[1], qvalid, q0, p.Lq, tid);
+        sg.load(p, (const T*)p.d_out + b * p.dos[0] + h * p.dos[2], p.dos[1], qvalid, q0, p.Lq, tid);
+        const int q = q0 + tid % KT, qc = min(q, p.Lq - 1);
+        const int64_t row = ((int64_t)b * p.H + h) * p.Lq + qc;
+        r_lse = p.lse[row];
+        r_delta = p.delta[row];  // (0 in invalid rows)
+        r_valid = qvalid[qc];
+        r_in = q < p.Lq;
     };
     if (t < tend) load(t);
     for (; t < tend; ++t) {
         __syncthreads();
-        sq.store(lq, tid);
-        sg.store(lg, tid);
+        sq.store(p, lq, nullptr, tid);
+        sg.store(p, lg, nullptr, tid);
         if (tid < KT) {
-            ll[tid] = r_lse;
-            ld[tid] = r_delta;
+            const bool r_on = r_valid && r_in;
+            ll[tid] = !r_on || r_lse == NEG_INF ? NEG_INF : -r_lse * LOG2E;
+            ld[tid] = r_on ? r_delta : 0.f;
         }
         __syncthreads();
         const int q0 = (first + t % per_head) * KT;
@@ -484,18 +907,8 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AttnP p) {
                     f32x4 x;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(s[n][e], p.scale2, nl[e]);
-                    if (diagonal) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (ki[n] > q0 + tt * 16 + 4 * g + e + off) x[e] = NEG_INF;
-                    }
-                    if (p.mask && ki[n] < p.Lk) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int q = q0 + tt * 16 + 4 * g + e;
-                            if (q < p.Lq && p.mask[b * p.mask_s[0] + (int64_t)q * p.mask_s[1] + ki[n]]) x[e] = NEG_INF;
-                        }
-                    }
+                    if (diagonal) hide_earlier(x, q0 + tt * 16 + 4 * g, ki[n] - off);
+                    if (p.mask) hide_masked_rows(x, p.mask + b * p.mask_s[0] + min(ki[n], p.Lk - 1), p.mask_s[1], q0 + tt * 16 + 4 * g, p.Lq);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         pr[n][u][e] = __builtin_amdgcn_exp2f(x[e]);
@@ -562,55 +975,64 @@ __global__ __launch_bounds__(256) void k_attn_sum(const float* part, int n_split
 
 enum Pass { FWD, DQ, DKV };
 
-struct Shape {  // of one launch: columns per workgroup, walked rows per tile
+struct Shape {  // of one launch: columns per workgroup, walked rows per step of a workgroup
     int col_tile, walk_tile;
     void (*kernel)(AttnP);
     int threads;
+    bool few;  // wave-private walks (k_attn_fwd_few)
 };
 
-template <typename T, int DP, int NW, int NQ, int KT>
-Shape shape(Pass pass) {
-    return {16 * NQ * NW, KT, pass == FWD ? k_attn_fwd<T, DP, NW, NQ, KT> : pass == DQ ? k_attn_dq<T, DP, NW, NQ, KT> : k_attn_dkv<T, DP, NW, NQ, KT>, 64 * NW};
+template <typename T, int DP, int NQ, int KT>
+Shape tiles(Pass pass) {  // four waves
+    return {64 * NQ, KT, pass == FWD ? k_attn_fwd<T, DP, 4, NQ, KT> : pass == DQ ? k_attn_dq<T, DP, 4, NQ, KT> : k_attn_dkv<T, DP, 4, NQ, KT>, 256, false};
 }
 
 template <typename T, int DP>
-Shape choose(Pass pass, int n_col) {
-    constexpr int KT = sizeof(T) == 2 ? 64 : DP <= 64 ? 32 : 32;
-    if (n_col <= 16) return shape<T, DP, 1, 1, 32>(pass);
-    if (n_col <= 32) return shape<T, DP, 1, 2, 32>(pass);
-    return shape<T, DP, 4, 1, KT>(pass);
+Shape choose(Pass pass, int n_col, int64_t n_bh) {
+    constexpr bool wide = sizeof(T) == 2 || DP == 32;  // two column tiles per wave fit the registers
+    constexpr int KT = sizeof(T) == 2 || DP == 32 ? 64 : 32;
+    if (n_col <= 32) {
+        if (pass == FWD) return {32, 32, n_col <= 16 ? k_attn_fwd_few<T, DP, 1> : k_attn_fwd_few<T, DP, 2>, 256, true};
+        constexpr int NQ = wide ? 2 : 1;  // one wave
+        return {16 * NQ, 32, pass == DQ ? k_attn_dq<T, DP, 1, NQ, 32> : k_attn_dkv<T, DP, 1, NQ, 32>, 64, false};
+    }
+    if constexpr (wide)
+        if (n_col > 64 && n_bh * ((n_col + 127) / 128) >= 256) return tiles<T, DP, 2, KT>(pass);
+    return tiles<T, DP, 1, KT>(pass);
 }
 
 Shape choose(const AttnP& p, Pass pass) {
     const int n_col = pass == DKV ? p.Lk : p.Lq;
-    if (p.dtype == 1) return p.D <= 32 ? choose<bf16, 32>(pass, n_col) : p.D <= 64 ? choose<bf16, 64>(pass, n_col) : choose<bf16, 128>(pass, n_col);
-    return p.D <= 32 ? choose<float, 32>(pass, n_col) : p.D <= 64 ? choose<float, 64>(pass, n_col) : choose<float, 128>(pass, n_col);
+    const int64_t n = (int64_t)p.B * (pass == DKV ? p.Hkv : p.H);
+    if (p.dtype == 1) return p.D <= 32 ? choose<bf16, 32>(pass, n_col, n) : p.D <= 64 ? choose<bf16, 64>(pass, n_col, n) : choose<bf16, 128>(pass, n_col, n);
+    return p.D <= 32 ? choose<float, 32>(pass, n_col, n) : p.D <= 64 ? choose<float, 64>(pass, n_col, n) : choose<float, 128>(pass, n_col, n);
 }
 
-// Few workgroups and a long walk: the walk is split over workgroups whose results a second kernel joins, until the chip has about two
-// workgroups per CU; a part keeps at least four tiles.
+// Few workgroups and a long walk: the walk is split over workgroups whose results a second kernel joins (about 5 us), until the chip has
+// about two workgroups per CU; a part keeps at least eight steps.
 struct Plan {
     Shape s;
-    int n_col_tile, n_split, split_len;
+    int n_col_tile, n_split, split_len, wpp;
     int64_t n_bh, blocks;
 };
 Plan plan(const AttnP& p, Pass pass) {
     Plan r;
     r.s = choose(p, pass);
-    const int n_col = pass == DKV ? p.Lk : p.Lq;
+    const int n_col = pass == DKV ? p.Lk : p.Lq, walk = pass == DKV ? p.Lq : p.Lk;
     r.n_col_tile = (n_col + r.s.col_tile - 1) / r.s.col_tile;
     r.n_bh = (int64_t)p.B * (pass == DKV ? p.Hkv : p.H);
-    const int walk = pass == DKV ? p.Lq : p.Lk;
-    const int64_t tiles = (int64_t)((walk + r.s.walk_tile - 1) / r.s.walk_tile) * (pass == DKV ? p.G : 1);
-    const int64_t base = r.n_bh * r.n_col_tile, waves = 512 * 4 / (r.s.threads / 64);
-    int64_t n = base * 2 <= waves ? waves / (base > 0 ? base : 1) : 1;
-    n = n < tiles / 4 ? n : tiles / 4;
-    if (n < 1) n = 1;
-    if (n > 64) n = 64;
-    r.split_len = (int)((tiles + n - 1) / n) * r.s.walk_tile;  // (DKV: the kernel cuts its own walk, only n_split counts)
-    r.n_split = pass == DKV ? (int)n : (int)((walk + r.split_len - 1) / (r.split_len > 0 ? r.split_len : 1));
+    const int64_t base = r.n_bh * r.n_col_tile;
+    // a wave of its own for every problem fills the chip from 2048 problems on; below, and with a walk to share, a workgroup takes one
+    r.wpp = r.s.few && walk > 64 && base < 2048 ? 4 : 1;
+    const int step = r.s.walk_tile * r.wpp;
+    const int64_t steps = (int64_t)((walk + step - 1) / step) * (pass == DKV ? p.G : 1), slots = 512 * 4 / (r.s.few ? r.wpp : r.s.threads / 64);
+    int64_t n = base * 2 <= slots ? slots / (base > 0 ? base : 1) : 1;
+    n = n < steps / 8 ? n : steps / 8;
+    n = n < 1 ? 1 : n > 64 ? 64 : n;
+    const int64_t len = (steps + n - 1) / n * step;  // (DKV: the kernel cuts its own walk, only n_split counts)
+    r.split_len = len < step ? step : len > 0x7fffffff - step ? 0x7fffffff - step : (int)len;
+    r.n_split = pass == DKV ? (int)n : (walk + r.split_len - 1) / r.split_len;
     if (r.n_split < 1) r.n_split = 1;
-    if (r.split_len < 1) r.split_len = r.s.walk_tile;
     r.blocks = base * r.n_split;
     return r;
 }
@@ -621,16 +1043,25 @@ int64_t part_floats(const AttnP& p, Pass pass, int n_split) {
     return pass == DQ ? (int64_t)n_split * p.B * p.Lq * p.H * p.D : 2 * (int64_t)n_split * p.B * p.Lk * p.Hkv * p.D;
 }
 
-const char* launch(AttnP p, Pass pass, const Plan& r, hipStream_t s) {
+const char* launch(AttnP p, const Plan& r, hipStream_t s) {
     p.n_col_tile = r.n_col_tile;
     p.n_split = r.n_split;
     p.split_len = r.split_len;
-    p.xcd = r.n_bh % 8 == 0 && (int64_t)r.n_col_tile * r.n_split > 1;
-    if (r.blocks <= 0) return nullptr;
-    if (r.blocks > 0x7fffffff) return "too many workgroups (batch x heads x tiles > 2^31)";
-    r.s.kernel<<<dim3((unsigned)r.blocks), dim3(r.s.threads), 0, s>>>(p);
+    p.wpp = r.wpp;
+    p.tile_major = p.causal && !r.s.few && r.n_bh * r.n_split < 64;
+    int64_t blocks = r.blocks;
+    if (blocks <= 0) return nullptr;
+    if (r.s.few)
+        blocks = r.wpp > 1 ? blocks : (blocks + 3) / 4;
+    else if (!p.tile_major)
+        blocks = (blocks + 7) / 8 * 8;
+    if (blocks > 0x7fffff00) return "too many workgroups (batch x heads x tiles > 2^31)";
+    r.s.kernel<<<dim3((unsigned)blocks), dim3(r.s.threads), 0, s>>>(p);
     return nullptr;
 }
+
+// both axes within one wave's reach: the whole backward pass is one kernel, as far as its operands fit the registers
+bool small(const AttnP& p) { return p.Lq >= 1 && p.Lk >= 1 && p.Lq <= 32 && p.Lk <= 32 && p.D <= (p.dtype == 1 ? 64 : 32); }
 
 template <typename T>
 void launch_sum(const float* part, int n_split, int B, int L, int H, int D, void* dst, const int64_t* st, hipStream_t s) {
@@ -642,6 +1073,7 @@ void launch_sum(const float* part, int n_split, int B, int L, int H, int D, void
 
 int64_t attention_workspace(const AttnP& p, bool backward) {
     if (!backward) return 4 * part_floats(p, FWD, plan(p, FWD).n_split);
+    if (small(p)) return 0;
     const int64_t a = part_floats(p, DQ, plan(p, DQ).n_split), b = part_floats(p, DKV, plan(p, DKV).n_split);
     return 4 * ((int64_t)p.B * p.H * p.Lq + (a > b ? a : b));  // delta, and the parts of one pass after the other
 }
@@ -652,7 +1084,7 @@ const char* run_attention(AttnP p, float* ws, hipStream_t s) {
     if (rows == 0) return nullptr;
     p.part = ws;
     p.part_lse = ws + (int64_t)r.n_split * rows * p.D;
-    if (const char* e = launch(p, FWD, r, s)) return e;
+    if (const char* e = launch(p, r, s)) return e;
     if (r.n_split > 1) {
         p.n_split = r.n_split;
         const unsigned blocks = (unsigned)((rows * ((p.D + 3) / 4) + 255) / 256);
@@ -665,17 +1097,24 @@ const char* run_attention(AttnP p, float* ws, hipStream_t s) {
 }
 
 const char* run_attention_backward(AttnP p, float* ws, hipStream_t s) {
+    if (small(p)) {
+        const int64_t blocks = ((int64_t)p.B * p.Hkv + 3) / 4;
+        if (blocks > 0x7fffff00) return "too many workgroups (batch x heads > 2^33)";
+        auto kernel = p.dtype == 1 ? (p.D <= 32 ? k_attn_bwd_small<bf16, 32> : k_attn_bwd_small<bf16, 64>) : k_attn_bwd_small<float, 32>;
+        if (blocks) kernel<<<dim3((unsigned)blocks), dim3(256), 0, s>>>(p);
+        return nullptr;
+    }
     p.delta = ws;
     p.part = ws + (int64_t)p.B * p.H * p.Lq;
     const Plan a = plan(p, DQ), b = plan(p, DKV);
-    if (const char* e = launch(p, DQ, a, s)) return e;
+    if (const char* e = launch(p, a, s)) return e;
     if (a.n_split > 1 && p.Lq > 0) {
         if (p.dtype == 1)
             launch_sum<bf16>(p.part, a.n_split, p.B, p.Lq, p.H, p.D, p.dq, p.dqs, s);
         else
             launch_sum<float>(p.part, a.n_split, p.B, p.Lq, p.H, p.D, p.dq, p.dqs, s);
     }
-    if (const char* e = launch(p, DKV, b, s)) return e;
+    if (const char* e = launch(p, b, s)) return e;
     if (b.n_split > 1 && p.Lk > 0) {
         const float* pv = p.part + (int64_t)b.n_split * p.B * p.Lk * p.Hkv * p.D;
         if (p.dtype == 1) {

@@ -20,47 +20,64 @@ namespace {
 enum Kind { FWD, DX, DW };
 
 // A tile of ROWS x COLS elements (a multiple of 8 columns) between global memory and LDS
-template <typename T, int ROWS, int COLS, int NT, bool GATED>
+template <typename T, int ROWS, int COLS, int NT, bool GATED, bool NARROW>
 struct Tile {
-    static constexpr int NP = Planes<T>::N, CH = COLS / 8, PT = (ROWS * CH + NT - 1) / NT, LD = COLS + LDS_PAD;
-    static_assert(NT % CH == 0, "a thread's chunks share their columns");
+    static constexpr int NP = Planes<T>::N, CH = COLS / 8, PT = ROWS * CH / NT, LD = COLS + LDS_PAD;
+    static_assert(NT % CH == 0 && ROWS * CH % NT == 0, "a thread's chunks are whole and share their columns");
     Held<T> r[PT];
     Held<T> gate[GATED ? PT : 1];
-    // rows row0 .. of a [., ld] matrix up to row_end, columns col0 .. up to col_end; what lies outside, or in an invalid row, is zero
-    __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t row0, int64_t row_end, int col0, int col_end, const uint8_t* valid, const T* act, int tid) {
+    uint8_t ok[PT];
+    int rows, col_left, shift;
+    // rows row0 .. (row0 < row_end) of a [., ld] matrix up to row_end, columns col0 .. (col0 < col_end) up to col_end; what lies outside, or in an
+    // invalid row, becomes zero
+    __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t row0, int64_t row_end, int col0, int col_end, const Valid& valid, const T* act, int tid) {
+        const int col = col0 + (tid % CH) * 8, cc = NARROW ? col < col_end ? col : col0 : chunk_start(col, col_end);
 #pragma unroll
         for (int c = 0; c < PT; ++c) {
-            const int idx = tid + c * NT, col = col0 + (idx % CH) * 8;
-            const int64_t row = row0 + idx / CH;
-            r[c].zero();
-            if constexpr (GATED) gate[c].zero();
-            if (idx < ROWS * CH && row < row_end && col < col_end) {
-                r[c].load(base + row * ld + col, col_end - col);
-                if constexpr (GATED)
-                    if (act) gate[c].load(act + row * ld + col, col_end - col);
-                if (valid && !valid[row]) r[c].zero();
+            const int64_t row = row0 + (tid + c * NT) / CH, rc = row < row_end ? row : row_end - 1;
+            if constexpr (NARROW)
+                r[c].load_narrow(base + rc * ld + cc, col_end - cc);
+            else
+                r[c].load(base + rc * ld + cc);
+            if constexpr (GATED) {
+                if constexpr (NARROW)
+                    gate[c].load_narrow(act + rc * ld + cc, col_end - cc);
+                else
+                    gate[c].load(act + rc * ld + cc);
+            }
+            ok[c] = valid[rc];
+        }
+        rows = row_end - row0 < ROWS ? (int)(row_end - row0) : ROWS;
+        col_left = col_end - col;
+        shift = col - cc;
+    }
+    // the ends of rows, the masks and the activation's gradient, where the loads are waited for
+    __device__ __forceinline__ void settle(bool ragged, int tid) {
+        if (!NARROW && ragged) {
+#pragma unroll
+            for (int c = 0; c < PT; ++c) {
+                r[c].fit(shift);
+                if constexpr (GATED) gate[c].fit(shift);
             }
         }
-    }
-    __device__ __forceinline__ void apply_gate() {
         if constexpr (GATED) {
 #pragma unroll
             for (int c = 0; c < PT; ++c)
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (!(gate[c].get(j) > 0.f)) r[c].set(j, 0.f);
+                    if (!(gate[c].get(j) > 0.f)) r[c].drop(j);
         }
+#pragma unroll
+        for (int c = 0; c < PT; ++c) r[c].keep(ok[c] && (tid + c * NT) / CH < rows && col_left > 0);
     }
     __device__ __forceinline__ void store(bf16* lds, int tid) const {
 #pragma unroll
         for (int c = 0; c < PT; ++c) {
             const int idx = tid + c * NT;
-            if (ROWS * CH % NT == 0 || idx < ROWS * CH) {
-                bf16x8 pl[NP];
-                r[c].planes(pl);
+            bf16x8 pl[NP];
+            r[c].planes(pl);
 #pragma unroll
-                for (int n = 0; n < NP; ++n) *reinterpret_cast<bf16x8*>(lds + (size_t)n * ROWS * LD + (idx / CH) * LD + (idx % CH) * 8) = pl[n];
-            }
+            for (int n = 0; n < NP; ++n) *reinterpret_cast<bf16x8*>(lds + (size_t)n * ROWS * LD + (idx / CH) * LD + (idx % CH) * 8) = pl[n];
         }
     }
     __device__ __forceinline__ void add_columns(float (&s)[8]) const {
@@ -71,7 +88,8 @@ struct Tile {
     }
 };
 
-template <typename T, Kind KIND, int TR, int TC, int WR, int WC, int KB>
+// GATED: with the activation's gradient.  NARROW: an operand's rows have fewer than 8 elements.
+template <typename T, Kind KIND, bool GATED, int TR, int TC, int WR, int WC, int KB, bool NARROW>
 __global__ __launch_bounds__(64 * WR * WC) void k_linear(const LinearP p) {
     constexpr int NP = Planes<T>::N, NT = 64 * WR * WC, MR = TR / WR / 16, MC = TC / WC / 16;
     constexpr bool AT = KIND != FWD, BT = KIND == DW;  // contraction across memory
@@ -94,22 +112,24 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear(const LinearP p) {
     const int64_t Kn = KIND == FWD ? p.K : KIND == DX ? p.N : p.M;           // extent of the contraction
     const T* A = KIND == DW ? (const T*)p.x : (const T*)p.weight;
     const T* B = KIND == FWD ? (const T*)p.x : (const T*)p.d_out;
-    const T* act = KIND == FWD ? nullptr : (const T*)p.act;
+    const T* act = GATED ? (const T*)p.act : nullptr;
     const int64_t lda = p.K, ldb = KIND == FWD ? p.K : p.N;
 
-    Tile<T, AR, AC, NT, false> ta;
-    Tile<T, BR, BC, NT, KIND != FWD> tb;
+    Tile<T, AR, AC, NT, false, NARROW> ta;
+    Tile<T, BR, BC, NT, GATED, NARROW> tb;
     int64_t k0 = (int64_t)split * p.split_len;
     const int64_t kend = KIND == DW ? (k0 + p.split_len < Kn ? k0 + p.split_len : Kn) : Kn;
+    const bool ragged_a = lda % 8 != 0, ragged_b = ldb % 8 != 0;
+    const Valid rows_valid(p.row_valid, 0), all(nullptr, 0);
     auto load = [&](int64_t k) {
         if constexpr (AT)
-            ta.load(A, lda, k, kend, r0, R, KIND == DW ? p.row_valid : nullptr, nullptr, tid);
+            ta.load(A, lda, k, kend, r0, R, KIND == DW ? rows_valid : all, nullptr, tid);
         else
-            ta.load(A, lda, r0, R, (int)k, (int)kend, nullptr, nullptr, tid);
+            ta.load(A, lda, r0, R, (int)k, (int)kend, all, nullptr, tid);
         if constexpr (BT)
-            tb.load(B, ldb, k, kend, (int)c0, (int)Cn, p.row_valid, act, tid);
+            tb.load(B, ldb, k, kend, (int)c0, (int)Cn, rows_valid, act, tid);
         else
-            tb.load(B, ldb, c0, Cn, (int)k, (int)kend, p.row_valid, act, tid);
+            tb.load(B, ldb, c0, Cn, (int)k, (int)kend, rows_valid, act, tid);
     };
     f32x4 acc[MC][MR];
 #pragma unroll
@@ -119,7 +139,8 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear(const LinearP p) {
     float sums[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (k0 < kend) load(k0);
     for (; k0 < kend; k0 += KB) {
-        if (act) tb.apply_gate();
+        ta.settle(ragged_a, tid);
+        tb.settle(ragged_b, tid);
         if (KIND == DW && rt == 0) tb.add_columns(sums);
         __syncthreads();
         ta.store(la, tid);
@@ -175,7 +196,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear(const LinearP p) {
                 store4((T*)p.dx + at, n, v);
             } else {
                 if (p.n_split > 1)
-                    store4(p.part + (int64_t)split * p.N * p.K + at, n, v);
+                    store4(p.part + split * ((int64_t)p.N * p.K + p.N) + at, n, v);
                 else if (p.dw)
                     store4((T*)p.dw + at, n, v);
             }
@@ -195,7 +216,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear(const LinearP p) {
                     float s = 0.f;
                     for (int k = 0; k < RT; ++k) s += red[k * TC + c];
                     if (p.n_split > 1)
-                        p.part[(int64_t)p.n_split * p.N * p.K + (int64_t)split * p.N + c0 + c] = s;
+                        p.part[split * ((int64_t)p.N * p.K + p.N) + (int64_t)p.N * p.K + c0 + c] = s;
                     else
                         ((T*)p.db)[c0 + c] = (T)s;
                 }
@@ -203,42 +224,61 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear(const LinearP p) {
     }
 }
 
-// dst[i] = sum over the splits, in split order
+// [dW, db][i] = sum over the splits of part[split][N K + N], always in the same order: 16 groups of 4 elements x 16 lanes over the splits
 template <typename T>
-__global__ __launch_bounds__(256) void k_linear_sum(const float* part, int n_split, int64_t n, T* dst) {
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i >= n) return;
+__global__ __launch_bounds__(256) void k_linear_sum(const float* part, int n_split, int64_t n_w, int n_b, T* dw, T* db) {
+    __shared__ __attribute__((aligned(16))) f32x4 red[16][17];
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int64_t n = n_w + n_b, i = ((int64_t)blockIdx.x * 16 + tx) * 4;
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
-    const int m = n - i < 4 ? (int)(n - i) : 4;
-    for (int k = 0; k < n_split; ++k) {
-        const float* src = part + k * n + i;
-        if (m == 4) {
+    if (i + 4 <= n) {
+        for (int k = ty; k < n_split; k += 16) {
             f32x4 v;
-            __builtin_memcpy(&v, src, 16);
+            __builtin_memcpy(&v, part + k * n + i, 16);
             s += v;
-        } else {
+        }
+    } else {
+        for (int k = ty; k < n_split; k += 16)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (e < m) s[e] += src[e];
+                if (i + e < n) s[e] += part[k * n + i + e];
+    }
+    red[ty][tx] = s;
+    __syncthreads();
+    if (ty) return;
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += red[k][tx];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (i + e < n_w) {
+            if (dw) dw[i + e] = (T)s[e];
+        } else if (i + e < n && db) {
+            db[i + e - n_w] = (T)s[e];
         }
     }
-    store4(dst + i, m, s);
 }
 
 struct Shape {
     void (*kernel)(LinearP);
     int tr, tc, kb, threads;
 };
-template <typename T, Kind KIND, int TR, int TC, int WR, int WC, int KB>
+template <typename T, Kind KIND, bool GATED, int TR, int TC, int WR, int WC, bool NARROW>
 Shape shape() {
-    return {k_linear<T, KIND, TR, TC, WR, WC, KB>, TR, TC, KB, 64 * WR * WC};
+    constexpr int KB = sizeof(T) == 2 ? 64 : 32;
+    return {k_linear<T, KIND, GATED, TR, TC, WR, WC, KB, NARROW>, TR, TC, KB, 64 * WR * WC};
+}
+template <typename T, Kind KIND, bool GATED>
+Shape choose(const LinearP& p, int64_t r, int64_t c) {
+    if (p.K < 8 || (KIND != FWD && p.N < 8)) return shape<T, KIND, GATED, 64, 64, 2, 2, true>();
+    // 128 x 128 tiles feed the matrix cores best; below one such tile per CU the smaller ones spread the work
+    if (KIND == DW ? r > 64 || c > 64 : (r + 127) / 128 * ((c + 127) / 128) >= 256) return shape<T, KIND, GATED, 128, 128, 2, 2, false>();
+    return shape<T, KIND, GATED, 64, 64, 2, 2, false>();
 }
 template <typename T, Kind KIND>
-Shape choose(int64_t r, int64_t c) {
-    constexpr int KB = sizeof(T) == 2 ? 64 : 32;
-    // 128 x 128 tiles feed the matrix cores best; below one such tile per CU the smaller ones spread the work
-    if (KIND == DW ? r > 64 || c > 64 : (r + 127) / 128 * ((c + 127) / 128) >= 256) return shape<T, KIND, 128, 128, 2, 2, KB>();
-    return shape<T, KIND, 64, 64, 2, 2, KB>();
+Shape choose(const LinearP& p, int64_t r, int64_t c) {
+    if constexpr (KIND != FWD)
+        if (p.act) return choose<T, KIND, true>(p, r, c);
+    return choose<T, KIND, false>(p, r, c);
 }
 
 struct Plan {
@@ -251,7 +291,7 @@ Plan plan(const LinearP& p) {
     Plan r;
     r.p = p;
     const int64_t R = KIND == FWD ? p.N : p.K, C = KIND == DW ? p.N : p.M;
-    r.s = p.dtype == 1 ? choose<bf16, KIND>(R, C) : choose<float, KIND>(R, C);
+    r.s = p.dtype == 1 ? choose<bf16, KIND>(p, R, C) : choose<float, KIND>(p, R, C);
     r.p.n_rt = (int)((R + r.s.tr - 1) / r.s.tr);
     r.p.n_ct = (C + r.s.tc - 1) / r.s.tc;
     r.p.n_split = 1;
@@ -277,8 +317,9 @@ const char* launch(const Plan& r, hipStream_t s) {
 }
 
 template <typename T>
-void launch_sum(const float* part, int n_split, int64_t n, void* dst, hipStream_t s) {
-    k_linear_sum<T><<<dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, s>>>(part, n_split, n, (T*)dst);
+void launch_sum(const LinearP& p, int n_split, hipStream_t s) {
+    const int64_t n = (int64_t)p.N * p.K;
+    k_linear_sum<T><<<dim3((unsigned)((n + p.N + 63) / 64)), dim3(256), 0, s>>>(p.part, n_split, n, p.N, (T*)p.dw, (T*)p.db);
 }
 
 }  // namespace
@@ -298,15 +339,10 @@ const char* run_linear_backward(LinearP p, float* ws, hipStream_t s) {
     const Plan r = plan<DW>(p);
     if (const char* e = launch(r, s)) return e;
     if (r.p.n_split > 1) {
-        const int64_t n = (int64_t)p.N * p.K;
-        const float* pb = ws + r.p.n_split * n;
-        if (p.dtype == 1) {
-            if (p.dw) launch_sum<bf16>(ws, r.p.n_split, n, p.dw, s);
-            if (p.db) launch_sum<bf16>(pb, r.p.n_split, p.N, p.db, s);
-        } else {
-            if (p.dw) launch_sum<float>(ws, r.p.n_split, n, p.dw, s);
-            if (p.db) launch_sum<float>(pb, r.p.n_split, p.N, p.db, s);
-        }
+        if (p.dtype == 1)
+            launch_sum<bf16>(p, r.p.n_split, s);
+        else
+            launch_sum<float>(p, r.p.n_split, s);
     }
     return nullptr;
 }

@@ -19,18 +19,34 @@ constexpr int NT = 256;
 template <typename T>
 constexpr int VEC = 16 / sizeof(T);
 
-template <typename T>
-__device__ __forceinline__ void load_chunk(const T* p, int n, float (&x)[VEC<T>]) {
+// Chunk `col` .. of a row of C elements, in two steps (see Held in tb_ops.hpp): an unconditional load from inside the row, and fit_chunk where the
+// row ends inside the chunk or in front of it.  NARROW: C < the chunk, single loads.
+template <typename T, bool NARROW>
+__device__ __forceinline__ void load_chunk(const T* row, int col, int C, float (&x)[VEC<T>]) {
     typedef T vec __attribute__((ext_vector_type(VEC<T>)));
-    vec v;
-    if (n >= VEC<T>) {
-        __builtin_memcpy(&v, p, 16);
+    if constexpr (NARROW) {
+#pragma unroll
+        for (int j = 0; j < VEC<T>; ++j) x[j] = col + j < C ? (float)row[col + j] : 0.f;
     } else {
+        vec v;
+        __builtin_memcpy(&v, row + min(col, C - VEC<T>), 16);
 #pragma unroll
-        for (int j = 0; j < VEC<T>; ++j) v[j] = j < n ? p[j] : (T)0.f;
+        for (int j = 0; j < VEC<T>; ++j) x[j] = (float)v[j];
     }
+}
+template <typename T, bool NARROW>
+__device__ __forceinline__ void fit_chunk(int col, int C, bool ragged, float (&x)[VEC<T>]) {
+    if constexpr (!NARROW) {
+        if (ragged) {  // (uniform)
+            const int shift = col - min(col, C - VEC<T>);
 #pragma unroll
-    for (int j = 0; j < VEC<T>; ++j) x[j] = (float)v[j];
+            for (int s = VEC<T> / 2; s; s >>= 1)
+#pragma unroll
+                for (int j = 0; j < VEC<T>; ++j) x[j] = shift & s ? (j + s < VEC<T> ? x[j + s] : 0.f) : x[j];
+        }
+#pragma unroll
+        for (int j = 0; j < VEC<T>; ++j) x[j] = col < C ? x[j] : 0.f;
+    }
 }
 
 template <typename T>
@@ -64,22 +80,21 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
     return v;
 }
 
-template <typename T, int LPR, int NV>
+template <typename T, int LPR, int NV, bool NARROW>
 __global__ __launch_bounds__(NT) void k_norm_fwd(const NormP p) {
     constexpr int V = VEC<T>, RPB = NT / LPR;
     __shared__ float red[4];
     const int lr = threadIdx.x % LPR;
     const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
-    const bool on = row < p.rows;
-    const T* x = (const T*)p.x + row * p.C;
+    const bool on = row < p.rows, ragged = p.C % V != 0;
+    const T* x = (const T*)p.x + (on ? row : p.rows - 1) * p.C;
     float v[NV][V];
     float s = 0.f;
 #pragma unroll
-    for (int c = 0; c < NV; ++c) {
-        const int col = (c * LPR + lr) * V;
+    for (int c = 0; c < NV; ++c) load_chunk<T, NARROW>(x, (c * LPR + lr) * V, p.C, v[c]);
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[c][j] = 0.f;
-        if (on && col < p.C) load_chunk<T>(x + col, p.C - col, v[c]);
+    for (int c = 0; c < NV; ++c) {
+        fit_chunk<T, NARROW>((c * LPR + lr) * V, p.C, ragged, v[c]);
 #pragma unroll
         for (int j = 0; j < V; ++j) s += v[c][j];
     }
@@ -102,8 +117,14 @@ __global__ __launch_bounds__(NT) void k_norm_fwd(const NormP p) {
         float g[V], b[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) g[j] = 1.f, b[j] = 0.f;
-        if (p.weight) load_chunk<T>((const T*)p.weight + col, p.C - col, g);
-        if (p.bias) load_chunk<T>((const T*)p.bias + col, p.C - col, b);
+        if (p.weight) {
+            load_chunk<T, NARROW>((const T*)p.weight, col, p.C, g);
+            fit_chunk<T, NARROW>(col, p.C, ragged, g);
+        }
+        if (p.bias) {
+            load_chunk<T, NARROW>((const T*)p.bias, col, p.C, b);
+            fit_chunk<T, NARROW>(col, p.C, ragged, b);
+        }
 #pragma unroll
         for (int j = 0; j < V; ++j) v[c][j] = __builtin_fmaf(v[c][j] * rstd, g[j], b[j]);
         store_chunk<T>(y + col, p.C - col, v[c]);
@@ -114,47 +135,51 @@ __global__ __launch_bounds__(NT) void k_norm_fwd(const NormP p) {
     }
 }
 
-template <typename T, int LPR, int NV>
+template <typename T, int LPR, int NV, bool NARROW>
 __global__ __launch_bounds__(NT) void k_norm_bwd(const NormP p) {
     constexpr int V = VEC<T>, RPB = NT / LPR;
     __shared__ float red[4];
     __shared__ float part[LPR > 64 ? 1 : 2 * 4 * LPR * V];
     const int lr = threadIdx.x % LPR;
+    const bool ragged = p.C % V != 0;
     float g[NV][V], dg[NV][V], db[NV][V];
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
         const int col = (c * LPR + lr) * V;
 #pragma unroll
         for (int j = 0; j < V; ++j) g[c][j] = 1.f, dg[c][j] = db[c][j] = 0.f;
-        if (p.weight && col < p.C) load_chunk<T>((const T*)p.weight + col, p.C - col, g[c]);
+        if (p.weight) {
+            load_chunk<T, NARROW>((const T*)p.weight, col, p.C, g[c]);
+            fit_chunk<T, NARROW>(col, p.C, ragged, g[c]);
+        }
     }
     const float inv = 1.f / (float)p.C;
     for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < p.rows; r0 += (int64_t)gridDim.x * RPB) {  // (workgroup-uniform trip count: row_sum may hold barriers)
         const int64_t row = r0 + threadIdx.x / LPR;
         const bool on = row < p.rows;
-        const float mean = on ? p.mean[row] : 0.f, rstd = on ? p.rstd[row] : 0.f;
+        const int64_t rc = on ? row : p.rows - 1;
+        const float mean = p.mean[rc], rstd = p.rstd[rc];
         float h[NV][V], a[NV][V], s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
-            const int col = (c * LPR + lr) * V;
-#pragma unroll
-            for (int j = 0; j < V; ++j) h[c][j] = a[c][j] = 0.f;
-            if (on && col < p.C) {
-                load_chunk<T>((const T*)p.x + row * p.C + col, p.C - col, h[c]);
-                load_chunk<T>((const T*)p.d_out + row * p.C + col, p.C - col, a[c]);
-            }
+            load_chunk<T, NARROW>((const T*)p.x + rc * p.C, (c * LPR + lr) * V, p.C, h[c]);
+            load_chunk<T, NARROW>((const T*)p.d_out + rc * p.C, (c * LPR + lr) * V, p.C, a[c]);
         }
 #pragma unroll
-        for (int c = 0; c < NV; ++c)
+        for (int c = 0; c < NV; ++c) {
+            fit_chunk<T, NARROW>((c * LPR + lr) * V, p.C, ragged, h[c]);
+            fit_chunk<T, NARROW>((c * LPR + lr) * V, p.C, ragged, a[c]);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 h[c][j] = (h[c][j] - mean) * rstd;
+                a[c][j] = on ? a[c][j] : 0.f;
                 db[c][j] += a[c][j];
                 dg[c][j] = __builtin_fmaf(a[c][j], h[c][j], dg[c][j]);
                 a[c][j] *= g[c][j];  // (columns past C hold dy = 0: they add nothing)
                 s1 += a[c][j];
                 s2 = __builtin_fmaf(a[c][j], h[c][j], s2);
             }
+        }
         s1 = row_sum<LPR>(s1, red) * inv;
         s2 = row_sum<LPR>(s2, red) * inv;
         if (on && p.dx) {
@@ -237,13 +262,14 @@ struct Shape {
     Kernel fwd, bwd;
     int rows;  // per workgroup and step
 };
-template <typename T, int LPR, int NV>
+template <typename T, int LPR, int NV, bool NARROW = false>
 Shape shape() {
-    return {k_norm_fwd<T, LPR, NV>, k_norm_bwd<T, LPR, NV>, NT / LPR};
+    return {k_norm_fwd<T, LPR, NV, NARROW>, k_norm_bwd<T, LPR, NV, NARROW>, NT / LPR};
 }
 template <typename T>
 Shape choose(int C) {
     const int n = (C + VEC<T> - 1) / VEC<T>;  // 16-byte chunks of a row
+    if (C < VEC<T>) return shape<T, 8, 1, true>();
     if (n <= 8) return shape<T, 8, 1>();
     if (n <= 16) return shape<T, 16, 1>();
     if (n <= 32) return shape<T, 32, 1>();

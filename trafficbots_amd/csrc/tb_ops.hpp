@@ -75,64 +75,74 @@ __device__ __forceinline__ void to_planes(const float (&x)[8], bf16x8 (&p)[NP]) 
     }
 }
 
-// ---- global memory: 8 consecutive elements of a row, the first `n` of them inside it (n >= 8: all).  Rows may start at any element:
-// gfx950 loads 16 bytes from any address, so odd widths and strides take the same path as aligned ones.
-struct Raw8f {
-    float x[8];
-};
-__device__ __forceinline__ void load8(const float* p, int n, float (&x)[8]) {
-    if (n >= 8) {
-        __builtin_memcpy(x, p, 32);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = j < n ? p[j] : 0.f;
-    }
-}
-__device__ __forceinline__ void load8(const bf16* p, int n, float (&x)[8]) {
-    bf16x8 v;
-    if (n >= 8) {
-        __builtin_memcpy(&v, p, 16);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : (bf16)0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = (float)v[j];
-}
-
-// the same 8 elements as they are held between the load and the LDS write of a staged tile: fp32 or packed bf16
+// ---- global memory: 8 consecutive elements of a row, as they are held between the load and their use (fp32, or packed bf16).  Rows may start
+// at any element: gfx950 loads 16 bytes from any address, so odd widths and strides take the same path as aligned ones.
+// Loads are unconditional and whole: a branch around a load makes the compiler wait for it at the branch's end, which cost 1 us for every
+// load of a walk.  The caller clamps a row or column that is out of range or masked to one that is there (chunk_start), and what does not
+// belong is dropped where the data is used: fit() moves the end of a row that is no multiple of 8 (`ragged`, uniform over the launch) to
+// the chunk's front, keep(false) makes the chunk zero.  Rows of fewer than 8 elements take single loads (load_narrow).
 template <typename T>
 struct Held;
 template <>
 struct Held<float> {
     float x[8];
-    __device__ __forceinline__ void zero() {
+    __device__ __forceinline__ void load(const float* p) { __builtin_memcpy(x, p, 32); }
+    __device__ __forceinline__ void load_narrow(const float* p, int n) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = 0.f;
+        for (int j = 0; j < 8; ++j) x[j] = j < n ? p[j] : 0.f;
     }
-    __device__ __forceinline__ void load(const float* p, int n) { load8(p, n, x); }
+    __device__ __forceinline__ void fit(int shift) {
+#pragma unroll
+        for (int s = 4; s; s >>= 1)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = shift & s ? (j + s < 8 ? x[j + s] : 0.f) : x[j];
+    }
+    __device__ __forceinline__ void keep(bool on) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = on ? x[j] : 0.f;
+    }
     __device__ __forceinline__ float get(int j) const { return x[j]; }
-    __device__ __forceinline__ void set(int j, float v) { x[j] = v; }
+    __device__ __forceinline__ void drop(int j) { x[j] = 0.f; }
     __device__ __forceinline__ void planes(bf16x8 (&p)[3]) const { to_planes<3>(x, p); }
 };
 template <>
 struct Held<bf16> {
-    bf16x8 v;
-    __device__ __forceinline__ void zero() {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 u;
+    __device__ __forceinline__ void load(const bf16* p) { __builtin_memcpy(&u, p, 16); }
+    __device__ __forceinline__ void load_narrow(const bf16* p, int n) {
+        bf16x8 v;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = (bf16)0.f;
+        for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : (bf16)0.f;
+        u = __builtin_bit_cast(u32x4, v);
     }
-    __device__ __forceinline__ void load(const bf16* p, int n) {
-        if (n >= 8) {
-            __builtin_memcpy(&v, p, 16);
-        } else {
+    __device__ __forceinline__ void fit(int shift) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : (bf16)0.f;
-        }
+        for (int s = 2; s; s >>= 1)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[j] = shift & 2 * s ? (j + s < 4 ? u[j + s] : 0u) : u[j];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = shift & 1 ? u[j] >> 16 | (j < 3 ? u[j + 1] << 16 : 0u) : u[j];
     }
-    __device__ __forceinline__ float get(int j) const { return (float)v[j]; }
-    __device__ __forceinline__ void set(int j, float f) { v[j] = (bf16)f; }
-    __device__ __forceinline__ void planes(bf16x8 (&p)[1]) const { p[0] = v; }
+    __device__ __forceinline__ void keep(bool on) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = on ? u[j] : 0u;
+    }
+    __device__ __forceinline__ float get(int j) const { return __builtin_bit_cast(float, j & 1 ? u[j / 2] & 0xffff0000u : u[j / 2] << 16); }
+    __device__ __forceinline__ void drop(int j) { u[j / 2] &= j & 1 ? 0x0000ffffu : 0xffff0000u; }
+    __device__ __forceinline__ void planes(bf16x8 (&p)[1]) const { p[0] = __builtin_bit_cast(bf16x8, u); }
+};
+
+// where the chunk of columns col .. col + 7 of rows of `width` >= 8 elements is loaded from; fit()'s shift is what it lies behind `col`
+__device__ __forceinline__ int chunk_start(int col, int width) { return min(col, width - 8); }
+
+// a validity mask that may be absent: then one byte that says yes, read with stride 0 (no branch around the load)
+__device__ const uint8_t YES = 1;
+struct Valid {
+    const uint8_t* p;
+    int64_t step;
+    __device__ __forceinline__ Valid(const uint8_t* mask, int64_t at) : p(mask ? mask + at : &YES), step(mask ? 1 : 0) {}
+    __device__ __forceinline__ uint8_t operator[](int64_t i) const { return p[i * step]; }
 };
 
 // 4 consecutive results of a row, the first `n` of them inside it

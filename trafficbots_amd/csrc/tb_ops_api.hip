@@ -36,7 +36,7 @@ const char* sizes(const tb_attention_io& io) {
     if (io.n_query > MAX_LEN || io.n_key > MAX_LEN) return "more than 2^30 queries or keys";
     if (io.n_head < 1 || io.n_kv_head < 1 || io.n_head % io.n_kv_head) return "n_head must be a positive multiple of n_kv_head";
     if ((int64_t)io.n_batch * io.n_head > MAX_LEN) return "more than 2^30 heads in the batch";
-    if (io.head_dim < 1 || io.head_dim > 128) return "head_dim must be 1 .. 128";
+    if (io.head_dim < 8 || io.head_dim > 128) return "head_dim must be 8 .. 128";
     return nullptr;
 }
 const char* sizes(const tb_layer_norm_io& io) {
@@ -59,7 +59,7 @@ void copy3(int64_t (&dst)[3], const int64_t (&src)[3]) {
 AttnP params(const tb_attention_io& io) {
     AttnP p = {};
     p.dtype = io.dtype;
-    p.B = io.n_batch, p.Lq = io.n_query, p.Lk = io.n_key, p.H = io.n_head, p.Hkv = io.n_kv_head, p.G = io.n_head / io.n_kv_head, p.D = io.head_dim;
+    p.B = io.n_batch, p.Lq = io.n_query, p.Lk = io.n_key, p.H = io.n_head, p.Hkv = io.n_kv_head, p.G = io.n_head / io.n_kv_head, p.D = io.head_dim, p.ragged = io.head_dim % 8 != 0;
     p.causal = io.causal != 0;
     p.scale = io.scale;
     p.scale2 = (float)((double)io.scale * 1.4426950408889634);

@@ -9,7 +9,7 @@ namespace op {
 
 struct AttnP {
     int dtype;  // 0 fp32, 1 bf16
-    int B, Lq, Lk, H, Hkv, G, D, causal;
+    int B, Lq, Lk, H, Hkv, G, D, causal, ragged;  // ragged: D is no multiple of 8
     float scale, scale2;  // scale2 = scale * log2(e): the softmax works in powers of two
     const void *q, *k, *v, *d_out;
     int64_t qs[3], ks[3], vs[3], os[3], dos[3], dqs[3], dks[3], dvs[3];  // elements over (batch, position, head)
@@ -18,7 +18,7 @@ struct AttnP {
     void *out, *dq, *dk, *dv;
     float *lse, *delta;
     // of one launch
-    int n_col_tile, n_split, split_len, xcd;
+    int n_col_tile, n_split, split_len, wpp, tile_major;
     float *part, *part_lse;
 };
 int64_t attention_workspace(const AttnP& p, bool backward);
@@ -49,7 +49,7 @@ struct LinearP {
     // of one launch
     int n_rt, n_split;
     int64_t n_ct, split_len;
-    float* part;  // [n_split][N][K], then [n_split][N]
+    float* part;  // [n_split][N K + N]: dW, db
 };
 int64_t linear_workspace(const LinearP& p);
 const char* run_linear(const LinearP& p, hipStream_t s);

@@ -907,9 +907,6 @@ class HipEngine:
             raise ValueError(f"{what}: {name} on {m.device}, the engine's device is {self.device}")
         return m.view(torch.uint8) if m.dtype == torch.bool else m
 
-    def _scratch(self, n_bytes: int) -> Optional[Tensor]:
-        return torch.empty(n_bytes, device=self.device, dtype=torch.uint8) if n_bytes > 0 else None
-
     def _attention_io(self, what: str, q: Tensor, k: Tensor, v: Tensor, query_valid, key_valid, attn_mask, causal: bool, scale, *more: Tensor):
         for name, t in (("q", q), ("k", k), ("v", v)):
             if t.dim() != 4:
@@ -931,33 +928,27 @@ class HipEngine:
             io.attn_mask_strides[0] = am.stride(0) if am.dim() == 3 else 0
             io.attn_mask_strides[1] = am.stride(-2)
         io.query_valid, io.key_valid, io.attn_mask = (None if m is None else m.data_ptr() for m in (qv, kv, am))
-        keep = [qv, kv, am]
-        for name, t in (("q", q), ("k", k), ("v", v)):
-            keep.append(self._strided(io, name, t))
-        return io, keep
+        q, k, v = self._adjacent(q), self._adjacent(k), self._adjacent(v)
+        io.q, io.k, io.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+        io.q_strides, io.k_strides, io.v_strides = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+        return io, (q, k, v, qv, kv, am)
 
     @staticmethod
-    def _strided(io, name: str, t: Tensor) -> Tensor:
+    def _adjacent(t: Tensor) -> Tensor:
         """A [batch, length, heads, head_dim] tensor where it lies; only the components must be adjacent."""
-        if t.shape[3] > 1 and t.stride(3) != 1:
-            t = t.contiguous()
-        setattr(io, name, t.data_ptr())
-        st = getattr(io, name + "_strides")
-        st[0], st[1], st[2] = t.stride(0), t.stride(1), t.stride(2)
-        return t
+        return t if t.stride(3) == 1 or t.shape[3] < 2 else t.contiguous()
 
     def attention(self, q: Tensor, k: Tensor, v: Tensor, query_valid: Optional[Tensor] = None, key_valid: Optional[Tensor] = None,
                   attn_mask: Optional[Tensor] = None, causal: bool = False, scale: Optional[float] = None) -> Tuple[Tensor, Tensor]:
-        """`tb_attention`: attention of q [B, Lq, H, D] over k, v [B, Lk, Hkv, D] (H a multiple of Hkv, D <= 128; fp32 or bf16; strided
+        """`tb_attention`: attention of q [B, Lq, H, D] over k, v [B, Lk, Hkv, D] (H a multiple of Hkv, 8 <= D <= 128; fp32 or bf16; strided
         tensors are read where they lie).  `query_valid` [B, Lq] / `key_valid` [B, Lk]: what their zeros mark is not looked at.
         `attn_mask` [Lq, Lk] or [B, Lq, Lk]: True = may NOT attend (`attention.py:90-99`).  `causal`: key j for queries i >= j + Lq - Lk.
         `scale` defaults to 1 / sqrt(D).  Returns (out [B, Lq, H, D], lse [B, H, Lq] fp32); a query without a key gets 0 and -inf."""
         io, keep = self._attention_io("attention", q, k, v, query_valid, key_valid, attn_mask, causal, scale)
-        out = torch.empty(q.shape, device=self.device, dtype=q.dtype)
-        lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], device=self.device, dtype=torch.float32)
-        keep.append(self._strided(io, "out", out))
-        io.lse = lse.data_ptr()
-        self._run("tb_attention", io, False)
+        out = q.new_empty(q.shape)
+        lse = q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)
+        io.out, io.out_strides, io.lse = out.data_ptr(), out.stride()[:3], lse.data_ptr()
+        self._run("tb_attention", io, self.lib.tb_attention, self.lib.tb_attention_workspace_bytes(C.byref(io), 0))
         return out, lse
 
     def attention_backward(self, d_out: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, query_valid: Optional[Tensor] = None,
@@ -969,11 +960,12 @@ class HipEngine:
         if d_out.shape != q.shape or out.shape != q.shape:
             raise ValueError(f"attention_backward: d_out {tuple(d_out.shape)} and out {tuple(out.shape)} must have q's shape {tuple(q.shape)}")
         lse = self._f32("attention_backward", "lse", lse, (q.shape[0], q.shape[2], q.shape[1]))
-        dq, dk, dv = (torch.empty(t.shape, device=self.device, dtype=t.dtype) for t in (q, k, v))
-        for name, t in (("out", out), ("d_out", d_out), ("dq", dq), ("dk", dk), ("dv", dv)):
-            keep.append(self._strided(io, name, t))
-        io.lse = lse.data_ptr()
-        self._run("tb_attention_backward", io, True)
+        out, d_out = self._adjacent(out), self._adjacent(d_out)
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        io.out, io.out_strides, io.d_out, io.d_out_strides, io.lse = out.data_ptr(), out.stride()[:3], d_out.data_ptr(), d_out.stride()[:3], lse.data_ptr()
+        io.dq, io.dk, io.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        io.dq_strides, io.dk_strides, io.dv_strides = dq.stride()[:3], dk.stride()[:3], dv.stride()[:3]
+        self._run("tb_attention_backward", io, self.lib.tb_attention_backward, self.lib.tb_attention_workspace_bytes(C.byref(io), 1))
         return dq, dk, dv
 
     def _f32(self, what: str, name: str, t: Tensor, shape) -> Tensor:
@@ -981,22 +973,22 @@ class HipEngine:
             raise ValueError(f"{what}: {name} must be float32 {tuple(shape)} on {self.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
         return t.contiguous()
 
-    def _run(self, name: str, io, backward: bool) -> None:
-        """One call of a training operator on the current stream; its scratch lives on that stream, in torch's allocator."""
-        need = getattr(self.lib, name.replace("_backward", "") + "_workspace_bytes")(C.byref(io), int(backward))
-        ws = self._scratch(need)
-        if ws is not None:
+    def _run(self, name: str, io, call, need: int = 0) -> None:
+        """One call of a training operator on the current stream, with `need` bytes of scratch: it lives on that stream, in torch's allocator."""
+        if need > 0:
+            ws = torch.empty(need, device=self.device, dtype=torch.uint8)
             io.workspace, io.workspace_bytes = ws.data_ptr(), need
-        self._check(getattr(self.lib, name)(self._ctx, C.byref(io), self._stream()), name)
+        # (torch.cuda.current_stream builds a Stream object around this handle: 2 us of a call's 10)
+        self._check(call(self._ctx, C.byref(io), torch._C._cuda_getCurrentRawStream(self.device.index)), name)
 
     def layer_norm(self, x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5
                    ) -> Tuple[Tensor, Tensor, Tensor]:
         """`tb_layer_norm` over the last axis of x [..., C] (C <= 8192; fp32 or bf16): (y [..., C], mean [...], rstd [...], both fp32)."""
         io, x, keep = self._norm_io("layer_norm", x, weight, bias)
-        y = torch.empty(x.shape, device=self.device, dtype=x.dtype)
-        mean, rstd = (torch.empty(x.shape[:-1], device=self.device, dtype=torch.float32) for _ in range(2))
+        y = x.new_empty(x.shape)
+        mean, rstd = x.new_empty(x.shape[:-1], dtype=torch.float32), x.new_empty(x.shape[:-1], dtype=torch.float32)
         io.eps, io.y, io.mean, io.rstd = float(eps), y.data_ptr(), mean.data_ptr(), rstd.data_ptr()
-        self._run("tb_layer_norm", io, False)
+        self._run("tb_layer_norm", io, self.lib.tb_layer_norm)
         return y, mean, rstd
 
     def layer_norm_backward(self, d_out: Tensor, x: Tensor, weight: Optional[Tensor], mean: Tensor, rstd: Tensor, want_dx: bool = True,
@@ -1008,11 +1000,11 @@ class HipEngine:
             raise ValueError(f"{what}: d_out {tuple(d_out.shape)} must have x's shape {tuple(x.shape)}")
         d_out = d_out.contiguous()
         mean, rstd = self._f32(what, "mean", mean, x.shape[:-1]), self._f32(what, "rstd", rstd, x.shape[:-1])
-        dx = torch.empty(x.shape, device=self.device, dtype=x.dtype) if want_dx else None
-        dw, db = (torch.empty(x.shape[-1], device=self.device, dtype=x.dtype) if want_dweight else None for _ in range(2))
+        dx = x.new_empty(x.shape) if want_dx else None
+        dw, db = (x.new_empty(x.shape[-1:]), x.new_empty(x.shape[-1:])) if want_dweight else (None, None)
         io.d_out, io.mean, io.rstd = d_out.data_ptr(), mean.data_ptr(), rstd.data_ptr()
         io.dx, io.dweight, io.dbias = (None if t is None else t.data_ptr() for t in (dx, dw, db))
-        self._run("tb_layer_norm_backward", io, True)
+        self._run("tb_layer_norm_backward", io, self.lib.tb_layer_norm_backward, self.lib.tb_layer_norm_workspace_bytes(C.byref(io), 1) if want_dweight else 0)
         return dx, dw, db
 
     def _norm_io(self, what: str, x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], *more: Tensor):
@@ -1042,13 +1034,13 @@ class HipEngine:
                 raise ValueError(f"{what}: residual has shape {tuple(residual.shape)}, expected {shape}")
             residual = residual.contiguous()
             io.residual = residual.data_ptr()
-        y = torch.empty(shape, device=self.device, dtype=x.dtype)
+        y = x.new_empty(shape)
         io.y = y.data_ptr()
         act = y
         if want_act and residual is not None:
-            act = torch.empty(shape, device=self.device, dtype=x.dtype)
+            act = x.new_empty(shape)
             io.act = act.data_ptr()
-        self._run("tb_linear", io, False)
+        self._run("tb_linear", io, self.lib.tb_linear)
         return (y, act) if want_act else y
 
     def linear_backward(self, d_out: Tensor, x: Tensor, weight: Tensor, act: Optional[Tensor] = None, row_valid: Optional[Tensor] = None,
@@ -1063,12 +1055,13 @@ class HipEngine:
             if t is not None and tuple(t.shape) != shape:
                 raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {shape}")
         d_out, act = d_out.contiguous(), None if act is None else act.contiguous()
-        dx = torch.empty(x.shape, device=self.device, dtype=x.dtype) if want_dx else None
-        dw = torch.empty(weight.shape, device=self.device, dtype=x.dtype) if want_dweight else None
-        db = torch.empty(weight.shape[0], device=self.device, dtype=x.dtype) if want_dbias else None
+        dx = x.new_empty(x.shape) if want_dx else None
+        dw = x.new_empty(weight.shape) if want_dweight else None
+        db = x.new_empty(weight.shape[:1]) if want_dbias else None
         io.d_out, io.act = d_out.data_ptr(), None if act is None else act.data_ptr()
         io.dx, io.dweight, io.dbias = (None if t is None else t.data_ptr() for t in (dx, dw, db))
-        self._run("tb_linear_backward", io, True)
+        need = self.lib.tb_linear_workspace_bytes(C.byref(io), 1) if want_dweight or want_dbias else 0
+        self._run("tb_linear_backward", io, self.lib.tb_linear_backward, need)
         return dx, dw, db
 
     def _linear_io(self, what: str, x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: Optional[str], row_valid: Optional[Tensor],
