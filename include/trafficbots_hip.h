@@ -614,7 +614,7 @@ int64_t tb_layer_norm_workspace_bytes(const tb_layer_norm_io* io, int32_t backwa
 
 /* Linear with its epilogue: a = act(x weight^T + bias), 0 in rows that are not valid, y = a + residual; act: 0 none, 1 ReLU.
  * backward: dz = d_out [a > 0 for ReLU] in valid rows, 0 elsewhere; dx = dz weight, dweight = dz^T x, dbias = sum of dz over the rows (the
- * residual's gradient is d_out itself).  Invalid rows of x are not looked at.  n_row may be 0; n_in, n_out >= 1.
+ * residual's gradient is d_out itself).  Invalid rows of x are not looked at.  n_row may be 0; 1 <= n_in, n_out <= 2^22.
  * Replaces: the Linears, masks and residuals of attention.py:81-87,142-146, transformer.py:197-222, mlp.py:62-85. */
 typedef struct tb_linear_io {
     int32_t dtype, n_in, n_out, activation;

@@ -44,6 +44,19 @@ def test_structs_of_the_operators_match_the_header():
                     names.append(re.search(r"([A-Za-z_][A-Za-z0-9_]*)\s*(\[\d+\])?$", part.strip()).group(1))
         assert names == [f[0] for f in cls._fields_], cname
     hip.load()  # (compares the sizes)
+    # the packed form of a call's arguments is the ctypes one: every value a number of its own
+    for cls, packer in ((hip.TbAttentionIO, hip.PACK_ATTENTION), (hip.TbLayerNormIO, hip.PACK_LAYER_NORM), (hip.TbLinearIO, hip.PACK_LINEAR)):
+        assert packer.size == C.sizeof(cls)
+        n, flat, io = 0, [], cls()
+        for name, kind in cls._fields_:
+            many = getattr(kind, "_length_", 0)
+            vals = list(range(n + 1, n + 1 + max(1, many)))
+            n += len(vals)
+            flat += vals
+            setattr(io, name, tuple(vals) if many else vals[0])
+        packed = cls()
+        packer.pack_into(packed, 0, *flat)
+        assert bytes(packed) == bytes(io), cls
 
 
 def test_workspace_sizes_refuse_what_the_operators_refuse():
@@ -53,11 +66,12 @@ def test_workspace_sizes_refuse_what_the_operators_refuse():
 
     def attention(**kw):
         io = hip.TbAttentionIO()
-        for k, v in dict(dict(dtype=0, n_batch=2, n_query=7, n_key=9, n_head=4, n_kv_head=2, head_dim=32), **kw).items():
+        for k, v in dict(dict(dtype=0, n_batch=2, n_query=70, n_key=90, n_head=4, n_kv_head=2, head_dim=32), **kw).items():
             setattr(io, k, v)
         return lib.tb_attention_workspace_bytes(C.byref(io), 0), lib.tb_attention_workspace_bytes(C.byref(io), 1)
 
-    assert attention()[0] == 0 and attention()[1] >= 4 * 2 * 4 * 7
+    assert attention()[0] == 0 and attention()[1] >= 4 * 2 * 4 * 70
+    assert attention(n_query=20, n_key=32) == (0, 0)  # one kernel does it all
     assert attention(n_query=1, n_key=1 << 16)[0] > 0  # one query over a long cache: the walk is split
     assert attention(n_query=0) == (0, 0) and attention(n_batch=0) == (0, 0) and attention(n_key=0)[0] == 0
     for bad in (dict(dtype=2), dict(dtype=-1), dict(n_batch=-1), dict(n_query=-1), dict(n_key=-1), dict(n_head=0), dict(n_kv_head=0), dict(n_kv_head=3),
@@ -81,7 +95,7 @@ def test_workspace_sizes_refuse_what_the_operators_refuse():
         return lib.tb_linear_workspace_bytes(C.byref(io), 0), lib.tb_linear_workspace_bytes(C.byref(io), 1)
 
     assert linear() == (0, 0) and linear(n_row=1 << 20)[1] > 0
-    for bad in (dict(dtype=3), dict(n_row=-1), dict(n_in=0), dict(n_out=0), dict(activation=2), dict(n_in=(1 << 24) + 1)):
+    for bad in (dict(dtype=3), dict(n_row=-1), dict(n_in=0), dict(n_out=0), dict(activation=2), dict(n_in=(1 << 22) + 1)):
         assert linear(**bad) == (-1, -1), bad
     for f in ("tb_attention", "tb_layer_norm", "tb_linear"):
         assert getattr(lib, f + "_workspace_bytes")(None, 0) == -1
@@ -428,6 +442,27 @@ def test_linear_over_many_rows(eng, dtype):
     _near("y", eng.linear(x.cuda(), w.cuda()), ref["y"], ref["y_bound"])
     for name, t in zip(("dx", "dw", "db"), eng.linear_backward(do.cuda(), x.cuda(), w.cuda())):
         _near(name, t, back[name], back[name + "_bound"])
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n,relu,residual,pad", [(16500, 64, 300, False, True, False), (16500, 128, 300, True, True, True), (33000, 192, 600, True, False, True),
+                                                      (32768, 64, 512, False, False, False), (40000, 128, 510, False, True, True)])
+def test_linear_with_direct_loads(eng, m, k, n, relu, residual, pad):
+    """bf16 rows of whole 128-byte lines: tiles of 128 and 256, odd and even numbers of steps, ragged edges."""
+    g = torch.Generator().manual_seed(m + k + n)
+    x, w, b, res = (torch.randn(*s, generator=g).to(BF16) for s in ((m, k), (n, k), (n,), (m, n)))
+    rv = torch.rand(m, generator=g) < 0.7 if pad else None
+    if pad:
+        x[~rv] = float("nan")
+    ref = oo.linear(x, w, b, relu, rv, res if residual else None)
+    kw = dict(activation="relu" if relu else None, row_valid=None if rv is None else rv.cuda(), residual=res.cuda() if residual else None, want_act=True)
+    y, act = eng.linear(x.cuda(), w.cuda(), b.cuda(), **kw)
+    _near("y", y, ref["y"], ref["y_bound"])
+    _near("act", act, ref["act"], ref["act_bound"])
+    # the same operands one element off the 16-byte grid take the other kernel: within the bound too
+    off = torch.empty(m * k + 1, dtype=BF16, device="cuda")[1:].view(m, k)
+    off.copy_(x)
+    _near("y", eng.linear(off, w.cuda(), b.cuda(), **kw)[0], ref["y"], ref["y_bound"])
 
 
 @gpu

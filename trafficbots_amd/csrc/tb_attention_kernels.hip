@@ -202,6 +202,14 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AttnP p) {
     const T* vp = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
     const Valid kvalid(p.key_valid, (int64_t)b * p.Lk);
 
+    int j0 = split * p.split_len, jend = min(p.Lk, j0 + p.split_len);
+    if (p.causal) jend = min(jend, min(p.Lq, qb + QT) + off);
+    Stage<T, DP, NT, KT> sk, sv;
+    if (j0 < jend) {
+        sk.load(p, kp, p.ks[1], kvalid, j0, jend, tid);
+        sv.load(p, vp, p.vs[1], kvalid, j0, jend, tid);
+    }
+
     Frag<NP> qf[NQ][KC];
     int qi[NQ];
 #pragma unroll
@@ -219,14 +227,6 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AttnP p) {
         l[n] = 0.f;
 #pragma unroll
         for (int d = 0; d < DN; ++d) acc[n][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    }
-    int j0 = split * p.split_len, jend = min(p.Lk, j0 + p.split_len);
-    if (p.causal) jend = min(jend, min(p.Lq, qb + QT) + off);
-
-    Stage<T, DP, NT, KT> sk, sv;
-    if (j0 < jend) {
-        sk.load(p, kp, p.ks[1], kvalid, j0, jend, tid);
-        sv.load(p, vp, p.vs[1], kvalid, j0, jend, tid);
     }
     for (; j0 < jend; j0 += KT) {
         __syncthreads();
@@ -318,11 +318,6 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnP p) {
 // loads straight into that layout; only what the second product reads down its rows goes through LDS, a region of the wave's own, so
 // there is no barrier in the walk.  One wave takes one problem; with `wpp` = 4 (a single query over a long cache) the four waves of a
 // workgroup share the walk of one problem and join at its end.
-__device__ __forceinline__ void wave_fence() {  // orders the wave's own LDS accesses across its lanes
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // which of a lane's two rows (one of each 16-row tile) are there and valid
 struct Rows32 {
     uint8_t valid[2];
@@ -708,6 +703,14 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(const AttnP p) {
     const T* vp = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
     const Valid kvalid(p.key_valid, (int64_t)b * p.Lk);
 
+    int j0 = split * p.split_len, jend = min(p.Lk, j0 + p.split_len);
+    if (p.causal) jend = min(jend, min(p.Lq, qb + QT) + off);
+    Stage<T, DP, NT, KT> sk, sv;
+    if (j0 < jend) {
+        sk.load(p, kp, p.ks[1], kvalid, j0, jend, tid);
+        sv.load(p, vp, p.vs[1], kvalid, j0, jend, tid);
+    }
+
     Frag<NP> qf[NQ][KC], gf[NQ][KC];
     int qi[NQ];
     float nlse[NQ], delta[NQ];
@@ -735,13 +738,6 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(const AttnP p) {
         if (in && g == 0 && split == 0) p.delta[row] = delta[n];
 #pragma unroll
         for (int d = 0; d < DN; ++d) acc[n][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    }
-    int j0 = split * p.split_len, jend = min(p.Lk, j0 + p.split_len);
-    if (p.causal) jend = min(jend, min(p.Lq, qb + QT) + off);
-    Stage<T, DP, NT, KT> sk, sv;
-    if (j0 < jend) {
-        sk.load(p, kp, p.ks[1], kvalid, j0, jend, tid);
-        sv.load(p, vp, p.vs[1], kvalid, j0, jend, tid);
     }
     for (; j0 < jend; j0 += KT) {
         __syncthreads();
@@ -832,20 +828,6 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AttnP p) {
     const int kb = kt * CT, k0 = kb + wave * 16 * NQ, off = p.Lk - p.Lq;
     const Valid qvalid(p.query_valid, (int64_t)b * p.Lq);
 
-    Frag<NP> kf[NQ][KC], vf[NQ][KC];
-    int ki[NQ];
-    bool on[NQ];
-    f32x4 dk[NQ][DN], dv[NQ][DN];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        ki[n] = k0 + n * 16 + i16;
-        const int64_t kc = min(ki[n], p.Lk - 1);
-        on[n] = kvalid[kc] && ki[n] < p.Lk;
-        load_columns<T, KC>(p, (const T*)p.k + b * p.ks[0] + kc * p.ks[1] + hk * p.ks[2], on[n], lane, kf[n]);
-        load_columns<T, KC>(p, (const T*)p.v + b * p.vs[0] + kc * p.vs[1] + hk * p.vs[2], on[n], lane, vf[n]);
-#pragma unroll
-        for (int d = 0; d < DN; ++d) dk[n][d] = dv[n][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    }
     // the walk: step t = (head of the group, query tile), query tiles from the first one that sees a key of this tile
     const int n_qt = (p.Lq + KT - 1) / KT, first = p.causal ? min(n_qt, max(0, kb - off) / KT) : 0, per_head = n_qt - first;
     const int n_step = p.G * per_head, len = (n_step + p.n_split - 1) / p.n_split;
@@ -868,6 +850,20 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AttnP p) {
         r_in = q < p.Lq;
     };
     if (t < tend) load(t);
+    Frag<NP> kf[NQ][KC], vf[NQ][KC];
+    int ki[NQ];
+    bool on[NQ];
+    f32x4 dk[NQ][DN], dv[NQ][DN];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        ki[n] = k0 + n * 16 + i16;
+        const int64_t kc = min(ki[n], p.Lk - 1);
+        on[n] = kvalid[kc] && ki[n] < p.Lk;
+        load_columns<T, KC>(p, (const T*)p.k + b * p.ks[0] + kc * p.ks[1] + hk * p.ks[2], on[n], lane, kf[n]);
+        load_columns<T, KC>(p, (const T*)p.v + b * p.vs[0] + kc * p.vs[1] + hk * p.vs[2], on[n], lane, vf[n]);
+#pragma unroll
+        for (int d = 0; d < DN; ++d) dk[n][d] = dv[n][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
     for (; t < tend; ++t) {
         __syncthreads();
         sq.store(p, lq, nullptr, tid);

