@@ -80,11 +80,11 @@ def test_workspace_sizes_refuse_what_the_operators_refuse():
 
     def norm(**kw):
         io = hip.TbLayerNormIO()
-        for k, v in dict(dict(dtype=0, n_row=5, n_col=128), **kw).items():
+        for k, v in dict(dict(dtype=0, n_row=5000, n_col=128), **kw).items():
             setattr(io, k, v)
         return lib.tb_layer_norm_workspace_bytes(C.byref(io), 0), lib.tb_layer_norm_workspace_bytes(C.byref(io), 1)
 
-    assert norm()[0] == 0 and norm()[1] > 0 and norm(n_row=0) == (0, 0)
+    assert norm()[0] == 0 and norm()[1] > 0 and norm(n_row=0) == (0, 0) and norm(n_row=40) == (0, 0)
     for bad in (dict(dtype=2), dict(n_row=-1), dict(n_col=0), dict(n_col=8193), dict(n_row=(1 << 31) + 1)):
         assert norm(**bad) == (-1, -1), bad
 
@@ -253,7 +253,7 @@ def _check_attention(eng, q, k, v, do, kw, ref=None):
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("b,lq,lk,h,hkv,d", [
     (1, 1, 1, 1, 1, 8), (2, 1, 33, 4, 4, 32), (3, 20, 20, 4, 4, 32), (2, 64, 256, 4, 4, 32), (2, 61, 61, 4, 2, 32), (1, 130, 67, 8, 2, 64),
-    (2, 17, 300, 3, 1, 40), (1, 33, 31, 2, 2, 128), (1, 200, 200, 4, 1, 72), (2, 65, 129, 2, 2, 9), (1, 16, 32, 2, 1, 96), (1, 257, 15, 1, 1, 100),
+    (2, 17, 300, 3, 1, 40), (1, 33, 31, 2, 2, 128), (1, 200, 200, 4, 1, 72), (2, 65, 129, 2, 2, 9), (3, 64, 64, 4, 2, 32), (2, 20, 31, 6, 2, 24), (2, 64, 33, 2, 1, 128), (2, 40, 64, 2, 2, 64), (1, 16, 32, 2, 1, 96), (1, 257, 15, 1, 1, 100),
 ])
 def test_attention_sizes(eng, dtype, b, lq, lk, h, hkv, d):
     _check_attention(eng, *_attention_inputs(b, lq, lk, h, hkv, d, dtype, seed=lq + lk))
@@ -362,7 +362,7 @@ def test_attention_offsets_beyond_32_bits(eng):
 
 @gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("rows,c", [(1, 1), (3, 7), (5, 64), (1, 128), (300, 128), (17, 129), (70, 255), (33, 512), (9, 1000), (5, 2047), (6, 4096), (3, 8191), (2, 8192), (5000, 33)])
+@pytest.mark.parametrize("rows,c", [(1, 1), (3, 7), (5, 64), (1, 128), (300, 128), (17, 129), (70, 255), (33, 512), (9, 1000), (5, 2047), (6, 4096), (3, 8191), (2, 8192), (5000, 33), (4096, 17), (4097, 256), (600, 2000)])
 def test_layer_norm(eng, dtype, rows, c):
     g = torch.Generator().manual_seed(rows + c)
     x = (torch.randn(rows, c, generator=g) * 2 + torch.randn(rows, 1, generator=g) * 5).to(dtype)
@@ -429,6 +429,27 @@ def test_linear(eng, dtype, m, k, n, relu, residual, pad):
     ref = oo.linear_backward(do, x, w, None if gate is None else gate.cpu(), rv)
     for name, t in zip(("dx", "dw", "db"), eng.linear_backward(do.cuda(), x.cuda(), w.cuda(), act=gate, row_valid=rvc)):
         _near(name, t, ref[name], ref[name + "_bound"])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m,k,n,relu,pad", [(16384, 128, 128, True, True), (20000, 100, 37, True, False), (16500, 8, 125, False, True), (70001, 40, 8, False, False)])
+def test_linear_backward_of_narrow_layers(eng, dtype, m, k, n, relu, pad):
+    """Both gradient products in one walk over the rows; each alone takes the other kernels."""
+    g = torch.Generator().manual_seed(m + k + n)
+    x, w, do, act = (torch.randn(*s, generator=g).to(dtype) for s in ((m, k), (n, k), (m, n), (m, n)))
+    act, rv = act.clamp_min(0) if relu else None, torch.rand(m, generator=g) < 0.7 if pad else None
+    if pad:
+        x[~rv] = float("nan")
+        do[~rv] = float("inf")
+    ref = oo.linear_backward(do, x, w, act, rv)
+    args = (do.cuda(), x.cuda(), w.cuda())
+    kw = dict(act=_on(act), row_valid=_on(rv))
+    for want in ((True, True, True), (True, True, False), (False, True, True), (True, False, False), (True, False, True)):
+        for name, t, have in zip(("dx", "dw", "db"), eng.linear_backward(*args, **kw, want_dx=want[0], want_dweight=want[1], want_dbias=want[2]), want):
+            assert (t is not None) == have
+            if have:
+                _near(name, t, ref[name], ref[name + "_bound"])
 
 
 @gpu

@@ -8,6 +8,7 @@
 // transposed (rows = the walked axis), so that the accumulator of the first product, lane column i and rows 4 g + 0..3, is already
 // the B operand of the second: two 16-row tiles give a lane 8 contraction slots, and the matching A operand (the walked tensor with its
 // rows as contraction) comes from the same LDS tile through the transposing read.  The probabilities never leave registers.
+// What is added to a score or a dp_ij -- the -inf of an invalid key, -D_i -- is the accumulator its product starts from: no instruction.
 // The dq and the dk / dv pass each recompute the scores (14 instead of 10 D flops per pair): no atomics, the same bits every run.
 #include "tb_ops.hpp"
 
@@ -59,14 +60,22 @@ struct Stage {
         }
         rows = end - row0;
     }
+    // drops what does not belong
+    __device__ __forceinline__ void settle(const AttnP& p, int tid) {
+#pragma unroll
+        for (int c = 0; c < PT; ++c) {
+            const int idx = tid + c * NT, col = (idx % CH) * 8;
+            if (p.ragged) r[c].fit(col - chunk_start(col, p.D));
+            r[c].keep(ok[c] && idx / CH < rows && col < p.D);
+        }
+    }
     // into LDS, and (unless null) `bias` = 0 for the rows that are there, -inf for the others
     __device__ __forceinline__ void store(const AttnP& p, bf16* lds, float* bias, int tid) {
+        settle(p, tid);
 #pragma unroll
         for (int c = 0; c < PT; ++c) {
             const int idx = tid + c * NT, col = (idx % CH) * 8;
             const bool on = ok[c] && idx / CH < rows;
-            if (p.ragged) r[c].fit(col - chunk_start(col, p.D));
-            r[c].keep(on && col < p.D);
             bf16x8 pl[NP];
             r[c].planes(pl);
 #pragma unroll
@@ -140,7 +149,10 @@ template <int KN, int DN>
 __device__ __forceinline__ void soften(f32x4 (&s)[KN], float& m, float& l, f32x4 (&acc)[DN], float scale2) {
     float mx = NEG_INF;
 #pragma unroll
-    for (int t = 0; t < KN; ++t) mx = fmaxf(fmaxf(mx, fmaxf(s[t][0], s[t][1])), fmaxf(s[t][2], s[t][3]));
+    for (int t = 0; t < KN; ++t) {  // (two v_max3)
+        mx = fmaxf(fmaxf(mx, s[t][0]), s[t][1]);
+        mx = fmaxf(fmaxf(mx, s[t][2]), s[t][3]);
+    }
     mx = fmaxf(m, max_over_groups(mx));
     if (__any(mx > m)) {
         const float alpha = __builtin_amdgcn_exp2f((m - (mx == NEG_INF ? 0.f : mx)) * scale2);
@@ -240,8 +252,9 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AttnP p) {
         f32x4 s[NQ][KN];
 #pragma unroll
         for (int t = 0; t < KN; ++t) {
+            const f32x4 bias = *reinterpret_cast<const f32x4*>(lb + t * 16 + 4 * g);
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) s[n][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            for (int n = 0; n < NQ; ++n) s[n][t] = bias;
 #pragma unroll
             for (int kc = 0; kc < KC; ++kc) {
                 Frag<NP> a;
@@ -250,13 +263,12 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AttnP p) {
                 for (int n = 0; n < NQ; ++n) s[n][t] = mma<NP>(a, qf[n][kc], s[n][t]);
             }
         }
-        const bool biased = p.key_valid || j0 + KT > jend, diagonal = p.causal && j0 + KT - 1 > q0 + off;
+        const bool diagonal = p.causal && j0 + KT - 1 > q0 + off;
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
+            if (diagonal) {
 #pragma unroll
-            for (int t = 0; t < KN; ++t) {
-                if (biased) s[n][t] += *reinterpret_cast<const f32x4*>(lb + t * 16 + 4 * g);
-                if (diagonal) hide_later(s[n][t], j0 + t * 16 + 4 * g, qi[n] + off);
+                for (int t = 0; t < KN; ++t) hide_later(s[n][t], j0 + t * 16 + 4 * g, qi[n] + off);
             }
             if (p.mask) {
                 const uint8_t* mask = p.mask + b * p.mask_s[0] + (int64_t)min(qi[n], p.Lq - 1) * p.mask_s[1];
@@ -316,8 +328,8 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnP p) {
 // ------------------------------------------------------------------------------------------------ few columns: private walks
 // With at most 32 columns a workgroup has nothing to share: each wave walks 32 rows at a time on its own.  The rows it needs as A operand it
 // loads straight into that layout; only what the second product reads down its rows goes through LDS, a region of the wave's own, so
-// there is no barrier in the walk.  One wave takes one problem; with `wpp` = 4 (a single query over a long cache) the four waves of a
-// workgroup share the walk of one problem and join at its end.
+// there is no barrier in the walk.  One wave takes one problem; with `wpp` = NW (a single query over a long cache) the waves of a workgroup
+// share the walk of one problem and join at its end.
 // which of a lane's two rows (one of each 16-row tile) are there and valid
 struct Rows32 {
     uint8_t valid[2];
@@ -374,16 +386,16 @@ __device__ __forceinline__ void row_bias(const Rows32& ok, int lane, f32x4 (&bia
     }
 }
 
-template <typename T, int DP, int NQ>
-__global__ __launch_bounds__(256) void k_attn_fwd_few(const AttnP p) {
+template <typename T, int DP, int NQ, int NW>
+__global__ __launch_bounds__(64 * NW) void k_attn_fwd_few(const AttnP p) {
     constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, LD = DP + LDS_PAD;
-    constexpr int JOIN = 2 * 16 * NQ * DP * 2;  // (in bf16 elements) two waves' accumulators
-    constexpr int REGION = 4 * NP * 32 * LD > JOIN ? 4 * NP * 32 * LD : JOIN;
+    constexpr int JOIN = NW / 2 * 16 * NQ * DP * 2;  // (in bf16 elements) half the waves' accumulators
+    constexpr int REGION = NW * NP * 32 * LD > JOIN ? NW * NP * 32 * LD : JOIN;
     __shared__ __attribute__((aligned(16))) bf16 region[REGION];
-    __shared__ float ml[2][4][16 * NQ];
+    __shared__ float ml[2][NW][16 * NQ];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, g = lane >> 4;
     const int part = p.wpp > 1 ? wave : 0;
-    const int64_t id = p.wpp > 1 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+    const int64_t id = p.wpp > 1 ? blockIdx.x : (int64_t)blockIdx.x * NW + wave;
     const int n_bh = p.B * p.H, split = (int)(id / n_bh), bh = (int)(id % n_bh);
     if (split >= p.n_split) return;  // (wpp > 1: the grid has no such workgroup)
     const int b = bh / p.H, h = bh % p.H, hk = h / p.G, off = p.Lk - p.Lq;
@@ -438,10 +450,9 @@ __global__ __launch_bounds__(256) void k_attn_fwd_few(const AttnP p) {
             f32x4 s[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                s[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+                s[t] = bias[t];
 #pragma unroll
                 for (int kc = 0; kc < KC; ++kc) s[t] = mma<NP>(kf[t][kc], qf[n][kc], s[t]);
-                s[t] += bias[t];
                 if (p.causal) hide_later(s[t], j0 + t * 16 + 4 * g, n * 16 + i16 + off);
             }
             if (p.mask) {
@@ -462,7 +473,7 @@ __global__ __launch_bounds__(256) void k_attn_fwd_few(const AttnP p) {
     }
 #pragma unroll
     for (int n = 0; n < NQ; ++n) l[n] = sum_over_groups(l[n]);
-    if (p.wpp > 1) {  // (workgroup-uniform) a common maximum, then the four waves' sums: 2, 3 into 0, 1, then 1 into 0
+    if (p.wpp > 1) {  // (workgroup-uniform) a common maximum, then the waves' sums, the upper half into the lower until one is left
         float* red = reinterpret_cast<float*>(region);
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
@@ -475,10 +486,10 @@ __global__ __launch_bounds__(256) void k_attn_fwd_few(const AttnP p) {
         for (int n = 0; n < NQ; ++n) {
             float mx = NEG_INF, sum = 0.f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) mx = fmaxf(mx, ml[0][w][n * 16 + i16]);
+            for (int w = 0; w < NW; ++w) mx = fmaxf(mx, ml[0][w][n * 16 + i16]);
             const float ref = mx == NEG_INF ? 0.f : mx;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) sum = __builtin_fmaf(ml[1][w][n * 16 + i16], __builtin_amdgcn_exp2f((ml[0][w][n * 16 + i16] - ref) * p.scale2), sum);
+            for (int w = 0; w < NW; ++w) sum = __builtin_fmaf(ml[1][w][n * 16 + i16], __builtin_amdgcn_exp2f((ml[0][w][n * 16 + i16] - ref) * p.scale2), sum);
             const float alpha = __builtin_amdgcn_exp2f((m[n] - ref) * p.scale2);
             m[n] = mx;
             l[n] = sum;
@@ -486,7 +497,7 @@ __global__ __launch_bounds__(256) void k_attn_fwd_few(const AttnP p) {
             for (int d = 0; d < DN; ++d) acc[n][d] *= alpha;
         }
 #pragma unroll
-        for (int half = 2; half >= 1; half >>= 1) {
+        for (int half = NW / 2; half >= 1; half >>= 1) {
             if (wave >= half && wave < 2 * half) {
 #pragma unroll
                 for (int n = 0; n < NQ; ++n)
@@ -511,7 +522,8 @@ __global__ __launch_bounds__(256) void k_attn_fwd_few(const AttnP p) {
     }
 }
 
-// Backward of a whole problem with at most 32 queries and 32 keys: one wave per key / value head, everything loaded once.  Queries as columns
+// Backward of a whole problem with at most 32 queries and 32 keys: one wave per head (none of them
+// shared), everything loaded once.  Queries as columns
 // give dq; the scores once more with keys as columns give dk and dv.  The same registers serve as A and as B operand (both layouts
 // hold 8 components of one row).  K, dO and Q pass one after the other through the wave's LDS region to be read down their rows.
 template <typename T, int DP>
@@ -541,14 +553,11 @@ __global__ __launch_bounds__(256, 2) void k_attn_bwd_small(const AttnP p) {
         as_frags<T, KC>(a, kf);
         as_frags<T, KC>(v, vf);
     }
-    f32x4 bias[2], dk[2][DN], dv[2][DN];
+    f32x4 bias[2];
     row_bias(kok, lane, bias);
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int d = 0; d < DN; ++d) dk[n][d] = dv[n][d] = zero;
-    for (int h = hk * p.G; h < (hk + 1) * p.G; ++h) {
-        Frag<NP> qf[2][KC], gf[2][KC];
+    const int h = hk;
+    Frag<NP> qf[2][KC], gf[2][KC];
+    {
         float nlse[2], delta[2];
         {
             Held<T> q[2][KC], go[2][KC], o[2][KC];
@@ -581,7 +590,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_bwd_small(const AttnP p) {
         for (int n = 0; n < 2; ++n)
             if (g == 0) {
                 nlse_r[n * 16 + i16] = nlse[n];
-                delta_r[n * 16 + i16] = delta[n];
+                delta_r[n * 16 + i16] = -delta[n];
             }
         wave_fence();
         {  // queries as columns: dq
@@ -591,7 +600,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_bwd_small(const AttnP p) {
                 f32x4 ds[2];
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    f32x4 s = zero, dp = zero;
+                    f32x4 s = bias[t], dp = {-delta[n], -delta[n], -delta[n], -delta[n]};
 #pragma unroll
                     for (int kc = 0; kc < KC; ++kc) {
                         s = mma<NP>(kf[t][kc], qf[n][kc], s);
@@ -600,11 +609,11 @@ __global__ __launch_bounds__(256, 2) void k_attn_bwd_small(const AttnP p) {
                     const int q = n * 16 + i16, j = t * 16 + 4 * g;
                     f32x4 x;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(s[e], p.scale2, nlse[n]) + bias[t][e];
+                    for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(s[e], p.scale2, nlse[n]);
                     if (p.causal) hide_later(x, j, q + off);
                     if (p.mask) hide_masked(x, p.mask + b * p.mask_s[0] + (int64_t)min(q, p.Lq - 1) * p.mask_s[1], j, p.Lk);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) ds[t][e] = __builtin_amdgcn_exp2f(x[e]) * (dp[e] - delta[n]);
+                    for (int e = 0; e < 4; ++e) ds[t][e] = __builtin_amdgcn_exp2f(x[e]) * dp[e];
                 }
                 as_operand<NP>(ds[0], ds[1], df[n]);
             }
@@ -620,74 +629,182 @@ __global__ __launch_bounds__(256, 2) void k_attn_bwd_small(const AttnP p) {
                 }
             }
         }
-        // keys as columns: dk, dv
-        Frag<NP> pf[2], df[2];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            f32x4 pr[2], ds[2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                f32x4 s = zero, dp = zero;
-#pragma unroll
-                for (int kc = 0; kc < KC; ++kc) {
-                    s = mma<NP>(qf[t][kc], kf[n][kc], s);
-                    dp = mma<NP>(gf[t][kc], vf[n][kc], dp);
-                }
-                const int key = n * 16 + i16, i = t * 16 + 4 * g;
-                const f32x4 nl = *reinterpret_cast<const f32x4*>(nlse_r + i), de = *reinterpret_cast<const f32x4*>(delta_r + i);
-                f32x4 x;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(s[e], p.scale2, nl[e]);
-                if (p.causal) hide_earlier(x, i, key - off);
-                if (p.mask) hide_masked_rows(x, p.mask + b * p.mask_s[0] + min(key, p.Lk - 1), p.mask_s[1], i, p.Lq);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    pr[t][e] = __builtin_amdgcn_exp2f(x[e]);
-                    ds[t][e] = pr[t][e] * (dp[e] - de[e]);
-                }
-            }
-            as_operand<NP>(pr[0], pr[1], pf[n]);
-            as_operand<NP>(ds[0], ds[1], df[n]);
-        }
-        wave_fence();
-        rows32_to_lds<NP, KC, LD>(gf, lds, lane);
-        wave_fence();
-#pragma unroll
-        for (int d = 0; d < DN; ++d) {
-            Frag<NP> a;
-            frag_cols<NP, LD>(lds, (size_t)32 * LD, 4 * g, 16 + 4 * g, d * 16, lane, a);
-#pragma unroll
-            for (int n = 0; n < 2; ++n) dv[n][d] = mma<NP>(a, pf[n], dv[n][d]);
-        }
-        wave_fence();
-        rows32_to_lds<NP, KC, LD>(qf, lds, lane);
-        wave_fence();
-#pragma unroll
-        for (int d = 0; d < DN; ++d) {
-            Frag<NP> a;
-            frag_cols<NP, LD>(lds, (size_t)32 * LD, 4 * g, 16 + 4 * g, d * 16, lane, a);
-#pragma unroll
-            for (int n = 0; n < 2; ++n) dk[n][d] = mma<NP>(a, df[n], dk[n][d]);
-        }
     }
+    // keys as columns: dk, dv
+    Frag<NP> pf[2], df[2];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-        const int key = n * 16 + i16;
-        if (key >= p.Lk) continue;
-        const bool on = kok.on(n, lane);
+        f32x4 pr[2], ds[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int key = n * 16 + i16, i = t * 16 + 4 * g;
+            const f32x4 nl = *reinterpret_cast<const f32x4*>(nlse_r + i);
+            f32x4 s = zero, dp = *reinterpret_cast<const f32x4*>(delta_r + i);
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) {
+                s = mma<NP>(qf[t][kc], kf[n][kc], s);
+                dp = mma<NP>(gf[t][kc], vf[n][kc], dp);
+            }
+            f32x4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(s[e], p.scale2, nl[e]);
+            if (p.causal) hide_earlier(x, i, key - off);
+            if (p.mask) hide_masked_rows(x, p.mask + b * p.mask_s[0] + min(key, p.Lk - 1), p.mask_s[1], i, p.Lq);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                pr[t][e] = __builtin_amdgcn_exp2f(x[e]);
+                ds[t][e] = pr[t][e] * dp[e];
+            }
+        }
+        as_operand<NP>(pr[0], pr[1], pf[n]);
+        as_operand<NP>(ds[0], ds[1], df[n]);
+    }
+    // (from LDS down the rows of dO, then of Q: a gradient's 16 components at a time, straight to memory)
+    auto give = [&](const Frag<NP> (&rows)[2][KC], const Frag<NP> (&cols)[2], T* dst, const int64_t* st, float scale) {
+        wave_fence();
+        rows32_to_lds<NP, KC, LD>(rows, lds, lane);
+        wave_fence();
 #pragma unroll
         for (int d = 0; d < DN; ++d) {
-            const int col = d * 16 + 4 * g;
-            if (col >= p.D) continue;
-            store4((T*)p.dk + b * p.dks[0] + key * p.dks[1] + hk * p.dks[2] + col, p.D - col, on ? dk[n][d] * p.scale : zero);
-            store4((T*)p.dv + b * p.dvs[0] + key * p.dvs[1] + hk * p.dvs[2] + col, p.D - col, on ? dv[n][d] : zero);
+            Frag<NP> a;
+            frag_cols<NP, LD>(lds, (size_t)32 * LD, 4 * g, 16 + 4 * g, d * 16, lane, a);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int key = n * 16 + i16, col = d * 16 + 4 * g;
+                const f32x4 o = mma<NP>(a, cols[n], zero) * scale;
+                if (key < p.Lk && col < p.D) store4(dst + b * st[0] + key * st[1] + hk * st[2] + col, p.D - col, kok.on(n, lane) ? o : zero);
+            }
+        }
+    };
+    give(gf, pf, (T*)p.dv, p.dvs, 1.f);
+    give(qf, df, (T*)p.dk, p.dks, p.scale);
+}
+
+// ------------------------------------------------------------------------------------------------ backward: one tile
+// KT keys in LDS (bias `lb`: 0 or -inf), queries as columns: acc += K^T ds
+template <int NP, int DP, int NQ, int KT>
+__device__ __forceinline__ void dq_tile(const AttnP& p, const bf16* lk, const bf16* lv, const float* lb, int lane, int b, int j0, int jend, bool diagonal, int off,
+                                        const int (&qi)[NQ], const Frag<NP> (&qf)[NQ][DP / 32], const Frag<NP> (&gf)[NQ][DP / 32], const float (&nlse)[NQ],
+                                        const float (&delta)[NQ], f32x4 (&acc)[NQ][DP / 16]) {
+    constexpr int KC = DP / 32, DN = DP / 16, KN = KT / 16, LD = DP + LDS_PAD;
+    const int g = lane >> 4;
+#pragma unroll
+    for (int t2 = 0; t2 < KN; t2 += 2) {
+        f32x4 ds[NQ][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int t = t2 + u;
+            f32x4 s[NQ], dp[NQ];
+            const f32x4 bias = *reinterpret_cast<const f32x4*>(lb + t * 16 + 4 * g);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                s[n] = bias;
+                dp[n] = (f32x4){-delta[n], -delta[n], -delta[n], -delta[n]};
+            }
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) {
+                Frag<NP> a, v;
+                frag_rows<NP, LD>(lk, (size_t)KT * LD, t * 16, kc * 32, lane, a);
+                frag_rows<NP, LD>(lv, (size_t)KT * LD, t * 16, kc * 32, lane, v);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    s[n] = mma<NP>(a, qf[n][kc], s[n]);
+                    dp[n] = mma<NP>(v, gf[n][kc], dp[n]);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                f32x4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(s[n][e], p.scale2, nlse[n]);
+                if (diagonal) hide_later(x, j0 + t * 16 + 4 * g, qi[n] + off);
+                if (p.mask) hide_masked(x, p.mask + b * p.mask_s[0] + (int64_t)min(qi[n], p.Lq - 1) * p.mask_s[1], j0 + t * 16 + 4 * g, jend);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ds[n][u][e] = __builtin_amdgcn_exp2f(x[e]) * dp[n][e];
+            }
+        }
+        Frag<NP> df[NQ];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) as_operand<NP>(ds[n][0], ds[n][1], df[n]);
+#pragma unroll
+        for (int d = 0; d < DN; ++d) {
+            Frag<NP> a;
+            frag_cols<NP, LD>(lk, (size_t)KT * LD, t2 * 16 + 4 * g, (t2 + 1) * 16 + 4 * g, d * 16, lane, a);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) acc[n][d] = mma<NP>(a, df[n], acc[n][d]);
+        }
+    }
+}
+// KT queries in LDS (-lse in powers of two, -inf where a query takes no part, and -D), keys as columns: dv += dO^T p, dk += Q^T ds
+template <int NP, int DP, int NQ, int KT>
+__device__ __forceinline__ void dkv_tile(const AttnP& p, const bf16* lq, const bf16* lg, const float* ll, const float* ld, int lane, int b, int q0, bool diagonal, int off,
+                                         const int (&ki)[NQ], const Frag<NP> (&kf)[NQ][DP / 32], const Frag<NP> (&vf)[NQ][DP / 32], f32x4 (&dk)[NQ][DP / 16],
+                                         f32x4 (&dv)[NQ][DP / 16]) {
+    constexpr int KC = DP / 32, DN = DP / 16, KN = KT / 16, LD = DP + LDS_PAD;
+    const int g = lane >> 4;
+#pragma unroll
+    for (int t2 = 0; t2 < KN; t2 += 2) {
+        f32x4 pr[NQ][2], ds[NQ][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int tt = t2 + u;
+            f32x4 s[NQ], dp[NQ];
+            const f32x4 nl = *reinterpret_cast<const f32x4*>(ll + tt * 16 + 4 * g), de = *reinterpret_cast<const f32x4*>(ld + tt * 16 + 4 * g);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                s[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+                dp[n] = de;
+            }
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) {
+                Frag<NP> a, v;
+                frag_rows<NP, LD>(lq, (size_t)KT * LD, tt * 16, kc * 32, lane, a);
+                frag_rows<NP, LD>(lg, (size_t)KT * LD, tt * 16, kc * 32, lane, v);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    s[n] = mma<NP>(a, kf[n][kc], s[n]);
+                    dp[n] = mma<NP>(v, vf[n][kc], dp[n]);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                f32x4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(s[n][e], p.scale2, nl[e]);
+                if (diagonal) hide_earlier(x, q0 + tt * 16 + 4 * g, ki[n] - off);
+                if (p.mask) hide_masked_rows(x, p.mask + b * p.mask_s[0] + min(ki[n], p.Lk - 1), p.mask_s[1], q0 + tt * 16 + 4 * g, p.Lq);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    pr[n][u][e] = __builtin_amdgcn_exp2f(x[e]);
+                    ds[n][u][e] = pr[n][u][e] * dp[n][e];
+                }
+            }
+        }
+        Frag<NP> pf[NQ], df[NQ];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            as_operand<NP>(pr[n][0], pr[n][1], pf[n]);
+            as_operand<NP>(ds[n][0], ds[n][1], df[n]);
+        }
+#pragma unroll
+        for (int d = 0; d < DN; ++d) {
+            Frag<NP> a, v;
+            frag_cols<NP, LD>(lg, (size_t)KT * LD, t2 * 16 + 4 * g, (t2 + 1) * 16 + 4 * g, d * 16, lane, a);
+            frag_cols<NP, LD>(lq, (size_t)KT * LD, t2 * 16 + 4 * g, (t2 + 1) * 16 + 4 * g, d * 16, lane, v);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                dv[n][d] = mma<NP>(a, pf[n], dv[n][d]);
+                dk[n][d] = mma<NP>(v, df[n], dk[n][d]);
+            }
         }
     }
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dq
+// (bf16, D = 128: two column tiles fit 256 registers with tiles of 32 keys, and two waves per SIMD then hide each other's LDS reads: 495 us
+// instead of 700 with one wave per SIMD and 64 keys, 8192 x 8192 causal, 16 heads)
 template <typename T, int DP, int NW, int NQ, int KT>
-__global__ __launch_bounds__(64 * NW) void k_attn_dq(const AttnP p) {
+__global__ __launch_bounds__(64 * NW, DP == 128 && NQ == 2 && NW == 4 ? 2 : 1) void k_attn_dq(const AttnP p) {
     constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, KN = KT / 16, NT = 64 * NW, LD = DP + LDS_PAD, QT = 16 * NQ * NW;
     __shared__ __attribute__((aligned(16))) bf16 lk[NP * KT * LD];
     __shared__ __attribute__((aligned(16))) bf16 lv[NP * KT * LD];
@@ -748,50 +865,8 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dq(const AttnP p) {
             sk.load(p, kp, p.ks[1], kvalid, j0 + KT, jend, tid);
             sv.load(p, vp, p.vs[1], kvalid, j0 + KT, jend, tid);
         }
-        const bool biased = p.key_valid || j0 + KT > jend, diagonal = p.causal && j0 + KT - 1 > q0 + off;
-#pragma unroll
-        for (int t2 = 0; t2 < KN; t2 += 2) {
-            f32x4 ds[NQ][2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int t = t2 + u;
-                f32x4 s[NQ], dp[NQ];
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) s[n] = dp[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int kc = 0; kc < KC; ++kc) {
-                    Frag<NP> a, v;
-                    frag_rows<NP, LD>(lk, (size_t)KT * LD, t * 16, kc * 32, lane, a);
-                    frag_rows<NP, LD>(lv, (size_t)KT * LD, t * 16, kc * 32, lane, v);
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n) {
-                        s[n] = mma<NP>(a, qf[n][kc], s[n]);
-                        dp[n] = mma<NP>(v, gf[n][kc], dp[n]);
-                    }
-                }
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) {
-                    f32x4 x;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(s[n][e], p.scale2, nlse[n]);
-                    if (biased) x += *reinterpret_cast<const f32x4*>(lb + t * 16 + 4 * g);
-                    if (diagonal) hide_later(x, j0 + t * 16 + 4 * g, qi[n] + off);
-                    if (p.mask) hide_masked(x, p.mask + b * p.mask_s[0] + (int64_t)min(qi[n], p.Lq - 1) * p.mask_s[1], j0 + t * 16 + 4 * g, jend);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) ds[n][u][e] = __builtin_amdgcn_exp2f(x[e]) * (dp[n][e] - delta[n]);
-                }
-            }
-            Frag<NP> df[NQ];
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) as_operand<NP>(ds[n][0], ds[n][1], df[n]);
-#pragma unroll
-            for (int d = 0; d < DN; ++d) {
-                Frag<NP> a;
-                frag_cols<NP, LD>(lk, (size_t)KT * LD, t2 * 16 + 4 * g, (t2 + 1) * 16 + 4 * g, d * 16, lane, a);
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) acc[n][d] = mma<NP>(a, df[n], acc[n][d]);
-            }
-        }
+        const bool diagonal = p.causal && j0 + KT - 1 > q0 + off;
+        dq_tile<NP, DP, NQ, KT>(p, lk, lv, lb, lane, b, j0, jend, diagonal, off, qi, qf, gf, nlse, delta, acc);
     }
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -871,65 +946,13 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AttnP p) {
         if (tid < KT) {
             const bool r_on = r_valid && r_in;
             ll[tid] = !r_on || r_lse == NEG_INF ? NEG_INF : -r_lse * LOG2E;
-            ld[tid] = r_on ? r_delta : 0.f;
+            ld[tid] = r_on ? -r_delta : 0.f;
         }
         __syncthreads();
         const int q0 = (first + t % per_head) * KT;
         if (t + 1 < tend) load(t + 1);
         const bool diagonal = p.causal && k0 + 16 * NQ - 1 > q0 + off;
-#pragma unroll
-        for (int t2 = 0; t2 < KN; t2 += 2) {
-            f32x4 pr[NQ][2], ds[NQ][2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int tt = t2 + u;
-                f32x4 s[NQ], dp[NQ];
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) s[n] = dp[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int kc = 0; kc < KC; ++kc) {
-                    Frag<NP> a, v;
-                    frag_rows<NP, LD>(lq, (size_t)KT * LD, tt * 16, kc * 32, lane, a);
-                    frag_rows<NP, LD>(lg, (size_t)KT * LD, tt * 16, kc * 32, lane, v);
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n) {
-                        s[n] = mma<NP>(a, kf[n][kc], s[n]);
-                        dp[n] = mma<NP>(v, vf[n][kc], dp[n]);
-                    }
-                }
-                const f32x4 nl = *reinterpret_cast<const f32x4*>(ll + tt * 16 + 4 * g), de = *reinterpret_cast<const f32x4*>(ld + tt * 16 + 4 * g);
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) {
-                    f32x4 x;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(s[n][e], p.scale2, nl[e]);
-                    if (diagonal) hide_earlier(x, q0 + tt * 16 + 4 * g, ki[n] - off);
-                    if (p.mask) hide_masked_rows(x, p.mask + b * p.mask_s[0] + min(ki[n], p.Lk - 1), p.mask_s[1], q0 + tt * 16 + 4 * g, p.Lq);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        pr[n][u][e] = __builtin_amdgcn_exp2f(x[e]);
-                        ds[n][u][e] = pr[n][u][e] * (dp[n][e] - de[e]);
-                    }
-                }
-            }
-            Frag<NP> pf[NQ], df[NQ];
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                as_operand<NP>(pr[n][0], pr[n][1], pf[n]);
-                as_operand<NP>(ds[n][0], ds[n][1], df[n]);
-            }
-#pragma unroll
-            for (int d = 0; d < DN; ++d) {
-                Frag<NP> a, v;
-                frag_cols<NP, LD>(lg, (size_t)KT * LD, t2 * 16 + 4 * g, (t2 + 1) * 16 + 4 * g, d * 16, lane, a);
-                frag_cols<NP, LD>(lq, (size_t)KT * LD, t2 * 16 + 4 * g, (t2 + 1) * 16 + 4 * g, d * 16, lane, v);
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) {
-                    dv[n][d] = mma<NP>(a, pf[n], dv[n][d]);
-                    dk[n][d] = mma<NP>(v, df[n], dk[n][d]);
-                }
-            }
-        }
+        dkv_tile<NP, DP, NQ, KT>(p, lq, lg, ll, ld, lane, b, q0, diagonal, off, ki, kf, vf, dk, dv);
     }
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -947,6 +970,95 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AttnP p) {
                 store4((T*)p.dk + b * p.dks[0] + ki[n] * p.dks[1] + hk * p.dks[2] + col, p.D - col, ok);
                 store4((T*)p.dv + b * p.dvs[0] + ki[n] * p.dvs[1] + hk * p.dvs[2] + col, p.D - col, ov);
             }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ backward of at most 64 x 64
+// One workgroup per key / value head, one launch, no scratch: K, V, Q and dO are staged once, each wave takes 16 queries for dq, then 16 keys
+// for dk and dv.  The operands of a wave's columns are rows of the same LDS tiles.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void k_attn_bwd_mid(const AttnP p) {
+    constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, LD = DP + LDS_PAD, L = 64;
+    __shared__ __attribute__((aligned(16))) bf16 lk[NP * L * LD];
+    __shared__ __attribute__((aligned(16))) bf16 lv[NP * L * LD];
+    __shared__ __attribute__((aligned(16))) bf16 lq[NP * L * LD];
+    __shared__ __attribute__((aligned(16))) bf16 lg[NP * L * LD];
+    __shared__ __attribute__((aligned(16))) float lb[L];
+    __shared__ __attribute__((aligned(16))) float ll[L];
+    __shared__ __attribute__((aligned(16))) float ld[L];
+    const int b = (int)(blockIdx.x / (unsigned)p.Hkv), hk = (int)(blockIdx.x % (unsigned)p.Hkv), off = p.Lk - p.Lq;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, g = lane >> 4;
+    const Valid kvalid(p.key_valid, (int64_t)b * p.Lk), qvalid(p.query_valid, (int64_t)b * p.Lq);
+    const int col[1] = {wave * 16 + i16};  // this lane's query, then its key
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    f32x4 dk[1][DN], dv[1][DN];
+#pragma unroll
+    for (int d = 0; d < DN; ++d) dk[0][d] = dv[0][d] = zero;
+    Stage<T, DP, 256, L> sk, sv, sq, sg;
+    sk.load(p, (const T*)p.k + b * p.ks[0] + hk * p.ks[2], p.ks[1], kvalid, 0, p.Lk, tid);
+    sv.load(p, (const T*)p.v + b * p.vs[0] + hk * p.vs[2], p.vs[1], kvalid, 0, p.Lk, tid);
+    for (int h = hk * p.G; h < (hk + 1) * p.G; ++h) {
+        sq.load(p, (const T*)p.q + b * p.qs[0] + h * p.qs[2], p.qs[1], qvalid, 0, p.Lq, tid);
+        sg.load(p, (const T*)p.d_out + b * p.dos[0] + h * p.dos[2], p.dos[1], qvalid, 0, p.Lq, tid);
+        Stage<T, DP, 256, L> so;
+        so.load(p, (const T*)p.out + b * p.os[0] + h * p.os[2], p.os[1], qvalid, 0, p.Lq, tid);
+        const float r_lse = p.lse[((int64_t)b * p.H + h) * p.Lq + min(tid % L, p.Lq - 1)];
+        const bool r_on = qvalid[min(tid % L, p.Lq - 1)] && tid % L < p.Lq;
+        __syncthreads();  // (the head before is done with the tiles)
+        if (h == hk * p.G) {
+            sk.store(p, lk, lb, tid);
+            sv.store(p, lv, nullptr, tid);
+        }
+        sq.store(p, lq, nullptr, tid);
+        sg.store(p, lg, nullptr, tid);
+        so.settle(p, tid);
+#pragma unroll
+        for (int c = 0; c < so.PT; ++c) {  // -D: a row's chunks are in adjacent lanes
+            float dot = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dot = __builtin_fmaf(sg.r[c].get(e), so.r[c].get(e), dot);
+#pragma unroll
+            for (int x = 1; x < so.CH; x <<= 1) dot += __shfl_xor(dot, x);
+            const int idx = tid + c * 256;
+            if (idx % so.CH == 0) ld[idx / so.CH] = -dot;
+        }
+        if (tid < L) ll[tid] = !r_on || r_lse == NEG_INF ? NEG_INF : -r_lse * LOG2E;
+        __syncthreads();
+        {
+            Frag<NP> qf[1][KC], gf[1][KC];
+            f32x4 acc[1][DN];
+            const float nlse[1] = {ll[col[0]]}, delta[1] = {-ld[col[0]]};
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) {
+                frag_rows<NP, LD>(lq, (size_t)L * LD, wave * 16, kc * 32, lane, qf[0][kc]);
+                frag_rows<NP, LD>(lg, (size_t)L * LD, wave * 16, kc * 32, lane, gf[0][kc]);
+            }
+#pragma unroll
+            for (int d = 0; d < DN; ++d) acc[0][d] = zero;
+            dq_tile<NP, DP, 1, L>(p, lk, lv, lb, lane, b, 0, p.Lk, p.causal, off, col, qf, gf, nlse, delta, acc);
+            if (col[0] < p.Lq) {
+#pragma unroll
+                for (int d = 0; d < DN; ++d)
+                    if (d * 16 + 4 * g < p.D) store4((T*)p.dq + b * p.dqs[0] + col[0] * p.dqs[1] + h * p.dqs[2] + d * 16 + 4 * g, p.D - d * 16 - 4 * g, acc[0][d] * p.scale);
+            }
+        }
+        Frag<NP> kf[1][KC], vf[1][KC];
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) {
+            frag_rows<NP, LD>(lk, (size_t)L * LD, wave * 16, kc * 32, lane, kf[0][kc]);
+            frag_rows<NP, LD>(lv, (size_t)L * LD, wave * 16, kc * 32, lane, vf[0][kc]);
+        }
+        dkv_tile<NP, DP, 1, L>(p, lq, lg, ll, ld, lane, b, 0, p.causal, off, col, kf, vf, dk, dv);
+    }
+    if (col[0] < p.Lk) {
+        const bool on = lb[col[0]] == 0.f;
+#pragma unroll
+        for (int d = 0; d < DN; ++d) {
+            const int c = d * 16 + 4 * g;
+            if (c >= p.D) continue;
+            store4((T*)p.dk + b * p.dks[0] + col[0] * p.dks[1] + hk * p.dks[2] + c, p.D - c, on ? dk[0][d] * p.scale : zero);
+            store4((T*)p.dv + b * p.dvs[0] + col[0] * p.dvs[1] + hk * p.dvs[2] + c, p.D - c, on ? dv[0][d] : zero);
         }
     }
 }
@@ -975,20 +1087,29 @@ struct Shape {  // of one launch: columns per workgroup, walked rows per step of
     int col_tile, walk_tile;
     void (*kernel)(AttnP);
     int threads;
-    bool few;  // wave-private walks (k_attn_fwd_few)
+    bool few;     // wave-private walks (k_attn_fwd_few)
+    int wpp = 1;  // waves that share a problem
 };
 
 template <typename T, int DP, int NQ, int KT>
 Shape tiles(Pass pass) {  // four waves
-    return {64 * NQ, KT, pass == FWD ? k_attn_fwd<T, DP, 4, NQ, KT> : pass == DQ ? k_attn_dq<T, DP, 4, NQ, KT> : k_attn_dkv<T, DP, 4, NQ, KT>, 256, false};
+    constexpr int KQ = DP == 128 && NQ == 2 ? 32 : KT;
+    if (pass == DQ) return {64 * NQ, KQ, k_attn_dq<T, DP, 4, NQ, KQ>, 256, false};
+    return {64 * NQ, KT, pass == FWD ? k_attn_fwd<T, DP, 4, NQ, KT> : k_attn_dkv<T, DP, 4, NQ, KT>, 256, false};
 }
 
 template <typename T, int DP>
-Shape choose(Pass pass, int n_col, int64_t n_bh) {
+Shape choose(Pass pass, int n_col, int walk, int64_t n_bh) {
     constexpr bool wide = sizeof(T) == 2 || DP == 32;  // two column tiles per wave fit the registers
     constexpr int KT = sizeof(T) == 2 || DP == 32 ? 64 : 32;
     if (n_col <= 32) {
-        if (pass == FWD) return {32, 32, n_col <= 16 ? k_attn_fwd_few<T, DP, 1> : k_attn_fwd_few<T, DP, 2>, 256, true};
+        if (pass == FWD) {
+            // one problem per workgroup below 2048 problems (with a walk to share), one per wave above; eight waves where their tiles fit LDS
+            const bool shared = walk > 64 && n_bh < 2048;
+            if constexpr (DP <= 64)
+                if (shared && n_col <= 16) return {32, 32, k_attn_fwd_few<T, DP, 1, 8>, 512, true, 8};
+            return {32, 32, n_col <= 16 ? k_attn_fwd_few<T, DP, 1, 4> : k_attn_fwd_few<T, DP, 2, 4>, 256, true, shared ? 4 : 1};
+        }
         constexpr int NQ = wide ? 2 : 1;  // one wave
         return {16 * NQ, 32, pass == DQ ? k_attn_dq<T, DP, 1, NQ, 32> : k_attn_dkv<T, DP, 1, NQ, 32>, 64, false};
     }
@@ -998,10 +1119,10 @@ Shape choose(Pass pass, int n_col, int64_t n_bh) {
 }
 
 Shape choose(const AttnP& p, Pass pass) {
-    const int n_col = pass == DKV ? p.Lk : p.Lq;
+    const int n_col = pass == DKV ? p.Lk : p.Lq, w = pass == DKV ? p.Lq : p.Lk;
     const int64_t n = (int64_t)p.B * (pass == DKV ? p.Hkv : p.H);
-    if (p.dtype == 1) return p.D <= 32 ? choose<bf16, 32>(pass, n_col, n) : p.D <= 64 ? choose<bf16, 64>(pass, n_col, n) : choose<bf16, 128>(pass, n_col, n);
-    return p.D <= 32 ? choose<float, 32>(pass, n_col, n) : p.D <= 64 ? choose<float, 64>(pass, n_col, n) : choose<float, 128>(pass, n_col, n);
+    if (p.dtype == 1) return p.D <= 32 ? choose<bf16, 32>(pass, n_col, w, n) : p.D <= 64 ? choose<bf16, 64>(pass, n_col, w, n) : choose<bf16, 128>(pass, n_col, w, n);
+    return p.D <= 32 ? choose<float, 32>(pass, n_col, w, n) : p.D <= 64 ? choose<float, 64>(pass, n_col, w, n) : choose<float, 128>(pass, n_col, w, n);
 }
 
 // Few workgroups and a long walk: the walk is split over workgroups whose results a second kernel joins (about 5 us), until the chip has
@@ -1018,8 +1139,7 @@ Plan plan(const AttnP& p, Pass pass) {
     r.n_col_tile = (n_col + r.s.col_tile - 1) / r.s.col_tile;
     r.n_bh = (int64_t)p.B * (pass == DKV ? p.Hkv : p.H);
     const int64_t base = r.n_bh * r.n_col_tile;
-    // a wave of its own for every problem fills the chip from 2048 problems on; below, and with a walk to share, a workgroup takes one
-    r.wpp = r.s.few && walk > 64 && base < 2048 ? 4 : 1;
+    r.wpp = r.s.wpp;
     const int step = r.s.walk_tile * r.wpp;
     const int64_t steps = (int64_t)((walk + step - 1) / step) * (pass == DKV ? p.G : 1), slots = 512 * 4 / (r.s.few ? r.wpp : r.s.threads / 64);
     int64_t n = base * 2 <= slots ? slots / (base > 0 ? base : 1) : 1;
@@ -1056,8 +1176,31 @@ const char* launch(AttnP p, const Plan& r, hipStream_t s) {
     return nullptr;
 }
 
-// both axes within one wave's reach: the whole backward pass is one kernel, as far as its operands fit the registers
-bool small(const AttnP& p) { return p.Lq >= 1 && p.Lk >= 1 && p.Lq <= 32 && p.Lk <= 32 && p.D <= (p.dtype == 1 ? 64 : 32); }
+// Short problems whose backward pass is one kernel: up to 32 x 32 (no shared heads) one wave does it all, as far as its operands fit the
+// registers; up to 64 x 64 one workgroup, as far as its four tiles fit LDS (fp32 with D > 64 does not).  Against the two-kernel form: 20 x 20, fp32 421 -> 231 us
+// (8192 x 4 heads); 61 x 61, bf16 one launch and one allocation less, which is what such a call costs.
+enum Short { NONE, WAVE, GROUP };
+Short short_backward(const AttnP& p) {
+    if (p.Lq < 1 || p.Lk < 1) return NONE;
+    if (p.G == 1 && p.Lq <= 32 && p.Lk <= 32 && p.D <= (p.dtype == 1 ? 64 : 32)) return WAVE;
+    if (p.Lq <= 64 && p.Lk <= 64 && (p.dtype == 1 || p.D <= 64)) return GROUP;
+    return NONE;
+}
+template <typename T>
+void launch_short(const AttnP& p, Short kind, hipStream_t s) {
+    const int64_t n = (int64_t)p.B * p.Hkv;
+    void (*kernel)(AttnP) = nullptr;
+    if (kind == WAVE) {
+        kernel = k_attn_bwd_small<T, 32>;
+        if constexpr (sizeof(T) == 2)
+            if (p.D > 32) kernel = k_attn_bwd_small<T, 64>;
+    } else {
+        kernel = p.D <= 32 ? k_attn_bwd_mid<T, 32> : k_attn_bwd_mid<T, 64>;
+        if constexpr (sizeof(T) == 2)
+            if (p.D > 64) kernel = k_attn_bwd_mid<T, 128>;
+    }
+    if (n) kernel<<<dim3((unsigned)(kind == WAVE ? (n + 3) / 4 : n)), dim3(256), 0, s>>>(p);  // (B * H <= 2^30)
+}
 
 template <typename T>
 void launch_sum(const float* part, int n_split, int B, int L, int H, int D, void* dst, const int64_t* st, hipStream_t s) {
@@ -1069,7 +1212,7 @@ void launch_sum(const float* part, int n_split, int B, int L, int H, int D, void
 
 int64_t attention_workspace(const AttnP& p, bool backward) {
     if (!backward) return 4 * part_floats(p, FWD, plan(p, FWD).n_split);
-    if (small(p)) return 0;
+    if (short_backward(p)) return 0;
     const int64_t a = part_floats(p, DQ, plan(p, DQ).n_split), b = part_floats(p, DKV, plan(p, DKV).n_split);
     return 4 * ((int64_t)p.B * p.H * p.Lq + (a > b ? a : b));  // delta, and the parts of one pass after the other
 }
@@ -1093,11 +1236,11 @@ const char* run_attention(AttnP p, float* ws, hipStream_t s) {
 }
 
 const char* run_attention_backward(AttnP p, float* ws, hipStream_t s) {
-    if (small(p)) {
-        const int64_t blocks = ((int64_t)p.B * p.Hkv + 3) / 4;
-        if (blocks > 0x7fffff00) return "too many workgroups (batch x heads > 2^33)";
-        auto kernel = p.dtype == 1 ? (p.D <= 32 ? k_attn_bwd_small<bf16, 32> : k_attn_bwd_small<bf16, 64>) : k_attn_bwd_small<float, 32>;
-        if (blocks) kernel<<<dim3((unsigned)blocks), dim3(256), 0, s>>>(p);
+    if (const Short kind = short_backward(p)) {
+        if (p.dtype == 1)
+            launch_short<bf16>(p, kind, s);
+        else
+            launch_short<float>(p, kind, s);
         return nullptr;
     }
     p.delta = ws;

@@ -396,6 +396,106 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear_direct(const LinearP p)
     }
 }
 
+// Both gradient products of a layer of at most 128 x 128 over many rows, in one walk: dy (and what gates it) and x are read once, where the
+// two products of their own read dy twice.  A workgroup of eight waves keeps W in LDS, walks tiles of RT rows in steps of the grid, and
+// holds its part of dW (64 x 32 of 128 x 128 per wave) in registers; dx of a tile leaves at once.  HBM-bound: 163840 rows of 128 fp32,
+// 336 MB, see DESIGN's table.
+template <typename T, bool GATED>
+__global__ __launch_bounds__(512) void k_linear_bwd_rows(const LinearP p) {
+    constexpr int NP = Planes<T>::N, NT = 512, RT = NP == 3 ? 32 : 64, F = 128, LD = F + LDS_PAD, CR = RT / 16;
+    __shared__ __attribute__((aligned(16))) bf16 lw[NP * F * LD];
+    __shared__ __attribute__((aligned(16))) bf16 lz[NP * RT * LD];
+    __shared__ __attribute__((aligned(16))) bf16 lx[NP * RT * LD];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, g = lane >> 4;
+    const bool ragged_k = p.K % 8 != 0, ragged_n = p.N % 8 != 0;
+    const T* act = GATED ? (const T*)p.act : nullptr;
+    {
+        Tile<T, F, F, NT, false, false> tw;
+        tw.load((const T*)p.weight, p.K, 0, p.N, 0, p.K, nullptr, nullptr, tid);
+        tw.settle(ragged_k, tid);
+        tw.store(lw, tid);
+    }
+    Tile<T, RT, F, NT, GATED, false> tz;
+    Tile<T, RT, F, NT, false, false> tx;
+    f32x4 acc[2][4];  // dW: input features wr + 16 r .., output features wc + 16 c ..
+    const int wr = (wave & 1) * 64, wc = (wave >> 1) * 32;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[c][r] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    float sums[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    int64_t m0 = (int64_t)blockIdx.x * RT;
+    auto load = [&](int64_t m) {
+        tz.load((const T*)p.d_out, p.N, m, p.M, 0, p.N, p.row_valid, act, tid);
+        tx.load((const T*)p.x, p.K, m, p.M, 0, p.K, p.row_valid, nullptr, tid);
+    };
+    if (m0 < p.M) load(m0);
+    for (; m0 < p.M; m0 += (int64_t)gridDim.x * RT) {
+        tz.settle(ragged_n, tid);
+        tx.settle(ragged_k, tid);
+        tz.add_columns(sums);
+        __syncthreads();
+        tz.store(lz, tid);
+        tx.store(lx, tid);
+        __syncthreads();
+        if (m0 + (int64_t)gridDim.x * RT < p.M) load(m0 + (int64_t)gridDim.x * RT);
+        f32x4 dx[CR];  // of input features 16 wave ..
+#pragma unroll
+        for (int c = 0; c < CR; ++c) dx[c] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < F; kk += 32) {
+            Frag<NP> fw;
+            frag_cols<NP, LD>(lw, (size_t)F * LD, kk + 8 * g, kk + 8 * g + 4, wave * 16, lane, fw);
+#pragma unroll
+            for (int c = 0; c < CR; ++c) {
+                Frag<NP> fz;
+                frag_rows<NP, LD>(lz, (size_t)RT * LD, c * 16, kk, lane, fz);
+                dx[c] = mma<NP>(fw, fz, dx[c]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < CR; ++c) {
+            const int64_t m = m0 + c * 16 + i16;
+            const int k = wave * 16 + 4 * g;
+            if (m < p.M && k < p.K) store4((T*)p.dx + m * p.K + k, p.K - k, dx[c]);
+        }
+#pragma unroll
+        for (int kk = 0; kk < RT; kk += 32) {
+            Frag<NP> fx[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) frag_cols<NP, LD>(lx, (size_t)RT * LD, kk + 8 * g, kk + 8 * g + 4, wr + r * 16, lane, fx[r]);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                Frag<NP> fz;
+                frag_cols<NP, LD>(lz, (size_t)RT * LD, kk + 8 * g, kk + 8 * g + 4, wc + c * 16, lane, fz);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[c][r] = mma<NP>(fx[r], fz, acc[c][r]);
+            }
+        }
+    }
+    float* part = p.part + (int64_t)blockIdx.x * ((int64_t)p.N * p.K + p.N);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int n = wc + c * 16 + i16, k = wr + r * 16 + 4 * g;
+            if (n < p.N && k < p.K) store4(part + (int64_t)n * p.K + k, p.K - k, acc[c][r]);
+        }
+    // db: the threads of one chunk of columns add up, in thread order
+    constexpr int CH = F / 8, RW = NT / CH;
+    static_assert(RW * F * 4 <= (int)sizeof(lw), "the column sums fit the weight's tile");
+    float* red = reinterpret_cast<float*>(lw);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) red[(tid / CH) * F + (tid % CH) * 8 + j] = sums[j];
+    __syncthreads();
+    if (tid < p.N) {
+        float s = 0.f;
+        for (int k = 0; k < RW; ++k) s += red[k * F + tid];
+        part[(int64_t)p.N * p.K + tid] = s;
+    }
+}
+
 // [dW, db][i] = sum over the splits of part[split][N K + N], always in the same order: 16 groups of 4 elements x 16 lanes over the splits
 template <typename T>
 __global__ __launch_bounds__(256) void k_linear_sum(const float* part, int n_split, int64_t n_w, int n_b, T* dw, T* db) {
@@ -508,14 +608,30 @@ void launch_sum(const LinearP& p, int n_split, hipStream_t s) {
 
 }  // namespace
 
-int64_t linear_workspace(const LinearP& p) {
-    const int n = plan<DW>(p).p.n_split;
-    return n > 1 ? 4 * (int64_t)n * ((int64_t)p.N * p.K + p.N) : 0;
+// both gradients of a narrow layer over many rows: k_linear_bwd_rows
+bool rows_backward(const LinearP& p) { return p.N >= 8 && p.K >= 8 && p.N <= 128 && p.K <= 128 && p.M >= 16384; }
+constexpr int ROWS_BLOCKS = 256;  // one per CU: its LDS holds the weight
+
+int64_t linear_workspace(const LinearP& p) {  // (whichever gradients are wanted)
+    const int64_t one = (int64_t)p.N * p.K + p.N;
+    const int n = plan<DW>(p).p.n_split, rows = rows_backward(p) ? ROWS_BLOCKS : 0;
+    return 4 * one * (n > 1 && n > rows ? n : rows);
 }
 
 const char* run_linear(const LinearP& p, hipStream_t s) { return launch(plan<FWD>(p), s); }
 
 const char* run_linear_backward(LinearP p, float* ws, hipStream_t s) {
+    if (rows_backward(p) && p.dx && p.dw) {
+        p.part = ws;
+        void (*kernel)(LinearP) = p.dtype == 1 ? (p.act ? k_linear_bwd_rows<bf16, true> : k_linear_bwd_rows<bf16, false>)
+                                               : (p.act ? k_linear_bwd_rows<float, true> : k_linear_bwd_rows<float, false>);
+        kernel<<<dim3(ROWS_BLOCKS), dim3(512), 0, s>>>(p);
+        if (p.dtype == 1)
+            launch_sum<bf16>(p, ROWS_BLOCKS, s);
+        else
+            launch_sum<float>(p, ROWS_BLOCKS, s);
+        return nullptr;
+    }
     if (p.dx)
         if (const char* e = launch(plan<DX>(p), s)) return e;
     if (!p.dw && !p.db) return nullptr;

@@ -33,7 +33,9 @@ struct NormP {
     const void *x, *weight, *bias, *d_out;
     void *y, *dx, *dw, *db;
     float *mean, *rstd;
-    float* part;  // of one launch: [workgroups][2 C]
+    // of one launch
+    int row_blocks;
+    float* part;  // [row_blocks][2 C]
 };
 int64_t norm_workspace(const NormP& p);
 const char* run_norm(const NormP& p, hipStream_t s);
