@@ -74,7 +74,7 @@ class Ins:
             return
         if _VMEM_LOAD.match(self.op):
             self.kind = "vmem"
-            to_lds = " lds" in (" " + text)
+            to_lds = " lds" in (" " + text) or "_lds_" in self.op  # (global_load_lds_*: the first operand is the address)
             returns = not self.op.startswith(("global_atomic", "buffer_atomic", "flat_atomic")) or " glc" in text or " sc0" in text
             if ops and not to_lds and returns:
                 self.dst = regs(ops[0])

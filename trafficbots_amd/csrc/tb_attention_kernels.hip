@@ -197,9 +197,9 @@ __device__ __forceinline__ void finish(const AttnP& p, const f32x4 (&acc)[DN], f
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-template <typename T, int DP, int NW, int NQ, int KT>
-__global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AttnP p) {
-    constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, KN = KT / 16, NT = 64 * NW, LD = DP + LDS_PAD, QT = 16 * NQ * NW;
+template <typename T, int DP, int NQ, int KT>
+__global__ __launch_bounds__(256) void k_attn_fwd(const AttnP p) {
+    constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, KN = KT / 16, NT = 256, LD = DP + LDS_PAD, QT = 64 * NQ;
     __shared__ __attribute__((aligned(16))) bf16 lk[NP * KT * LD];
     __shared__ __attribute__((aligned(16))) bf16 lv[NP * KT * LD];
     __shared__ __attribute__((aligned(16))) float lb[KT];
@@ -325,11 +325,92 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnP p) {
     if (col == 0) p.lse[row] = on ? (ref + __builtin_amdgcn_logf(sum)) * LN2 : NEG_INF;
 }
 
+// ------------------------------------------------------------------------------------------------ backward: what its kernels share
+// the columns' side of a query: q, do, -lse in powers of two (-inf where it takes no part: p = 2^(-inf) = 0) and D = do . out
+template <typename T, int KC>
+__device__ __forceinline__ void query_columns(const AttnP& p, const Valid& qvalid, int b, int h, int q, int lane, Frag<Planes<T>::N> (&qf)[KC], Frag<Planes<T>::N> (&gf)[KC],
+                                              float& nlse, float& delta) {
+    const int64_t qc = min(q, p.Lq - 1);
+    const bool on = qvalid[qc] && q < p.Lq;
+    const float lse = p.lse[((int64_t)b * p.H + h) * p.Lq + qc];
+    load_columns<T, KC>(p, (const T*)p.q + b * p.qs[0] + qc * p.qs[1] + h * p.qs[2], on, lane, qf);
+    Held<T> go[KC], o[KC];
+    load_columns<T, KC>(p, (const T*)p.d_out + b * p.dos[0] + qc * p.dos[1] + h * p.dos[2], on, lane, go);
+    load_columns<T, KC>(p, (const T*)p.out + b * p.os[0] + qc * p.os[1] + h * p.os[2], on, lane, o);
+    float dot = 0.f;
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dot = __builtin_fmaf(go[kc].get(e), o[kc].get(e), dot);
+        go[kc].planes(gf[kc].p);
+    }
+    delta = sum_over_groups(dot);
+    nlse = !on || lse == NEG_INF ? NEG_INF : -lse * LOG2E;
+}
+// a query's / a key's gradients, or this split's part of them
+template <typename T, int DN>
+__device__ __forceinline__ void store_dq(const AttnP& p, const f32x4 (&acc)[DN], int b, int h, int q, int split, int g) {
+#pragma unroll
+    for (int d = 0; d < DN; ++d) {
+        const int col = d * 16 + 4 * g;
+        if (col >= p.D) continue;
+        const f32x4 o = acc[d] * p.scale;
+        if (p.n_split > 1)
+            store4(p.part + (((int64_t)split * p.B * p.Lq + (int64_t)b * p.Lq + q) * p.H + h) * p.D + col, p.D - col, o);
+        else
+            store4((T*)p.dq + b * p.dqs[0] + q * p.dqs[1] + h * p.dqs[2] + col, p.D - col, o);
+    }
+}
+template <typename T, int DN>
+__device__ __forceinline__ void store_dkv(const AttnP& p, const f32x4 (&dk)[DN], const f32x4 (&dv)[DN], bool on, int b, int hk, int key, int split, int g) {
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < DN; ++d) {
+        const int col = d * 16 + 4 * g;
+        if (col >= p.D) continue;
+        const f32x4 ok = on ? dk[d] * p.scale : zero, ov = on ? dv[d] : zero;
+        if (p.n_split > 1) {
+            const int64_t at = (((int64_t)split * p.B * p.Lk + (int64_t)b * p.Lk + key) * p.Hkv + hk) * p.D + col;
+            store4(p.part + at, p.D - col, ok);
+            store4(p.part + (int64_t)p.n_split * p.B * p.Lk * p.Hkv * p.D + at, p.D - col, ov);
+        } else {
+            store4((T*)p.dk + b * p.dks[0] + key * p.dks[1] + hk * p.dks[2] + col, p.D - col, ok);
+            store4((T*)p.dv + b * p.dvs[0] + key * p.dvs[1] + hk * p.dvs[2] + col, p.D - col, ov);
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ few columns: private walks
 // With at most 32 columns a workgroup has nothing to share: each wave walks 32 rows at a time on its own.  The rows it needs as A operand it
 // loads straight into that layout; only what the second product reads down its rows goes through LDS, a region of the wave's own, so
 // there is no barrier in the walk.  One wave takes one problem; with `wpp` = NW (a single query over a long cache) the waves of a workgroup
 // share the walk of one problem and join at its end.
+// wave -> (row of the (batch, head) list, split, column tile); with wpp > 1 all waves of a workgroup get the same, and none is beyond the list
+__device__ __forceinline__ bool decode_few(const AttnP& p, int n_bh, int n_wave, int wave, int& bh, int& split, int& tile) {
+    const int64_t id = p.wpp > 1 ? blockIdx.x : (int64_t)blockIdx.x * n_wave + wave, rest = id / n_bh;
+    bh = (int)(id % n_bh);
+    tile = (int)(rest % p.n_col_tile);
+    split = (int)(rest / p.n_col_tile);
+    return split < p.n_split;
+}
+// sum of the waves' accumulators into wave 0's, the upper half into the lower until one is left (`red`: half the waves' accumulators)
+template <int NW, int N>
+__device__ __forceinline__ void join_waves(f32x4 (&acc)[N], float* red, int wave, int lane) {
+#pragma unroll
+    for (int half = NW / 2; half >= 1; half >>= 1) {
+        __syncthreads();
+        if (wave >= half && wave < 2 * half) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) *reinterpret_cast<f32x4*>(red + (((wave - half) * N + i) * 64 + lane) * 4) = acc[i];
+        }
+        __syncthreads();
+        if (wave < half) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] += *reinterpret_cast<const f32x4*>(red + ((wave * N + i) * 64 + lane) * 4);
+        }
+    }
+}
+
 // which of a lane's two rows (one of each 16-row tile) are there and valid
 struct Rows32 {
     uint8_t valid[2];
@@ -389,15 +470,14 @@ __device__ __forceinline__ void row_bias(const Rows32& ok, int lane, f32x4 (&bia
 template <typename T, int DP, int NQ, int NW>
 __global__ __launch_bounds__(64 * NW) void k_attn_fwd_few(const AttnP p) {
     constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, LD = DP + LDS_PAD;
-    constexpr int JOIN = NW / 2 * 16 * NQ * DP * 2;  // (in bf16 elements) half the waves' accumulators
+    constexpr int JOIN = NW / 2 * 16 * DP * 2;  // (in bf16 elements) half the waves' accumulators of a column tile
     constexpr int REGION = NW * NP * 32 * LD > JOIN ? NW * NP * 32 * LD : JOIN;
     __shared__ __attribute__((aligned(16))) bf16 region[REGION];
     __shared__ float ml[2][NW][16 * NQ];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, g = lane >> 4;
     const int part = p.wpp > 1 ? wave : 0;
-    const int64_t id = p.wpp > 1 ? blockIdx.x : (int64_t)blockIdx.x * NW + wave;
-    const int n_bh = p.B * p.H, split = (int)(id / n_bh), bh = (int)(id % n_bh);
-    if (split >= p.n_split) return;  // (wpp > 1: the grid has no such workgroup)
+    int bh, split, tile;
+    if (!decode_few(p, p.B * p.H, NW, wave, bh, split, tile)) return;
     const int b = bh / p.H, h = bh % p.H, hk = h / p.G, off = p.Lk - p.Lq;
     const T* kp = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
     const T* vp = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
@@ -497,22 +577,7 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd_few(const AttnP p) {
             for (int d = 0; d < DN; ++d) acc[n][d] *= alpha;
         }
 #pragma unroll
-        for (int half = NW / 2; half >= 1; half >>= 1) {
-            if (wave >= half && wave < 2 * half) {
-#pragma unroll
-                for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                    for (int d = 0; d < DN; ++d) *reinterpret_cast<f32x4*>(red + ((((wave - half) * NQ + n) * DN + d) * 64 + lane) * 4) = acc[n][d];
-            }
-            __syncthreads();
-            if (wave < half) {
-#pragma unroll
-                for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                    for (int d = 0; d < DN; ++d) acc[n][d] += *reinterpret_cast<const f32x4*>(red + (((wave * NQ + n) * DN + d) * 64 + lane) * 4);
-            }
-            __syncthreads();
-        }
+        for (int n = 0; n < NQ; ++n) join_waves<NW, DN>(acc[n], red, wave, lane);
         if (wave) return;
     }
 #pragma unroll
@@ -522,10 +587,228 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd_few(const AttnP p) {
     }
 }
 
+// dq of at most 16 NQ queries per tile: as above, K down its rows from the wave's LDS region
+template <typename T, int DP, int NQ>
+__global__ __launch_bounds__(256) void k_attn_dq_few(const AttnP p) {
+    constexpr int NP = Planes<T>::N, NW = 4, KC = DP / 32, DN = DP / 16, LD = DP + LDS_PAD;
+    __shared__ __attribute__((aligned(16))) bf16 region[NW * NP * 32 * LD];
+    static_assert(NW / 2 * 16 * DP * 4 <= (int)sizeof(region), "the join fits");
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, g = lane >> 4;
+    int bh, split, tile;
+    if (!decode_few(p, p.B * p.H, NW, wave, bh, split, tile)) return;
+    const int part = p.wpp > 1 ? wave : 0;
+    const int b = bh / p.H, h = bh % p.H, hk = h / p.G, off = p.Lk - p.Lq, qb = tile * 16 * NQ;
+    const T* kp = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
+    const T* vp = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
+    const Valid kvalid(p.key_valid, (int64_t)b * p.Lk), qvalid(p.query_valid, (int64_t)b * p.Lq);
+    bf16* lk = region + wave * NP * 32 * LD;
+
+    const int first = split * p.split_len, step = 32 * p.wpp;
+    int jend = min(p.Lk, first + p.split_len), j0 = first + part * 32;
+    if (p.causal) jend = min(jend, min(p.Lq, qb + 16 * NQ) + off);
+    Held<T> rk[2][KC], rv[2][KC];
+    Rows32 ok;
+    if (j0 < jend) {
+        load_rows32<T, KC>(p, kp, p.ks[1], kvalid, j0, jend, lane, rk, ok);
+        load_rows32<T, KC>(p, vp, p.vs[1], kvalid, j0, jend, lane, rv, ok);
+    }
+    Frag<NP> qf[NQ][KC], gf[NQ][KC];
+    f32x4 acc[NQ][DN];
+    float nlse[NQ], delta[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        query_columns<T, KC>(p, qvalid, b, h, qb + n * 16 + i16, lane, qf[n], gf[n], nlse[n], delta[n]);
+        const int q = qb + n * 16 + i16;
+        if (q < p.Lq && g == 0 && split == 0 && part == 0) p.delta[((int64_t)b * p.H + h) * p.Lq + q] = delta[n];
+#pragma unroll
+        for (int d = 0; d < DN; ++d) acc[n][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+    for (; j0 < jend; j0 += step) {
+        Frag<NP> kf[2][KC], vf[2][KC];
+        f32x4 bias[2];
+        row_bias(ok, lane, bias);
+        keep_rows32<T, KC>(p, rk, ok, lane);
+        keep_rows32<T, KC>(p, rv, ok, lane);
+        as_frags<T, KC>(rk, kf);
+        as_frags<T, KC>(rv, vf);
+        wave_fence();
+        rows32_to_lds<NP, KC, LD>(kf, lk, lane);
+        wave_fence();
+        if (j0 + step < jend) {
+            load_rows32<T, KC>(p, kp, p.ks[1], kvalid, j0 + step, jend, lane, rk, ok);
+            load_rows32<T, KC>(p, vp, p.vs[1], kvalid, j0 + step, jend, lane, rv, ok);
+        }
+        Frag<NP> df[NQ];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            f32x4 ds[2];
+            const int q = qb + n * 16 + i16;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                f32x4 s = bias[t], dp = {-delta[n], -delta[n], -delta[n], -delta[n]};
+#pragma unroll
+                for (int kc = 0; kc < KC; ++kc) {
+                    s = mma<NP>(kf[t][kc], qf[n][kc], s);
+                    dp = mma<NP>(vf[t][kc], gf[n][kc], dp);
+                }
+                const int j = j0 + t * 16 + 4 * g;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[e] = __builtin_fmaf(s[e], p.scale2, nlse[n]);
+                if (p.causal) hide_later(s, j, q + off);
+                if (p.mask) hide_masked(s, p.mask + b * p.mask_s[0] + (int64_t)min(q, p.Lq - 1) * p.mask_s[1], j, jend);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ds[t][e] = __builtin_amdgcn_exp2f(s[e]) * dp[e];
+            }
+            as_operand<NP>(ds[0], ds[1], df[n]);
+        }
+#pragma unroll
+        for (int d = 0; d < DN; ++d) {
+            Frag<NP> a;
+            frag_cols<NP, LD>(lk, (size_t)32 * LD, 4 * g, 16 + 4 * g, d * 16, lane, a);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) acc[n][d] = mma<NP>(a, df[n], acc[n][d]);
+        }
+    }
+    if (p.wpp > 1) {  // (workgroup-uniform)
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) join_waves<NW, DN>(acc[n], reinterpret_cast<float*>(region), wave, lane);
+        if (wave) return;
+    }
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+        if (qb + n * 16 + i16 < p.Lq) store_dq<T, DN>(p, acc[n], b, h, qb + n * 16 + i16, split, g);
+}
+
+// dk, dv of at most 16 NQ keys per tile: the walk goes over 32 queries at a time of every head of the group; dO, then Q pass through the region
+template <typename T, int DP, int NQ>
+__global__ __launch_bounds__(256) void k_attn_dkv_few(const AttnP p) {
+    constexpr int NP = Planes<T>::N, NW = 4, KC = DP / 32, DN = DP / 16, LD = DP + LDS_PAD;
+    __shared__ __attribute__((aligned(16))) bf16 region[NW * NP * 32 * LD];
+    __shared__ __attribute__((aligned(16))) float rowv[NW][2][32];
+    static_assert(NW / 2 * 16 * DP * 4 <= (int)sizeof(region), "the join fits");
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, g = lane >> 4;
+    int bh, split, tile;
+    if (!decode_few(p, p.B * p.Hkv, NW, wave, bh, split, tile)) return;
+    const int part = p.wpp > 1 ? wave : 0;
+    const int b = bh / p.Hkv, hk = bh % p.Hkv, off = p.Lk - p.Lq, kb = tile * 16 * NQ;
+    const Valid kvalid(p.key_valid, (int64_t)b * p.Lk), qvalid(p.query_valid, (int64_t)b * p.Lq);
+    bf16* lds = region + wave * NP * 32 * LD;
+    float* nlse_r = rowv[wave][0];
+    float* delta_r = rowv[wave][1];
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+
+    const int n_qt = (p.Lq + 31) / 32, per_first = p.causal ? min(n_qt, max(0, kb - off) / 32) : 0, per_head = n_qt - per_first;
+    const int n_step = p.G * per_head, len = (n_step + p.n_split - 1) / p.n_split, tend = min(n_step, (split + 1) * len);
+    int t = split * len + part;
+    Held<T> rq[2][KC], rg[2][KC];
+    Rows32 ok;
+    float r_lse[2], r_delta[2];
+    auto load = [&](int at) {
+        const int h = hk * p.G + at / per_head, q0 = (per_first + at % per_head) * 32;
+        load_rows32<T, KC>(p, (const T*)p.q + b * p.qs[0] + h * p.qs[2], p.qs[1], qvalid, q0, p.Lq, lane, rq, ok);
+        load_rows32<T, KC>(p, (const T*)p.d_out + b * p.dos[0] + h * p.dos[2], p.dos[1], qvalid, q0, p.Lq, lane, rg, ok);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int64_t row = ((int64_t)b * p.H + h) * p.Lq + min(q0 + u * 16 + i16, p.Lq - 1);
+            r_lse[u] = p.lse[row];
+            r_delta[u] = p.delta[row];
+        }
+    };
+    if (t < tend) load(t);
+    Frag<NP> kf[NQ][KC], vf[NQ][KC];
+    bool on[NQ];
+    f32x4 dk[NQ][DN], dv[NQ][DN];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int key = kb + n * 16 + i16, kc = min(key, p.Lk - 1);
+        on[n] = kvalid[kc] && key < p.Lk;
+        load_columns<T, KC>(p, (const T*)p.k + b * p.ks[0] + (int64_t)kc * p.ks[1] + hk * p.ks[2], on[n], lane, kf[n]);
+        load_columns<T, KC>(p, (const T*)p.v + b * p.vs[0] + (int64_t)kc * p.vs[1] + hk * p.vs[2], on[n], lane, vf[n]);
+#pragma unroll
+        for (int d = 0; d < DN; ++d) dk[n][d] = dv[n][d] = zero;
+    }
+    for (; t < tend; t += p.wpp) {
+        Frag<NP> qf[2][KC], gf[2][KC];
+        const int q0 = (per_first + t % per_head) * 32;
+        keep_rows32<T, KC>(p, rq, ok, lane);
+        keep_rows32<T, KC>(p, rg, ok, lane);
+        as_frags<T, KC>(rq, qf);
+        as_frags<T, KC>(rg, gf);
+        wave_fence();
+        rows32_to_lds<NP, KC, LD>(gf, lds, lane);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if (g == 0) {
+                const bool in = ok.on(u, lane);
+                nlse_r[u * 16 + i16] = !in || r_lse[u] == NEG_INF ? NEG_INF : -r_lse[u] * LOG2E;
+                delta_r[u * 16 + i16] = in ? -r_delta[u] : 0.f;
+            }
+        wave_fence();
+        if (t + p.wpp < tend) load(t + p.wpp);
+        Frag<NP> pf[NQ], df[NQ];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            f32x4 pr[2], ds[2];
+            const int key = kb + n * 16 + i16;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int i = u * 16 + 4 * g;
+                const f32x4 nl = *reinterpret_cast<const f32x4*>(nlse_r + i);
+                f32x4 s = zero, dp = *reinterpret_cast<const f32x4*>(delta_r + i);
+#pragma unroll
+                for (int kc = 0; kc < KC; ++kc) {
+                    s = mma<NP>(qf[u][kc], kf[n][kc], s);
+                    dp = mma<NP>(gf[u][kc], vf[n][kc], dp);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[e] = __builtin_fmaf(s[e], p.scale2, nl[e]);
+                if (p.causal) hide_earlier(s, q0 + i, key - off);
+                if (p.mask) hide_masked_rows(s, p.mask + b * p.mask_s[0] + min(key, p.Lk - 1), p.mask_s[1], q0 + i, p.Lq);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    pr[u][e] = __builtin_amdgcn_exp2f(s[e]);
+                    ds[u][e] = pr[u][e] * dp[e];
+                }
+            }
+            as_operand<NP>(pr[0], pr[1], pf[n]);
+            as_operand<NP>(ds[0], ds[1], df[n]);
+        }
+#pragma unroll
+        for (int d = 0; d < DN; ++d) {
+            Frag<NP> a;
+            frag_cols<NP, LD>(lds, (size_t)32 * LD, 4 * g, 16 + 4 * g, d * 16, lane, a);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) dv[n][d] = mma<NP>(a, pf[n], dv[n][d]);
+        }
+        wave_fence();
+        rows32_to_lds<NP, KC, LD>(qf, lds, lane);
+        wave_fence();
+#pragma unroll
+        for (int d = 0; d < DN; ++d) {
+            Frag<NP> a;
+            frag_cols<NP, LD>(lds, (size_t)32 * LD, 4 * g, 16 + 4 * g, d * 16, lane, a);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) dk[n][d] = mma<NP>(a, df[n], dk[n][d]);
+        }
+    }
+    if (p.wpp > 1) {  // (workgroup-uniform)
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            join_waves<NW, DN>(dk[n], reinterpret_cast<float*>(region), wave, lane);
+            join_waves<NW, DN>(dv[n], reinterpret_cast<float*>(region), wave, lane);
+        }
+        if (wave) return;
+    }
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+        if (kb + n * 16 + i16 < p.Lk) store_dkv<T, DN>(p, dk[n], dv[n], on[n], b, hk, kb + n * 16 + i16, split, g);
+}
+
 // Backward of a whole problem with at most 32 queries and 32 keys: one wave per head (none of them
 // shared), everything loaded once.  Queries as columns
 // give dq; the scores once more with keys as columns give dk and dv.  The same registers serve as A and as B operand (both layouts
-// hold 8 components of one row).  K, dO and Q pass one after the other through the wave's LDS region to be read down their rows.
+// hold 8 components of one row).  D_i = sum_j p_ij dp_ij is summed here, where a row's probabilities are all at hand: `out` is not read, and
+// its rounding does not enter.  K, dO and Q pass one after the other through the wave's LDS region to be read down their rows.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void k_attn_bwd_small(const AttnP p) {
     constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, LD = DP + LDS_PAD;
@@ -558,75 +841,72 @@ __global__ __launch_bounds__(256, 2) void k_attn_bwd_small(const AttnP p) {
     const int h = hk;
     Frag<NP> qf[2][KC], gf[2][KC];
     {
-        float nlse[2], delta[2];
+        float nlse[2];
         {
-            Held<T> q[2][KC], go[2][KC], o[2][KC];
+            Held<T> q[2][KC], go[2][KC];
             Rows32 ok;
             float lse[2];
 #pragma unroll
             for (int n = 0; n < 2; ++n) lse[n] = p.lse[((int64_t)b * p.H + h) * p.Lq + min(n * 16 + i16, p.Lq - 1)];
             load_rows32<T, KC>(p, (const T*)p.q + b * p.qs[0] + h * p.qs[2], p.qs[1], qvalid, 0, p.Lq, lane, q, ok);
             load_rows32<T, KC>(p, (const T*)p.d_out + b * p.dos[0] + h * p.dos[2], p.dos[1], qvalid, 0, p.Lq, lane, go, ok);
-            load_rows32<T, KC>(p, (const T*)p.out + b * p.os[0] + h * p.os[2], p.os[1], qvalid, 0, p.Lq, lane, o, ok);
             keep_rows32<T, KC>(p, q, ok, lane);
             keep_rows32<T, KC>(p, go, ok, lane);
-            keep_rows32<T, KC>(p, o, ok, lane);
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                float dot = 0.f;
-#pragma unroll
-                for (int kc = 0; kc < KC; ++kc)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) dot = __builtin_fmaf(go[n][kc].get(e), o[n][kc].get(e), dot);
-                delta[n] = sum_over_groups(dot);
-                nlse[n] = !ok.on(n, lane) || lse[n] == NEG_INF ? NEG_INF : -lse[n] * LOG2E;
-            }
+            for (int n = 0; n < 2; ++n) nlse[n] = !ok.on(n, lane) || lse[n] == NEG_INF ? NEG_INF : -lse[n] * LOG2E;
             as_frags<T, KC>(q, qf);
             as_frags<T, KC>(go, gf);
         }
         wave_fence();
         rows32_to_lds<NP, KC, LD>(kf, lds, lane);
+        // queries as columns: dq
+        Frag<NP> df[2];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-            if (g == 0) {
-                nlse_r[n * 16 + i16] = nlse[n];
-                delta_r[n * 16 + i16] = -delta[n];
+        for (int n = 0; n < 2; ++n) {
+            f32x4 pr[2], dp[2];
+            float dot = 0.f;
+            const int q = n * 16 + i16;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                f32x4 s = bias[t];
+                dp[t] = zero;
+#pragma unroll
+                for (int kc = 0; kc < KC; ++kc) {
+                    s = mma<NP>(kf[t][kc], qf[n][kc], s);
+                    dp[t] = mma<NP>(vf[t][kc], gf[n][kc], dp[t]);
+                }
+                const int j = t * 16 + 4 * g;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[e] = __builtin_fmaf(s[e], p.scale2, nlse[n]);
+                if (p.causal) hide_later(s, j, q + off);
+                if (p.mask) hide_masked(s, p.mask + b * p.mask_s[0] + (int64_t)min(q, p.Lq - 1) * p.mask_s[1], j, p.Lk);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    pr[t][e] = __builtin_amdgcn_exp2f(s[e]);
+                    dot = __builtin_fmaf(pr[t][e], dp[t][e], dot);
+                }
             }
+            dot = sum_over_groups(dot);  // D = sum_j p dp
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) pr[t][e] *= dp[t][e] - dot;
+            as_operand<NP>(pr[0], pr[1], df[n]);
+            if (g == 0) {
+                nlse_r[q] = nlse[n];
+                delta_r[q] = -dot;
+            }
+        }
         wave_fence();
-        {  // queries as columns: dq
-            Frag<NP> df[2];
+#pragma unroll
+        for (int d = 0; d < DN; ++d) {
+            Frag<NP> a;
+            frag_cols<NP, LD>(lds, (size_t)32 * LD, 4 * g, 16 + 4 * g, d * 16, lane, a);
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-                f32x4 ds[2];
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    f32x4 s = bias[t], dp = {-delta[n], -delta[n], -delta[n], -delta[n]};
-#pragma unroll
-                    for (int kc = 0; kc < KC; ++kc) {
-                        s = mma<NP>(kf[t][kc], qf[n][kc], s);
-                        dp = mma<NP>(vf[t][kc], gf[n][kc], dp);
-                    }
-                    const int q = n * 16 + i16, j = t * 16 + 4 * g;
-                    f32x4 x;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(s[e], p.scale2, nlse[n]);
-                    if (p.causal) hide_later(x, j, q + off);
-                    if (p.mask) hide_masked(x, p.mask + b * p.mask_s[0] + (int64_t)min(q, p.Lq - 1) * p.mask_s[1], j, p.Lk);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) ds[t][e] = __builtin_amdgcn_exp2f(x[e]) * dp[e];
-                }
-                as_operand<NP>(ds[0], ds[1], df[n]);
-            }
-#pragma unroll
-            for (int d = 0; d < DN; ++d) {
-                Frag<NP> a;
-                frag_cols<NP, LD>(lds, (size_t)32 * LD, 4 * g, 16 + 4 * g, d * 16, lane, a);
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const int q = n * 16 + i16, col = d * 16 + 4 * g;
-                    const f32x4 o = mma<NP>(a, df[n], zero) * p.scale;
-                    if (q < p.Lq && col < p.D) store4((T*)p.dq + b * p.dqs[0] + q * p.dqs[1] + h * p.dqs[2] + col, p.D - col, o);
-                }
+                const int q = n * 16 + i16, col = d * 16 + 4 * g;
+                const f32x4 o = mma<NP>(a, df[n], zero) * p.scale;
+                if (q < p.Lq && col < p.D) store4((T*)p.dq + b * p.dqs[0] + q * p.dqs[1] + h * p.dqs[2] + col, p.D - col, o);
             }
         }
     }
@@ -681,25 +961,27 @@ __global__ __launch_bounds__(256, 2) void k_attn_bwd_small(const AttnP p) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward: one tile
-// KT keys in LDS (bias `lb`: 0 or -inf), queries as columns: acc += K^T ds
-template <int NP, int DP, int NQ, int KT>
+// KT keys in LDS (bias `lb`: 0 or -inf), queries as columns: acc += K^T ds.  WHOLE: these are all the keys, and `delta` is the sum over p dp
+// taken here; otherwise it is given (D = do . out).
+template <int NP, int DP, int NQ, int KT, bool WHOLE = false>
 __device__ __forceinline__ void dq_tile(const AttnP& p, const bf16* lk, const bf16* lv, const float* lb, int lane, int b, int j0, int jend, bool diagonal, int off,
                                         const int (&qi)[NQ], const Frag<NP> (&qf)[NQ][DP / 32], const Frag<NP> (&gf)[NQ][DP / 32], const float (&nlse)[NQ],
-                                        const float (&delta)[NQ], f32x4 (&acc)[NQ][DP / 16]) {
-    constexpr int KC = DP / 32, DN = DP / 16, KN = KT / 16, LD = DP + LDS_PAD;
+                                        float (&delta)[NQ], f32x4 (&acc)[NQ][DP / 16]) {
+    constexpr int KC = DP / 32, DN = DP / 16, KN = KT / 16, LD = DP + LDS_PAD, STEP = WHOLE ? KN : 2;
     const int g = lane >> 4;
 #pragma unroll
-    for (int t2 = 0; t2 < KN; t2 += 2) {
-        f32x4 ds[NQ][2];
+    for (int t0 = 0; t0 < KN; t0 += STEP) {
+        f32x4 ds[NQ][STEP], dp[NQ][STEP];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int t = t2 + u;
-            f32x4 s[NQ], dp[NQ];
+        for (int u = 0; u < STEP; ++u) {
+            const int t = t0 + u;
+            f32x4 s[NQ];
             const f32x4 bias = *reinterpret_cast<const f32x4*>(lb + t * 16 + 4 * g);
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
                 s[n] = bias;
-                dp[n] = (f32x4){-delta[n], -delta[n], -delta[n], -delta[n]};
+                const float start = WHOLE ? 0.f : -delta[n];
+                dp[n][u] = (f32x4){start, start, start, start};
             }
 #pragma unroll
             for (int kc = 0; kc < KC; ++kc) {
@@ -709,7 +991,7 @@ __device__ __forceinline__ void dq_tile(const AttnP& p, const bf16* lk, const bf
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) {
                     s[n] = mma<NP>(a, qf[n][kc], s[n]);
-                    dp[n] = mma<NP>(v, gf[n][kc], dp[n]);
+                    dp[n][u] = mma<NP>(v, gf[n][kc], dp[n][u]);
                 }
             }
 #pragma unroll
@@ -720,18 +1002,36 @@ __device__ __forceinline__ void dq_tile(const AttnP& p, const bf16* lk, const bf
                 if (diagonal) hide_later(x, j0 + t * 16 + 4 * g, qi[n] + off);
                 if (p.mask) hide_masked(x, p.mask + b * p.mask_s[0] + (int64_t)min(qi[n], p.Lq - 1) * p.mask_s[1], j0 + t * 16 + 4 * g, jend);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) ds[n][u][e] = __builtin_amdgcn_exp2f(x[e]) * dp[n][e];
+                for (int e = 0; e < 4; ++e) ds[n][u][e] = __builtin_amdgcn_exp2f(x[e]) * (WHOLE ? 1.f : dp[n][u][e]);
             }
         }
-        Frag<NP> df[NQ];
+        if constexpr (WHOLE) {
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) as_operand<NP>(ds[n][0], ds[n][1], df[n]);
+            for (int n = 0; n < NQ; ++n) {
+                float dot = 0.f;
 #pragma unroll
-        for (int d = 0; d < DN; ++d) {
-            Frag<NP> a;
-            frag_cols<NP, LD>(lk, (size_t)KT * LD, t2 * 16 + 4 * g, (t2 + 1) * 16 + 4 * g, d * 16, lane, a);
+                for (int u = 0; u < STEP; ++u)
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) acc[n][d] = mma<NP>(a, df[n], acc[n][d]);
+                    for (int e = 0; e < 4; ++e) dot = __builtin_fmaf(ds[n][u][e], dp[n][u][e], dot);
+                delta[n] = sum_over_groups(dot);
+#pragma unroll
+                for (int u = 0; u < STEP; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) ds[n][u][e] *= dp[n][u][e] - delta[n];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < STEP; u += 2) {
+            Frag<NP> df[NQ];
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) as_operand<NP>(ds[n][u], ds[n][u + 1], df[n]);
+#pragma unroll
+            for (int d = 0; d < DN; ++d) {
+                Frag<NP> a;
+                frag_cols<NP, LD>(lk, (size_t)KT * LD, (t0 + u) * 16 + 4 * g, (t0 + u + 1) * 16 + 4 * g, d * 16, lane, a);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) acc[n][d] = mma<NP>(a, df[n], acc[n][d]);
+            }
         }
     }
 }
@@ -803,9 +1103,9 @@ __device__ __forceinline__ void dkv_tile(const AttnP& p, const bf16* lq, const b
 // ------------------------------------------------------------------------------------------------ backward: dq
 // (bf16, D = 128: two column tiles fit 256 registers with tiles of 32 keys, and two waves per SIMD then hide each other's LDS reads: 495 us
 // instead of 700 with one wave per SIMD and 64 keys, 8192 x 8192 causal, 16 heads)
-template <typename T, int DP, int NW, int NQ, int KT>
-__global__ __launch_bounds__(64 * NW, DP == 128 && NQ == 2 && NW == 4 ? 2 : 1) void k_attn_dq(const AttnP p) {
-    constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, KN = KT / 16, NT = 64 * NW, LD = DP + LDS_PAD, QT = 16 * NQ * NW;
+template <typename T, int DP, int NQ, int KT>
+__global__ __launch_bounds__(256, DP == 128 && NQ == 2 ? 2 : 1) void k_attn_dq(const AttnP p) {
+    constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, KN = KT / 16, NT = 256, LD = DP + LDS_PAD, QT = 64 * NQ;
     __shared__ __attribute__((aligned(16))) bf16 lk[NP * KT * LD];
     __shared__ __attribute__((aligned(16))) bf16 lv[NP * KT * LD];
     __shared__ __attribute__((aligned(16))) float lb[KT];
@@ -835,24 +1135,8 @@ __global__ __launch_bounds__(64 * NW, DP == 128 && NQ == 2 && NW == 4 ? 2 : 1) v
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         qi[n] = q0 + n * 16 + i16;
-        const bool in = qi[n] < p.Lq;
-        const int64_t qc = in ? qi[n] : p.Lq - 1, row = (int64_t)bh * p.Lq + qc;
-        const bool on = qvalid[qc] && in;
-        const float lse = p.lse[row];
-        load_columns<T, KC>(p, (const T*)p.q + b * p.qs[0] + qc * p.qs[1] + h * p.qs[2], on, lane, qf[n]);
-        Held<T> go[KC], o[KC];
-        load_columns<T, KC>(p, (const T*)p.d_out + b * p.dos[0] + qc * p.dos[1] + h * p.dos[2], on, lane, go);
-        load_columns<T, KC>(p, (const T*)p.out + b * p.os[0] + qc * p.os[1] + h * p.os[2], on, lane, o);
-        float dot = 0.f;
-#pragma unroll
-        for (int kc = 0; kc < KC; ++kc) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) dot = __builtin_fmaf(go[kc].get(e), o[kc].get(e), dot);
-            go[kc].planes(gf[n][kc].p);
-        }
-        delta[n] = sum_over_groups(dot);
-        nlse[n] = !on || lse == NEG_INF ? NEG_INF : -lse * LOG2E;  // an empty row: p = 2^(-inf) = 0
-        if (in && g == 0 && split == 0) p.delta[row] = delta[n];
+        query_columns<T, KC>(p, qvalid, b, h, qi[n], lane, qf[n], gf[n], nlse[n], delta[n]);
+        if (qi[n] < p.Lq && g == 0 && split == 0) p.delta[(int64_t)bh * p.Lq + qi[n]] = delta[n];
 #pragma unroll
         for (int d = 0; d < DN; ++d) acc[n][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
@@ -869,27 +1153,16 @@ __global__ __launch_bounds__(64 * NW, DP == 128 && NQ == 2 && NW == 4 ? 2 : 1) v
         dq_tile<NP, DP, NQ, KT>(p, lk, lv, lb, lane, b, j0, jend, diagonal, off, qi, qf, gf, nlse, delta, acc);
     }
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        if (qi[n] >= p.Lq) continue;
-#pragma unroll
-        for (int d = 0; d < DN; ++d) {
-            const int col = d * 16 + 4 * g;
-            if (col >= p.D) continue;
-            const f32x4 o = acc[n][d] * p.scale;
-            if (p.n_split > 1)
-                store4(p.part + (((int64_t)split * p.B * p.Lq + (int64_t)b * p.Lq + qi[n]) * p.H + h) * p.D + col, p.D - col, o);
-            else
-                store4((T*)p.dq + b * p.dqs[0] + qi[n] * p.dqs[1] + h * p.dqs[2] + col, p.D - col, o);
-        }
-    }
+    for (int n = 0; n < NQ; ++n)
+        if (qi[n] < p.Lq) store_dq<T, DN>(p, acc[n], b, h, qi[n], split, g);
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
 // Columns are keys; the walk goes over the query tiles of every head of the key's group, so the gradients of shared heads are summed
 // in registers.  A split takes a contiguous part of that walk.
-template <typename T, int DP, int NW, int NQ, int KT>
-__global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AttnP p) {
-    constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, KN = KT / 16, NT = 64 * NW, LD = DP + LDS_PAD, CT = 16 * NQ * NW;
+template <typename T, int DP, int NQ, int KT>
+__global__ __launch_bounds__(256) void k_attn_dkv(const AttnP p) {
+    constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, KN = KT / 16, NT = 256, LD = DP + LDS_PAD, CT = 64 * NQ;
     __shared__ __attribute__((aligned(16))) bf16 lq[NP * KT * LD];
     __shared__ __attribute__((aligned(16))) bf16 lg[NP * KT * LD];
     __shared__ __attribute__((aligned(16))) float ll[KT];
@@ -955,23 +1228,8 @@ __global__ __launch_bounds__(64 * NW) void k_attn_dkv(const AttnP p) {
         dkv_tile<NP, DP, NQ, KT>(p, lq, lg, ll, ld, lane, b, q0, diagonal, off, ki, kf, vf, dk, dv);
     }
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        if (ki[n] >= p.Lk) continue;
-#pragma unroll
-        for (int d = 0; d < DN; ++d) {
-            const int col = d * 16 + 4 * g;
-            if (col >= p.D) continue;
-            const f32x4 zero = {0.f, 0.f, 0.f, 0.f}, ok = on[n] ? dk[n][d] * p.scale : zero, ov = on[n] ? dv[n][d] : zero;
-            if (p.n_split > 1) {
-                const int64_t at = (((int64_t)split * p.B * p.Lk + (int64_t)b * p.Lk + ki[n]) * p.Hkv + hk) * p.D + col;
-                store4(p.part + at, p.D - col, ok);
-                store4(p.part + (int64_t)p.n_split * p.B * p.Lk * p.Hkv * p.D + at, p.D - col, ov);
-            } else {
-                store4((T*)p.dk + b * p.dks[0] + ki[n] * p.dks[1] + hk * p.dks[2] + col, p.D - col, ok);
-                store4((T*)p.dv + b * p.dvs[0] + ki[n] * p.dvs[1] + hk * p.dvs[2] + col, p.D - col, ov);
-            }
-        }
-    }
+    for (int n = 0; n < NQ; ++n)
+        if (ki[n] < p.Lk) store_dkv<T, DN>(p, dk[n], dv[n], on[n], b, hk, ki[n], split, g);
 }
 
 // ------------------------------------------------------------------------------------------------ backward of at most 64 x 64
@@ -1001,8 +1259,6 @@ __global__ __launch_bounds__(256) void k_attn_bwd_mid(const AttnP p) {
     for (int h = hk * p.G; h < (hk + 1) * p.G; ++h) {
         sq.load(p, (const T*)p.q + b * p.qs[0] + h * p.qs[2], p.qs[1], qvalid, 0, p.Lq, tid);
         sg.load(p, (const T*)p.d_out + b * p.dos[0] + h * p.dos[2], p.dos[1], qvalid, 0, p.Lq, tid);
-        Stage<T, DP, 256, L> so;
-        so.load(p, (const T*)p.out + b * p.os[0] + h * p.os[2], p.os[1], qvalid, 0, p.Lq, tid);
         const float r_lse = p.lse[((int64_t)b * p.H + h) * p.Lq + min(tid % L, p.Lq - 1)];
         const bool r_on = qvalid[min(tid % L, p.Lq - 1)] && tid % L < p.Lq;
         __syncthreads();  // (the head before is done with the tiles)
@@ -1012,23 +1268,13 @@ __global__ __launch_bounds__(256) void k_attn_bwd_mid(const AttnP p) {
         }
         sq.store(p, lq, nullptr, tid);
         sg.store(p, lg, nullptr, tid);
-        so.settle(p, tid);
-#pragma unroll
-        for (int c = 0; c < so.PT; ++c) {  // -D: a row's chunks are in adjacent lanes
-            float dot = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) dot = __builtin_fmaf(sg.r[c].get(e), so.r[c].get(e), dot);
-#pragma unroll
-            for (int x = 1; x < so.CH; x <<= 1) dot += __shfl_xor(dot, x);
-            const int idx = tid + c * 256;
-            if (idx % so.CH == 0) ld[idx / so.CH] = -dot;
-        }
         if (tid < L) ll[tid] = !r_on || r_lse == NEG_INF ? NEG_INF : -r_lse * LOG2E;
         __syncthreads();
         {
             Frag<NP> qf[1][KC], gf[1][KC];
             f32x4 acc[1][DN];
-            const float nlse[1] = {ll[col[0]]}, delta[1] = {-ld[col[0]]};
+            const float nlse[1] = {ll[col[0]]};
+            float delta[1];
 #pragma unroll
             for (int kc = 0; kc < KC; ++kc) {
                 frag_rows<NP, LD>(lq, (size_t)L * LD, wave * 16, kc * 32, lane, qf[0][kc]);
@@ -1036,13 +1282,15 @@ __global__ __launch_bounds__(256) void k_attn_bwd_mid(const AttnP p) {
             }
 #pragma unroll
             for (int d = 0; d < DN; ++d) acc[0][d] = zero;
-            dq_tile<NP, DP, 1, L>(p, lk, lv, lb, lane, b, 0, p.Lk, p.causal, off, col, qf, gf, nlse, delta, acc);
+            dq_tile<NP, DP, 1, L, true>(p, lk, lv, lb, lane, b, 0, p.Lk, p.causal, off, col, qf, gf, nlse, delta, acc);
+            if (g == 0) ld[col[0]] = -delta[0];
             if (col[0] < p.Lq) {
 #pragma unroll
                 for (int d = 0; d < DN; ++d)
                     if (d * 16 + 4 * g < p.D) store4((T*)p.dq + b * p.dqs[0] + col[0] * p.dqs[1] + h * p.dqs[2] + d * 16 + 4 * g, p.D - d * 16 - 4 * g, acc[0][d] * p.scale);
             }
         }
+        __syncthreads();  // every wave's D
         Frag<NP> kf[1][KC], vf[1][KC];
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) {
@@ -1094,8 +1342,8 @@ struct Shape {  // of one launch: columns per workgroup, walked rows per step of
 template <typename T, int DP, int NQ, int KT>
 Shape tiles(Pass pass) {  // four waves
     constexpr int KQ = DP == 128 && NQ == 2 ? 32 : KT;
-    if (pass == DQ) return {64 * NQ, KQ, k_attn_dq<T, DP, 4, NQ, KQ>, 256, false};
-    return {64 * NQ, KT, pass == FWD ? k_attn_fwd<T, DP, 4, NQ, KT> : k_attn_dkv<T, DP, 4, NQ, KT>, 256, false};
+    if (pass == DQ) return {64 * NQ, KQ, k_attn_dq<T, DP, NQ, KQ>, 256, false};
+    return {64 * NQ, KT, pass == FWD ? k_attn_fwd<T, DP, NQ, KT> : k_attn_dkv<T, DP, NQ, KT>, 256, false};
 }
 
 template <typename T, int DP>
@@ -1103,15 +1351,16 @@ Shape choose(Pass pass, int n_col, int walk, int64_t n_bh) {
     constexpr bool wide = sizeof(T) == 2 || DP == 32;  // two column tiles per wave fit the registers
     constexpr int KT = sizeof(T) == 2 || DP == 32 ? 64 : 32;
     if (n_col <= 32) {
-        if (pass == FWD) {
-            // one problem per workgroup below 2048 problems (with a walk to share), one per wave above; eight waves where their tiles fit LDS
-            const bool shared = walk > 64 && n_bh < 2048;
-            if constexpr (DP <= 64)
-                if (shared && n_col <= 16) return {32, 32, k_attn_fwd_few<T, DP, 1, 8>, 512, true, 8};
-            return {32, 32, n_col <= 16 ? k_attn_fwd_few<T, DP, 1, 4> : k_attn_fwd_few<T, DP, 2, 4>, 256, true, shared ? 4 : 1};
-        }
-        constexpr int NQ = wide ? 2 : 1;  // one wave
-        return {16 * NQ, 32, pass == DQ ? k_attn_dq<T, DP, 1, NQ, 32> : k_attn_dkv<T, DP, 1, NQ, 32>, 64, false};
+        // one problem per workgroup below 2048 problems (with a walk to share), one per wave above; the forward on eight waves where their
+        // tiles fit LDS (one query, 1024 keys, fp32: 14.2 us on four, 12.4 on eight)
+        const bool shared = walk > 64 && n_bh < 2048;
+        const int wpp = shared ? 4 : 1;
+        constexpr int NQ = wide ? 2 : 1;
+        if (pass == DQ) return n_col <= 16 ? Shape{16, 32, k_attn_dq_few<T, DP, 1>, 256, true, wpp} : Shape{16 * NQ, 32, k_attn_dq_few<T, DP, NQ>, 256, true, wpp};
+        if (pass == DKV) return n_col <= 16 ? Shape{16, 32, k_attn_dkv_few<T, DP, 1>, 256, true, wpp} : Shape{16 * NQ, 32, k_attn_dkv_few<T, DP, NQ>, 256, true, wpp};
+        if constexpr (DP <= 64)
+            if (shared && n_col <= 16) return {32, 32, k_attn_fwd_few<T, DP, 1, 8>, 512, true, 8};
+        return {32, 32, n_col <= 16 ? k_attn_fwd_few<T, DP, 1, 4> : k_attn_fwd_few<T, DP, 2, 4>, 256, true, wpp};
     }
     if constexpr (wide)
         if (n_col > 64 && n_bh * ((n_col + 127) / 128) >= 256) return tiles<T, DP, 2, KT>(pass);

@@ -96,30 +96,81 @@ struct Tile {
     }
 };
 
-// the forward's epilogue: accumulators of output features r0 + 16 r + 4 g + 0..3 of the rows c0 + 16 c + i16
-template <typename T, int MR, int MC>
-__device__ __forceinline__ void store_forward(const LinearP& p, const f32x4 (&acc)[MC][MR], int r0, int64_t c0, int i16, int g) {
+// ---- epilogue.  A wave's accumulators pass through a region of LDS of its own, 16 columns at a time (chunk c of column r at place c ^ (r % 8):
+// no bank conflicts); lanes then hold 16 bytes of consecutive r, and rows of the output leave in whole lines (straight from the accumulators a lane
+// would store 8 bytes of every row).
+template <typename T>
+constexpr int VEC = 16 / sizeof(T);
+template <typename T>
+struct Row16 {  // 16 bytes of a row in fp32
+    float v[VEC<T>];
+};
+template <typename T>
+__device__ __forceinline__ void add_row(Row16<T>& a, const T* p, int n) {
+    typedef T vec __attribute__((ext_vector_type(VEC<T>)));
+    vec x;
+    if (n >= VEC<T>) {
+        __builtin_memcpy(&x, p, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC<T>; ++j) x[j] = p[j < n ? j : 0];
+    }
+#pragma unroll
+    for (int j = 0; j < VEC<T>; ++j) a.v[j] += (float)x[j];
+}
+template <typename T>
+__device__ __forceinline__ void put_row(const Row16<T>& a, T* p, int n) {
+    typedef T vec __attribute__((ext_vector_type(VEC<T>)));
+    vec x;
+#pragma unroll
+    for (int j = 0; j < VEC<T>; ++j) x[j] = (T)a.v[j];
+    if (n >= VEC<T>) {
+        __builtin_memcpy(p, &x, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC<T>; ++j)
+            if (j < n) p[j] = x[j];
+    }
+}
+// bias, activation, row mask and residual for features n0 .. (the first n >= 1 of them inside) of row m
+template <typename T>
+__device__ __forceinline__ void finish_row(const LinearP& p, int64_t m, int n0, int n, Row16<T>& a) {
+    const int64_t at = m * p.N + n0;
+    const bool valid = !p.row_valid || p.row_valid[m];
+    if (p.bias) add_row<T>(a, (const T*)p.bias + n0, n);
+    if (p.relu)
+#pragma unroll
+        for (int j = 0; j < VEC<T>; ++j) a.v[j] = a.v[j] < 0.f ? 0.f : a.v[j];  // (a NaN stays)
+#pragma unroll
+    for (int j = 0; j < VEC<T>; ++j) a.v[j] = valid ? a.v[j] : 0.f;
+    if (p.act_out) put_row<T>(a, (T*)p.act_out + at, n);
+    if (p.residual) add_row<T>(a, (const T*)p.residual + at, n);
+    put_row<T>(a, (T*)p.y + at, n);
+}
+// rows r0 .. of columns c0 ..: `give(column, r, n, values)` for every 16 bytes of T (the first n of them inside the R rows)
+template <typename T, int MR, int MC, typename F>
+__device__ __forceinline__ void through_lds(const f32x4 (&acc)[MC][MR], float* ep, int lane, int64_t c0, int64_t C, int r0, int R, F&& give) {
+    constexpr int Q = VEC<T> / 4;  // 4-float chunks per 16 bytes of T
+    const int i16 = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int c = 0; c < MC; ++c) {
-        const int64_t col = c0 + c * 16 + i16;
-        if (col >= p.M) continue;
-        const bool valid = !p.row_valid || p.row_valid[col];
+        wave_fence();
 #pragma unroll
-        for (int r = 0; r < MR; ++r) {
-            const int row = r0 + r * 16 + 4 * g, n = p.N - row;
-            if (n <= 0) continue;
-            f32x4 v = acc[c][r];
-            const int64_t at = col * p.N + row;
-            if (p.bias) v += load4((const T*)p.bias + row, n);
-            if (p.relu)
+        for (int r = 0; r < MR; ++r) *reinterpret_cast<f32x4*>(ep + i16 * MR * 16 + ((r * 4 + g) ^ (i16 & 7)) * 4) = acc[c][r];
+        wave_fence();
+#pragma unroll 1  // (registers)
+        for (int q = lane; q < 16 * MR * 4 / Q; q += 64) {
+            const int row = q / (MR * 4 / Q), ch = q % (MR * 4 / Q) * Q, r = r0 + ch * 4, n = R - r;
+            const int64_t col = c0 + c * 16 + row;
+            Row16<T> a;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];  // (a NaN stays)
-            if (!valid) v = (f32x4){0.f, 0.f, 0.f, 0.f};
-            if (p.act_out) store4((T*)p.act_out + at, n, v);
-            if (p.residual) v += load4((const T*)p.residual + at, n);
-            store4((T*)p.y + at, n, v);
+            for (int x = 0; x < Q; ++x) {
+                const f32x4 v = *reinterpret_cast<const f32x4*>(ep + row * MR * 16 + ((ch + x) ^ (row & 7)) * 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a.v[x * 4 + e] = v[e];
+            }
+            if (col < C && n > 0) give(col, r, n, a);
         }
-        __builtin_amdgcn_sched_barrier(0);  // (a column's loads together, not the whole tile's: registers)
     }
 }
 
@@ -153,7 +204,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear(const LinearP p) {
     Tile<T, AR, AC, NT, false, NARROW> ta;
     Tile<T, BR, BC, NT, GATED, NARROW> tb;
     int64_t k0 = (int64_t)split * p.split_len;
-    const int64_t kend = KIND == DW ? (k0 + p.split_len < Kn ? k0 + p.split_len : Kn) : Kn;
+    const int64_t kend = k0 + p.split_len < Kn ? k0 + p.split_len : Kn;
     const bool ragged_a = lda % 8 != 0, ragged_b = ldb % 8 != 0;
     auto load = [&](int64_t k) {
         if constexpr (AT)
@@ -203,29 +254,19 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear(const LinearP p) {
             }
         }
     }
-    if constexpr (KIND == FWD) {
-        store_forward<T, MR, MC>(p, acc, r0 + wr, c0 + wc, i16, g);
-        return;
-    }
-#pragma unroll
-    for (int c = 0; c < MC; ++c) {
-        const int64_t col = c0 + wc + c * 16 + i16;
-        if (col >= Cn) continue;
-#pragma unroll
-        for (int r = 0; r < MR; ++r) {
-            const int row = r0 + wr + r * 16 + 4 * g, n = R - row;
-            if (n <= 0) continue;
-            f32x4 v = acc[c][r];
-            const int64_t at = col * R + row;
-            if constexpr (KIND == DX) {
-                store4((T*)p.dx + at, n, v);
-            } else {
-                if (p.n_split > 1)
-                    store4(p.part + split * ((int64_t)p.N * p.K + p.N) + at, n, v);
-                else if (p.dw)
-                    store4((T*)p.dw + at, n, v);
-            }
-        }
+    static_assert(WR * WC * 16 * MR * 16 * 4 <= (int)sizeof(la), "the regions fit the A tile");
+    float* ep = reinterpret_cast<float*>(la) + wave * 16 * MR * 16;
+    __syncthreads();
+    if (p.n_split > 1) {  // this split's part
+        float* part = p.part + split * (KIND == DW ? (int64_t)p.N * p.K + p.N : Cn * R);
+        through_lds<float, MR, MC>(acc, ep, lane, c0 + wc, Cn, r0 + wr, R, [&](int64_t c, int r, int n, Row16<float>& a) { put_row<float>(a, part + c * R + r, n); });
+    } else {
+        through_lds<T, MR, MC>(acc, ep, lane, c0 + wc, Cn, r0 + wr, R, [&](int64_t c, int r, int n, Row16<T>& a) {
+            if constexpr (KIND == FWD)
+                finish_row<T>(p, c, r, n, a);
+            else if (KIND == DX || p.dw)
+                put_row<T>(a, (KIND == DX ? (T*)p.dx : (T*)p.dw) + c * R + r, n);
+        });
     }
     if constexpr (KIND == DW) {
         if (rt == 0 && p.db) {  // (workgroup-uniform) the threads of one chunk of columns add up, in thread order
@@ -247,42 +288,6 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear(const LinearP p) {
                 }
         }
     }
-}
-
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ f32x8 load8(const bf16* p, int n) {
-    bf16x8 v;
-    if (n >= 8) {
-        __builtin_memcpy(&v, p, 16);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = p[j < n ? j : 0];
-    }
-    return __builtin_convertvector(v, f32x8);
-}
-__device__ __forceinline__ void store8(bf16* p, int n, f32x8 v) {
-    const bf16x8 h = __builtin_convertvector(v, bf16x8);
-    if (n >= 8) {
-        __builtin_memcpy(p, &h, 16);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < n) p[j] = h[j];
-    }
-}
-// the forward's epilogue for features n0 .. n0 + 7 (the first n >= 1 of them inside) of row m, bf16
-__device__ __forceinline__ void store_row8(const LinearP& p, int64_t m, int n0, int n, f32x8 v) {
-    const int64_t at = m * p.N + n0;
-    const bool valid = !p.row_valid || p.row_valid[m];
-    if (p.bias) v += load8((const bf16*)p.bias + n0, n);
-    if (p.relu)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];  // (a NaN stays)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = valid ? v[j] : 0.f;
-    if (p.act_out) store8((bf16*)p.act_out + at, n, v);
-    if (p.residual) v += load8((const bf16*)p.residual + at, n);
-    store8((bf16*)p.y + at, n, v);
 }
 
 // 16 bytes per lane from global memory into LDS, lane l at dst + 16 l bytes
@@ -374,26 +379,10 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear_direct(const LinearP p)
         if (k + 2 * KB < p.K) issue(l0, k + 2 * KB);
         multiply(l1);
     }
-    // Epilogue through LDS, 16 rows of y at a time in a region of the wave's own: lanes then hold 8 consecutive features, and rows leave in
-    // whole lines (straight from the accumulators a lane would store 8 bytes of every row).  Chunk c of row r lies at c ^ (r % 8), as above.
     static_assert(NW * 16 * MR * 16 * 4 <= (int)sizeof(l0), "the regions fit one buffer");
-    float* ep = reinterpret_cast<float*>(l0) + wave * 16 * MR * 16;
     __syncthreads();
-#pragma unroll
-    for (int c = 0; c < MC; ++c) {
-        wave_fence();
-#pragma unroll
-        for (int r = 0; r < MR; ++r) *reinterpret_cast<f32x4*>(ep + i16 * MR * 16 + ((r * 4 + g) ^ (i16 & 7)) * 4) = acc[c][r];
-        wave_fence();
-#pragma unroll 1  // (registers)
-        for (int q = lane; q < 16 * MR * 2; q += 64) {
-            const int row = q / (MR * 2), ch = (q % (MR * 2)) * 2, n0 = r0 + wr + ch * 4, n = p.N - n0;
-            const int64_t m = c0 + wc + c * 16 + row;
-            const f32x4 lo = *reinterpret_cast<const f32x4*>(ep + row * MR * 16 + (ch ^ (row & 7)) * 4);
-            const f32x4 hi = *reinterpret_cast<const f32x4*>(ep + row * MR * 16 + ((ch + 1) ^ (row & 7)) * 4);
-            if (m < p.M && n > 0) store_row8(p, m, n0, n, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-        }
-    }
+    through_lds<bf16, MR, MC>(acc, reinterpret_cast<float*>(l0) + wave * 16 * MR * 16, lane, c0 + wc, p.M, r0 + wr, p.N,
+                              [&](int64_t m, int n0, int n, Row16<bf16>& a) { finish_row<bf16>(p, m, n0, n, a); });
 }
 
 // Both gradient products of a layer of at most 128 x 128 over many rows, in one walk: dy (and what gates it) and x are read once, where the
@@ -530,6 +519,24 @@ __global__ __launch_bounds__(256) void k_linear_sum(const float* part, int n_spl
     }
 }
 
+// the forward's epilogue on the sum of the splits (in split order)
+template <typename T>
+__global__ __launch_bounds__(256) void k_linear_finish(const LinearP p) {
+    const int chunks = (p.N + VEC<T> - 1) / VEC<T>;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, m = id / chunks;
+    if (m >= p.M) return;
+    const int n0 = (int)(id % chunks) * VEC<T>, n = p.N - n0;
+    Row16<T> a;
+#pragma unroll
+    for (int j = 0; j < VEC<T>; ++j) a.v[j] = 0.f;
+    for (int s = 0; s < p.n_split; ++s) {
+        const float* src = p.part + (s * p.M + m) * p.N + n0;
+#pragma unroll
+        for (int j = 0; j < VEC<T>; ++j) a.v[j] += src[j < n ? j : 0];
+    }
+    finish_row<T>(p, m, n0, n, a);
+}
+
 struct Shape {
     void (*kernel)(LinearP);
     int tr, tc, kb, threads;
@@ -578,17 +585,19 @@ Plan plan(const LinearP& p) {
         r.s = p.dtype == 1 ? choose<bf16, KIND>(p, R, C) : choose<float, KIND>(p, R, C);
     r.p.n_rt = (int)((R + r.s.tr - 1) / r.s.tr);
     r.p.n_ct = (C + r.s.tc - 1) / r.s.tc;
-    r.p.n_split = 1;
-    r.p.split_len = 0;
-    if (KIND == DW) {  // about two workgroups per CU; a part keeps at least four tiles of the contraction
-        const int64_t tiles = (p.M + r.s.kb - 1) / r.s.kb, base = (int64_t)r.p.n_rt * r.p.n_ct;
-        int64_t n = 512 / (base > 0 ? base : 1);
-        if (n > tiles / 4) n = tiles / 4;
-        if (n < 1) n = 1;
-        r.p.split_len = (tiles + n - 1) / n * r.s.kb;
-        r.p.n_split = r.p.split_len > 0 ? (int)((p.M + r.p.split_len - 1) / r.p.split_len) : 1;
-        if (r.p.n_split < 1) r.p.n_split = 1;
-    }
+    // Splits of the contraction.  dW: about two workgroups per CU, a part keeps at least four steps.  The others only where the tiles leave CUs
+    // idle and the contraction is long: the join is a launch of its own (14 x 818 x 56 fp32, dx: 26 steps on one CU).
+    const int64_t K = KIND == FWD ? p.K : KIND == DX ? p.N : p.M, steps = (K + r.s.kb - 1) / r.s.kb, base = (int64_t)r.p.n_rt * r.p.n_ct;
+    int64_t n = 1;
+    if (KIND == DW)
+        n = 512 / (base > 0 ? base : 1);
+    else if (steps >= 16 && base > 0 && base <= 128)  // (the direct kernels start at 256 tiles)
+        n = 256 / base < 16 ? 256 / base : 16;
+    if (n > steps / 4) n = steps / 4;
+    if (n < 1) n = 1;
+    r.p.split_len = (steps + n - 1) / n * r.s.kb;
+    r.p.n_split = r.p.split_len > 0 ? (int)((K + r.p.split_len - 1) / r.p.split_len) : 1;
+    if (r.p.n_split < 1) r.p.n_split = 1;
     r.blocks = ((int64_t)r.p.n_rt * r.p.n_ct * r.p.n_split + 7) / 8 * 8;
     return r;
 }
@@ -601,9 +610,8 @@ const char* launch(const Plan& r, hipStream_t s) {
 }
 
 template <typename T>
-void launch_sum(const LinearP& p, int n_split, hipStream_t s) {
-    const int64_t n = (int64_t)p.N * p.K;
-    k_linear_sum<T><<<dim3((unsigned)((n + p.N + 63) / 64)), dim3(256), 0, s>>>(p.part, n_split, n, p.N, (T*)p.dw, (T*)p.db);
+void launch_sum(const float* part, int n_split, int64_t n_w, int n_b, void* dw, void* db, hipStream_t s) {
+    k_linear_sum<T><<<dim3((unsigned)((n_w + n_b + 63) / 64)), dim3(256), 0, s>>>(part, n_split, n_w, n_b, (T*)dw, (T*)db);
 }
 
 }  // namespace
@@ -612,13 +620,28 @@ void launch_sum(const LinearP& p, int n_split, hipStream_t s) {
 bool rows_backward(const LinearP& p) { return p.N >= 8 && p.K >= 8 && p.N <= 128 && p.K <= 128 && p.M >= 16384; }
 constexpr int ROWS_BLOCKS = 256;  // one per CU: its LDS holds the weight
 
-int64_t linear_workspace(const LinearP& p) {  // (whichever gradients are wanted)
-    const int64_t one = (int64_t)p.N * p.K + p.N;
-    const int n = plan<DW>(p).p.n_split, rows = rows_backward(p) ? ROWS_BLOCKS : 0;
-    return 4 * one * (n > 1 && n > rows ? n : rows);
+int64_t linear_workspace(const LinearP& p, bool backward) {  // (whichever gradients are wanted)
+    auto parts = [](int n, int64_t one) { return n > 1 ? 4 * n * one : (int64_t)0; };
+    if (!backward) return parts(plan<FWD>(p).p.n_split, p.M * p.N);
+    const int64_t one = (int64_t)p.N * p.K + p.N, dx = parts(plan<DX>(p).p.n_split, p.M * p.K), dw = parts(plan<DW>(p).p.n_split, one);
+    const int64_t rows = rows_backward(p) ? 4 * ROWS_BLOCKS * one : 0, m = dx > dw ? dx : dw;
+    return m > rows ? m : rows;
 }
 
-const char* run_linear(const LinearP& p, hipStream_t s) { return launch(plan<FWD>(p), s); }
+const char* run_linear(LinearP p, float* ws, hipStream_t s) {
+    p.part = ws;
+    const Plan r = plan<FWD>(p);
+    if (const char* e = launch(r, s)) return e;
+    if (r.p.n_split > 1) {
+        const int vec = p.dtype == 1 ? VEC<bf16> : VEC<float>;
+        const dim3 grid((unsigned)((p.M * ((p.N + vec - 1) / vec) + 255) / 256));
+        if (p.dtype == 1)
+            k_linear_finish<bf16><<<grid, dim3(256), 0, s>>>(r.p);
+        else
+            k_linear_finish<float><<<grid, dim3(256), 0, s>>>(r.p);
+    }
+    return nullptr;
+}
 
 const char* run_linear_backward(LinearP p, float* ws, hipStream_t s) {
     if (rows_backward(p) && p.dx && p.dw) {
@@ -627,22 +650,30 @@ const char* run_linear_backward(LinearP p, float* ws, hipStream_t s) {
                                                : (p.act ? k_linear_bwd_rows<float, true> : k_linear_bwd_rows<float, false>);
         kernel<<<dim3(ROWS_BLOCKS), dim3(512), 0, s>>>(p);
         if (p.dtype == 1)
-            launch_sum<bf16>(p, ROWS_BLOCKS, s);
+            launch_sum<bf16>(ws, ROWS_BLOCKS, (int64_t)p.N * p.K, p.N, p.dw, p.db, s);
         else
-            launch_sum<float>(p, ROWS_BLOCKS, s);
+            launch_sum<float>(ws, ROWS_BLOCKS, (int64_t)p.N * p.K, p.N, p.dw, p.db, s);
         return nullptr;
     }
-    if (p.dx)
-        if (const char* e = launch(plan<DX>(p), s)) return e;
+    p.part = ws;  // (one product after the other)
+    if (p.dx) {
+        const Plan r = plan<DX>(p);
+        if (const char* e = launch(r, s)) return e;
+        if (r.p.n_split > 1) {
+            if (p.dtype == 1)
+                launch_sum<bf16>(ws, r.p.n_split, p.M * p.K, 0, p.dx, nullptr, s);
+            else
+                launch_sum<float>(ws, r.p.n_split, p.M * p.K, 0, p.dx, nullptr, s);
+        }
+    }
     if (!p.dw && !p.db) return nullptr;
-    p.part = ws;
     const Plan r = plan<DW>(p);
     if (const char* e = launch(r, s)) return e;
     if (r.p.n_split > 1) {
         if (p.dtype == 1)
-            launch_sum<bf16>(p, r.p.n_split, s);
+            launch_sum<bf16>(ws, r.p.n_split, (int64_t)p.N * p.K, p.N, p.dw, p.db, s);
         else
-            launch_sum<float>(p, r.p.n_split, s);
+            launch_sum<float>(ws, r.p.n_split, (int64_t)p.N * p.K, p.N, p.dw, p.db, s);
     }
     return nullptr;
 }

@@ -130,7 +130,7 @@ extern "C" int64_t tb_layer_norm_workspace_bytes(const tb_layer_norm_io* io, int
     return !io || sizes(*io) ? -1 : backward ? tb::op::norm_workspace(params(*io)) : 0;
 }
 extern "C" int64_t tb_linear_workspace_bytes(const tb_linear_io* io, int32_t backward) {
-    return !io || sizes(*io) ? -1 : backward ? tb::op::linear_workspace(params(*io)) : 0;
+    return !io || sizes(*io) ? -1 : tb::op::linear_workspace(params(*io), backward != 0);
 }
 
 extern "C" int tb_attention(tb_ctx* ctx, const tb_attention_io* io, tb_stream stream) {
@@ -182,7 +182,8 @@ extern "C" int tb_linear(tb_ctx* ctx, const tb_linear_io* io, tb_stream stream) 
         if (!io->weight || (io->n_row && (!io->x || !io->y))) return "a required buffer pointer is NULL";
         LinearP p = params(*io);
         p.act_out = io->act;
-        return tb::op::run_linear(p, (hipStream_t)stream);
+        if (const char* e = scratch(*io, tb::op::linear_workspace(p, false))) return e;
+        return tb::op::run_linear(p, (float*)io->workspace, (hipStream_t)stream);
     });
 }
 extern "C" int tb_linear_backward(tb_ctx* ctx, const tb_linear_io* io, tb_stream stream) {
@@ -193,8 +194,7 @@ extern "C" int tb_linear_backward(tb_ctx* ctx, const tb_linear_io* io, tb_stream
         if (io->activation == 1 && io->n_row && !io->act) return "ReLU's gradient needs act (what tb_linear wrote there)";
         LinearP p = params(*io);
         p.act = io->activation == 1 ? io->act : nullptr;
-        if (io->dweight || io->dbias)
-            if (const char* e = scratch(*io, tb::op::linear_workspace(p))) return e;
+        if (const char* e = scratch(*io, tb::op::linear_workspace(p, true))) return e;
         return tb::op::run_linear_backward(p, (float*)io->workspace, (hipStream_t)stream);
     });
 }

@@ -51,10 +51,10 @@ struct LinearP {
     // of one launch
     int n_rt, n_split;
     int64_t n_ct, split_len;
-    float* part;  // [n_split][N K + N]: dW, db
+    float* part;  // [n_split][M N] (forward), [n_split][M K] (dx) or [n_split][N K + N] (dW, db)
 };
-int64_t linear_workspace(const LinearP& p);
-const char* run_linear(const LinearP& p, hipStream_t s);
+int64_t linear_workspace(const LinearP& p, bool backward);
+const char* run_linear(LinearP p, float* ws, hipStream_t s);
 const char* run_linear_backward(LinearP p, float* ws, hipStream_t s);
 
 }  // namespace op

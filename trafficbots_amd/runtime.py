@@ -1040,7 +1040,7 @@ class HipEngine:
         io = hip.TbLinearIO()
         hip.PACK_LINEAR.pack_into(io, 0, dtype, weight.shape[1], weight.shape[0], 1 if activation else 0, n_row, x.data_ptr(), weight.data_ptr(), _ptr(bias),
                                   _ptr(rv), _ptr(residual), y.data_ptr(), _ptr(act), 0, 0, 0, 0, 0, 0)
-        self._run("tb_linear", io, self.lib.tb_linear)
+        self._run("tb_linear", io, self.lib.tb_linear, self.lib.tb_linear_workspace_bytes(C.byref(io), 0))
         return (y, y if act is None else act) if want_act else y
 
     def linear_backward(self, d_out: Tensor, x: Tensor, weight: Tensor, act: Optional[Tensor] = None, row_valid: Optional[Tensor] = None,
@@ -1059,8 +1059,7 @@ class HipEngine:
         io = hip.TbLinearIO()
         hip.PACK_LINEAR.pack_into(io, 0, dtype, weight.shape[1], weight.shape[0], 0 if act is None else 1, n_row, x.data_ptr(), weight.data_ptr(), 0, _ptr(rv), 0, 0,
                                   _ptr(act), d_out.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), 0, 0)
-        need = self.lib.tb_linear_workspace_bytes(C.byref(io), 1) if want_dweight or want_dbias else 0
-        self._run("tb_linear_backward", io, self.lib.tb_linear_backward, need)
+        self._run("tb_linear_backward", io, self.lib.tb_linear_backward, self.lib.tb_linear_workspace_bytes(C.byref(io), 1))
         return dx, dw, db
 
     def _linear_args(self, what: str, x: Tensor, weight: Tensor, row_valid: Optional[Tensor], *more: Optional[Tensor]):
