@@ -105,18 +105,34 @@ template <typename T>
 struct Row16 {  // 16 bytes of a row in fp32
     float v[VEC<T>];
 };
+// 16 bytes of a row as they lie in memory, loaded ahead: from the last place inside the row where they would end behind it (`lead` elements early)
+template <typename T>
+struct Ahead {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 u;
+    __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(&u, p, 16); }
+    __device__ __forceinline__ void fit(int lead) {
+        const int words = lead * (int)sizeof(T) / 4;
+#pragma unroll
+        for (int s = 2; s; s >>= 1)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[j] = words & s ? (j + s < 4 ? u[j + s] : 0u) : u[j];
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[j] = lead & 1 ? u[j] >> 16 | (j < 3 ? u[j + 1] << 16 : 0u) : u[j];
+        }
+    }
+    __device__ __forceinline__ void add_to(Row16<T>& a) const {
+        typedef T vec __attribute__((ext_vector_type(VEC<T>)));
+        const vec x = __builtin_bit_cast(vec, u);
+#pragma unroll
+        for (int j = 0; j < VEC<T>; ++j) a.v[j] += (float)x[j];
+    }
+};
 template <typename T>
 __device__ __forceinline__ void add_row(Row16<T>& a, const T* p, int n) {
-    typedef T vec __attribute__((ext_vector_type(VEC<T>)));
-    vec x;
-    if (n >= VEC<T>) {
-        __builtin_memcpy(&x, p, 16);
-    } else {
 #pragma unroll
-        for (int j = 0; j < VEC<T>; ++j) x[j] = p[j < n ? j : 0];
-    }
-#pragma unroll
-    for (int j = 0; j < VEC<T>; ++j) a.v[j] += (float)x[j];
+    for (int j = 0; j < VEC<T>; ++j) a.v[j] += j < n ? (float)p[j] : 0.f;
 }
 template <typename T>
 __device__ __forceinline__ void put_row(const Row16<T>& a, T* p, int n) {
@@ -132,44 +148,100 @@ __device__ __forceinline__ void put_row(const Row16<T>& a, T* p, int n) {
             if (j < n) p[j] = x[j];
     }
 }
-// bias, activation, row mask and residual for features n0 .. (the first n >= 1 of them inside) of row m
-template <typename T>
-__device__ __forceinline__ void finish_row(const LinearP& p, int64_t m, int n0, int n, Row16<T>& a) {
-    const int64_t at = m * p.N + n0;
-    const bool valid = !p.row_valid || p.row_valid[m];
-    if (p.bias) add_row<T>(a, (const T*)p.bias + n0, n);
-    if (p.relu)
+// activation and row mask, what the gradient keeps of them, and the output once `res` has been added
+template <typename T, typename F>
+__device__ __forceinline__ void finish_row(const LinearP& p, int64_t at, int n, bool valid, Row16<T>& a, F&& res) {
 #pragma unroll
-        for (int j = 0; j < VEC<T>; ++j) a.v[j] = a.v[j] < 0.f ? 0.f : a.v[j];  // (a NaN stays)
-#pragma unroll
-    for (int j = 0; j < VEC<T>; ++j) a.v[j] = valid ? a.v[j] : 0.f;
+    for (int j = 0; j < VEC<T>; ++j) {
+        if (p.relu) a.v[j] = a.v[j] < 0.f ? 0.f : a.v[j];  // (a NaN stays)
+        a.v[j] = valid ? a.v[j] : 0.f;
+    }
     if (p.act_out) put_row<T>(a, (T*)p.act_out + at, n);
-    if (p.residual) add_row<T>(a, (const T*)p.residual + at, n);
+    if (p.residual) res(a);
     put_row<T>(a, (T*)p.y + at, n);
 }
-// rows r0 .. of columns c0 ..: `give(column, r, n, values)` for every 16 bytes of T (the first n of them inside the R rows)
-template <typename T, int MR, int MC, typename F>
-__device__ __forceinline__ void through_lds(const f32x4 (&acc)[MC][MR], float* ep, int lane, int64_t c0, int64_t C, int r0, int R, F&& give) {
-    constexpr int Q = VEC<T> / 4;  // 4-float chunks per 16 bytes of T
-    const int i16 = lane & 15, g = lane >> 4;
+// 16 columns of accumulators into a wave's region
+template <int MR>
+__device__ __forceinline__ void to_region(const f32x4 (&acc)[MR], float* ep, int i16, int g) {
+    wave_fence();
+#pragma unroll
+    for (int r = 0; r < MR; ++r) *reinterpret_cast<f32x4*>(ep + i16 * MR * 16 + ((r * 4 + g) ^ (i16 & 7)) * 4) = acc[r];
+    wave_fence();
+}
+// ... and the 16 bytes of T from chunk `ch` of column `row` on
+template <typename T, int MR>
+__device__ __forceinline__ void from_region(const float* ep, int row, int ch, Row16<T>& a) {
+#pragma unroll
+    for (int x = 0; x < VEC<T> / 4; ++x) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(ep + row * MR * 16 + ((ch + x) ^ (row & 7)) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a.v[x * 4 + e] = v[e];
+    }
+}
+// rows r0 .. of columns c0 .. of a [C, R] output
+template <typename T, int MR, int MC>
+__device__ __forceinline__ void store_plain(const f32x4 (&acc)[MC][MR], float* ep, int lane, int64_t c0, int64_t C, int r0, int R, T* dst) {
+    constexpr int PER = MR * 16 / VEC<T>;
 #pragma unroll
     for (int c = 0; c < MC; ++c) {
-        wave_fence();
-#pragma unroll
-        for (int r = 0; r < MR; ++r) *reinterpret_cast<f32x4*>(ep + i16 * MR * 16 + ((r * 4 + g) ^ (i16 & 7)) * 4) = acc[c][r];
-        wave_fence();
-#pragma unroll 1  // (registers)
-        for (int q = lane; q < 16 * MR * 4 / Q; q += 64) {
-            const int row = q / (MR * 4 / Q), ch = q % (MR * 4 / Q) * Q, r = r0 + ch * 4, n = R - r;
+        to_region<MR>(acc[c], ep, lane & 15, lane >> 4);
+#pragma unroll 2
+        for (int q = lane; q < 16 * PER; q += 64) {
+            const int row = q / PER, ch = q % PER * (VEC<T> / 4), r = r0 + ch * 4, n = R - r;
             const int64_t col = c0 + c * 16 + row;
             Row16<T> a;
+            from_region<T, MR>(ep, row, ch, a);
+            if (col < C && n > 0) put_row<T>(a, dst + col * R + r, n);
+        }
+    }
+}
+// the forward's: with bias, activation, row mask and residual.  What is read is loaded ahead, a column tile at a time: waiting for the residual
+// of every 16 bytes took as long as the product (27709 x 8 -> 1250, fp32).
+template <typename T, int MR, int MC>
+__device__ __forceinline__ void store_forward(const LinearP& p, const f32x4 (&acc)[MC][MR], float* ep, int lane, int64_t c0, int r0) {
+    constexpr int PER = MR * 16 / VEC<T>, IT = 16 * PER / 64;
+    static_assert(16 * PER % 64 == 0, "whole rounds of the wave");
+    const bool ahead = p.N >= VEC<T>, ragged = p.N % VEC<T> != 0;
+    const Valid rows_valid(p.row_valid, 0);
 #pragma unroll
-            for (int x = 0; x < Q; ++x) {
-                const f32x4 v = *reinterpret_cast<const f32x4*>(ep + row * MR * 16 + ((ch + x) ^ (row & 7)) * 4);
+    for (int c = 0; c < MC; ++c) {
+        Ahead<T> res[IT], bias[IT];
+        uint8_t valid[IT];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) a.v[x * 4 + e] = v[e];
+        for (int i = 0; i < IT; ++i) {
+            const int q = i * 64 + lane, r = r0 + q % PER * VEC<T>, rs = min(r, p.N - VEC<T>);
+            const int64_t m = c0 + c * 16 + q / PER, mc = m < p.M ? m : p.M - 1;
+            valid[i] = rows_valid[mc];
+            if (ahead) {
+                if (p.bias) bias[i].load((const T*)p.bias + rs);
+                if (p.residual) res[i].load((const T*)p.residual + mc * p.N + rs);
             }
-            if (col < C && n > 0) give(col, r, n, a);
+        }
+        to_region<MR>(acc[c], ep, lane & 15, lane >> 4);
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int q = i * 64 + lane, row = q / PER, ch = q % PER * (VEC<T> / 4), r = r0 + ch * 4, n = p.N - r;
+            const int64_t m = c0 + c * 16 + row, at = m * p.N + r;
+            Row16<T> a;
+            from_region<T, MR>(ep, row, ch, a);
+            if (ahead && ragged) {  // (uniform)
+                const int lead = r - min(r, p.N - VEC<T>);
+                bias[i].fit(lead);
+                res[i].fit(lead);
+            }
+            if (m >= p.M || n <= 0) continue;
+            if (p.bias) {
+                if (ahead)
+                    bias[i].add_to(a);
+                else
+                    add_row<T>(a, (const T*)p.bias + r, n);
+            }
+            finish_row<T>(p, at, n, valid[i], a, [&](Row16<T>& b) {
+                if (ahead)
+                    res[i].add_to(b);
+                else
+                    add_row<T>(b, (const T*)p.residual + at, n);
+            });
         }
     }
 }
@@ -259,14 +331,11 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear(const LinearP p) {
     __syncthreads();
     if (p.n_split > 1) {  // this split's part
         float* part = p.part + split * (KIND == DW ? (int64_t)p.N * p.K + p.N : Cn * R);
-        through_lds<float, MR, MC>(acc, ep, lane, c0 + wc, Cn, r0 + wr, R, [&](int64_t c, int r, int n, Row16<float>& a) { put_row<float>(a, part + c * R + r, n); });
-    } else {
-        through_lds<T, MR, MC>(acc, ep, lane, c0 + wc, Cn, r0 + wr, R, [&](int64_t c, int r, int n, Row16<T>& a) {
-            if constexpr (KIND == FWD)
-                finish_row<T>(p, c, r, n, a);
-            else if (KIND == DX || p.dw)
-                put_row<T>(a, (KIND == DX ? (T*)p.dx : (T*)p.dw) + c * R + r, n);
-        });
+        store_plain<float, MR, MC>(acc, ep, lane, c0 + wc, Cn, r0 + wr, R, part);
+    } else if constexpr (KIND == FWD) {
+        store_forward<T, MR, MC>(p, acc, ep, lane, c0 + wc, r0 + wr);
+    } else if (KIND == DX || p.dw) {
+        store_plain<T, MR, MC>(acc, ep, lane, c0 + wc, Cn, r0 + wr, R, KIND == DX ? (T*)p.dx : (T*)p.dw);
     }
     if constexpr (KIND == DW) {
         if (rt == 0 && p.db) {  // (workgroup-uniform) the threads of one chunk of columns add up, in thread order
@@ -381,8 +450,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear_direct(const LinearP p)
     }
     static_assert(NW * 16 * MR * 16 * 4 <= (int)sizeof(l0), "the regions fit one buffer");
     __syncthreads();
-    through_lds<bf16, MR, MC>(acc, reinterpret_cast<float*>(l0) + wave * 16 * MR * 16, lane, c0 + wc, p.M, r0 + wr, p.N,
-                              [&](int64_t m, int n0, int n, Row16<bf16>& a) { finish_row<bf16>(p, m, n0, n, a); });
+    store_forward<bf16, MR, MC>(p, acc, reinterpret_cast<float*>(l0) + wave * 16 * MR * 16, lane, c0 + wc, r0 + wr);
 }
 
 // Both gradient products of a layer of at most 128 x 128 over many rows, in one walk: dy (and what gates it) and x are read once, where the
@@ -534,7 +602,9 @@ __global__ __launch_bounds__(256) void k_linear_finish(const LinearP p) {
 #pragma unroll
         for (int j = 0; j < VEC<T>; ++j) a.v[j] += src[j < n ? j : 0];
     }
-    finish_row<T>(p, m, n0, n, a);
+    const int64_t at = m * p.N + n0;
+    if (p.bias) add_row<T>(a, (const T*)p.bias + n0, n);
+    finish_row<T>(p, at, n, !p.row_valid || p.row_valid[m], a, [&](Row16<T>& b) { add_row<T>(b, (const T*)p.residual + at, n); });
 }
 
 struct Shape {
