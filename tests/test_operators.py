@@ -285,6 +285,15 @@ def test_attention_of_few_rows_is_split_and_joined(eng, dtype, b, lq, lk, h, hkv
 
 @gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("mask", [None, "batch", "causal"])
+@pytest.mark.parametrize("b,lq,lk,h,hkv,d", [(5, 1, 100, 8, 1, 128), (2, 3, 70, 20, 2, 44), (1, 5, 300, 6, 1, 32), (70, 1, 66, 64, 2, 32), (3, 7, 130, 8, 2, 64), (1, 2, 2100, 32, 2, 33)])
+def test_attention_of_few_rows_shares_a_walk(eng, dtype, mask, b, lq, lk, h, hkv, d):
+    """The queries of all heads on one key / value head are columns of one walk: 8 to 32 of them."""
+    _check_attention(eng, *_attention_inputs(b, lq, lk, h, hkv, d, dtype, seed=lq + h, pad=True, mask=mask))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_attention_reads_and_broadcasts_views(eng, dtype):
     """One packed projection [B, L, 3, H, D], heads in front of positions, a batch-broadcast key, components that are not adjacent, masks
     that are views: the same bits as from contiguous copies."""

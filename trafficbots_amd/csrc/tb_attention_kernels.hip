@@ -178,16 +178,13 @@ __device__ __forceinline__ void finish(const AttnP& p, const f32x4 (&acc)[DN], f
     const bool on = valid && (sum > 0.f || sum != sum);  // (a NaN row stays NaN)
     const float inv = on ? 1.f / sum : 0.f, lse2 = on ? m * p.scale2 + __builtin_amdgcn_logf(sum) : NEG_INF;
     const int64_t rows = (int64_t)p.B * p.H * p.Lq, row = ((int64_t)b * p.H + h) * p.Lq + q;
+    f32x4 o[DN];
 #pragma unroll
-    for (int d = 0; d < DN; ++d) {
-        const int col = d * 16 + 4 * g;
-        if (col >= p.D) continue;
-        const f32x4 o = on ? acc[d] * inv : (f32x4){0.f, 0.f, 0.f, 0.f};
-        if (p.n_split > 1)
-            store4(p.part + (split * rows + row) * p.D + col, p.D - col, o);
-        else
-            store4((T*)p.out + b * p.os[0] + q * p.os[1] + h * p.os[2] + col, p.D - col, o);
-    }
+    for (int d = 0; d < DN; ++d) o[d] = on ? acc[d] * inv : (f32x4){0.f, 0.f, 0.f, 0.f};
+    if (p.n_split > 1)
+        store_row<float, DN>(p.part + (split * rows + row) * p.D, p.D, g, o);
+    else
+        store_row<T, DN>((T*)p.out + b * p.os[0] + q * p.os[1] + h * p.os[2], p.D, g, o);
     if (g == 0) {
         if (p.n_split > 1)
             p.part_lse[split * rows + row] = lse2;
@@ -304,24 +301,26 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnP p) {
     const int cols = (p.D + 3) / 4;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)p.B * p.H * p.Lq, row = id / cols;
     if (row >= rows) return;
-    const int col = (int)(id % cols) * 4, q = (int)(row % p.Lq), h = (int)(row / p.Lq % p.H);
+    const int col = min((int)(id % cols) * 4, p.D - 4), q = (int)(row % p.Lq), h = (int)(row / p.Lq % p.H);  // (the last columns perhaps twice)
     const int64_t b = row / p.Lq / p.H;
     float m = NEG_INF;
+#pragma unroll 8
     for (int s = 0; s < p.n_split; ++s) m = fmaxf(m, p.part_lse[s * rows + row]);
     const float ref = m == NEG_INF ? 0.f : m;
     float sum = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
     for (int s = 0; s < p.n_split; ++s) {
         const float w = __builtin_amdgcn_exp2f(p.part_lse[s * rows + row] - ref);
-        const float* src = p.part + (s * rows + row) * p.D + col;
+        f32x4 x;
+        __builtin_memcpy(&x, p.part + (s * rows + row) * p.D + col, 16);
         sum += w;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (col + e < p.D) o[e] = __builtin_fmaf(w, src[e], o[e]);
+        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(w, x[e], o[e]);
     }
     const bool on = sum > 0.f || sum != sum;
     o = on ? o * (1.f / sum) : (f32x4){0.f, 0.f, 0.f, 0.f};
-    store4((T*)p.out + b * p.os[0] + q * p.os[1] + h * p.os[2] + col, p.D - col, o);
+    store4((T*)p.out + b * p.os[0] + q * p.os[1] + h * p.os[2] + col, 4, o);
     if (col == 0) p.lse[row] = on ? (ref + __builtin_amdgcn_logf(sum)) * LN2 : NEG_INF;
 }
 
@@ -350,32 +349,58 @@ __device__ __forceinline__ void query_columns(const AttnP& p, const Valid& qvali
 // a query's / a key's gradients, or this split's part of them
 template <typename T, int DN>
 __device__ __forceinline__ void store_dq(const AttnP& p, const f32x4 (&acc)[DN], int b, int h, int q, int split, int g) {
+    f32x4 o[DN];
 #pragma unroll
-    for (int d = 0; d < DN; ++d) {
-        const int col = d * 16 + 4 * g;
-        if (col >= p.D) continue;
-        const f32x4 o = acc[d] * p.scale;
-        if (p.n_split > 1)
-            store4(p.part + (((int64_t)split * p.B * p.Lq + (int64_t)b * p.Lq + q) * p.H + h) * p.D + col, p.D - col, o);
-        else
-            store4((T*)p.dq + b * p.dqs[0] + q * p.dqs[1] + h * p.dqs[2] + col, p.D - col, o);
-    }
+    for (int d = 0; d < DN; ++d) o[d] = acc[d] * p.scale;
+    if (p.n_split > 1)
+        store_row<float, DN>(p.part + (((int64_t)split * p.B * p.Lq + (int64_t)b * p.Lq + q) * p.H + h) * p.D, p.D, g, o);
+    else
+        store_row<T, DN>((T*)p.dq + b * p.dqs[0] + q * p.dqs[1] + h * p.dqs[2], p.D, g, o);
 }
 template <typename T, int DN>
 __device__ __forceinline__ void store_dkv(const AttnP& p, const f32x4 (&dk)[DN], const f32x4 (&dv)[DN], bool on, int b, int hk, int key, int split, int g) {
-    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    f32x4 ok[DN], ov[DN];
 #pragma unroll
-    for (int d = 0; d < DN; ++d) {
-        const int col = d * 16 + 4 * g;
-        if (col >= p.D) continue;
-        const f32x4 ok = on ? dk[d] * p.scale : zero, ov = on ? dv[d] : zero;
-        if (p.n_split > 1) {
-            const int64_t at = (((int64_t)split * p.B * p.Lk + (int64_t)b * p.Lk + key) * p.Hkv + hk) * p.D + col;
-            store4(p.part + at, p.D - col, ok);
-            store4(p.part + (int64_t)p.n_split * p.B * p.Lk * p.Hkv * p.D + at, p.D - col, ov);
-        } else {
-            store4((T*)p.dk + b * p.dks[0] + key * p.dks[1] + hk * p.dks[2] + col, p.D - col, ok);
-            store4((T*)p.dv + b * p.dvs[0] + key * p.dvs[1] + hk * p.dvs[2] + col, p.D - col, ov);
+    for (int d = 0; d < DN; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // (a choice between two whole vectors would put both into memory)
+            ok[d][e] = on ? dk[d][e] * p.scale : 0.f;
+            ov[d][e] = on ? dv[d][e] : 0.f;
+        }
+    if (p.n_split > 1) {
+        const int64_t at = (((int64_t)split * p.B * p.Lk + (int64_t)b * p.Lk + key) * p.Hkv + hk) * p.D;
+        store_row<float, DN>(p.part + at, p.D, g, ok);
+        store_row<float, DN>(p.part + (int64_t)p.n_split * p.B * p.Lk * p.Hkv * p.D + at, p.D, g, ov);
+    } else {
+        store_row<T, DN>((T*)p.dk + b * p.dks[0] + key * p.dks[1] + hk * p.dks[2], p.D, g, ok);
+        store_row<T, DN>((T*)p.dv + b * p.dvs[0] + key * p.dvs[1] + hk * p.dvs[2], p.D, g, ov);
+    }
+}
+
+// 32 rows in the wave's LDS region read down their rows (A) times an operand of two column tiles (B): the gradients of `count` columns, given to
+// memory as soon as they are there (fp32; all at the end: 132 -> 150 us, 8192 x 4 heads of 20 x 20), in bf16 a pair of tiles at a time
+template <typename T, int DP, typename Row, typename Last>
+__device__ __forceinline__ void product(const bf16* lds, int lane, const Frag<Planes<T>::N> (&cols)[2], Row row, int count, int D, Last last) {
+    constexpr int NP = Planes<T>::N, DN = DP / 16, LD = DP + LDS_PAD;
+    const int i16 = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int d = 0; d < DN; d += 2) {
+        f32x4 o[2][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            Frag<NP> a;
+            frag_cols<NP, LD>(lds, (size_t)32 * LD, 4 * g, 16 + 4 * g, (d + u) * 16, lane, a);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                o[n][u] = last(n, mma<NP>(a, cols[n], (f32x4){0.f, 0.f, 0.f, 0.f}));
+                if constexpr (sizeof(T) == 4)
+                    if (n * 16 + i16 < count && (d + u) * 16 + 4 * g < D) store4(row(n, d + u) + 4 * g, D - (d + u) * 16 - 4 * g, o[n][u]);
+            }
+        }
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+                if (n * 16 + i16 < count) store_row<T, 2>(row(n, d), D - d * 16, g, o[n]);
         }
     }
 }
@@ -467,6 +492,18 @@ __device__ __forceinline__ void row_bias(const Rows32& ok, int lane, f32x4 (&bia
     }
 }
 
+// Column c of a problem of `pack` heads: with G heads on one key / value head and G Lq <= 32, the queries of all of them are columns of one walk,
+// so each key is read and put into operands once and not G times.
+struct Column {
+    int h, q;  // head behind the problem's first, query (clamped)
+    bool in;
+};
+__device__ __forceinline__ Column column(const AttnP& p, int c) {
+    const bool in = c < p.pack * p.Lq;
+    const int h = p.pack > 1 && in ? (int)((unsigned)c / (unsigned)p.Lq) : 0;
+    return {h, min(c - h * p.Lq, p.Lq - 1), in};
+}
+
 template <typename T, int DP, int NQ, int NW>
 __global__ __launch_bounds__(64 * NW) void k_attn_fwd_few(const AttnP p) {
     constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, LD = DP + LDS_PAD;
@@ -477,8 +514,9 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd_few(const AttnP p) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, g = lane >> 4;
     const int part = p.wpp > 1 ? wave : 0;
     int bh, split, tile;
-    if (!decode_few(p, p.B * p.H, NW, wave, bh, split, tile)) return;
-    const int b = bh / p.H, h = bh % p.H, hk = h / p.G, off = p.Lk - p.Lq;
+    const int per_b = p.H / p.pack;
+    if (!decode_few(p, p.B * per_b, NW, wave, bh, split, tile)) return;
+    const int b = bh / per_b, h = bh % per_b * p.pack, hk = h / p.G, off = p.Lk - p.Lq;
     const T* kp = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
     const T* vp = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
     const Valid kvalid(p.key_valid, (int64_t)b * p.Lk);
@@ -488,11 +526,12 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd_few(const AttnP p) {
     Frag<NP> qf[NQ][KC];
     f32x4 acc[NQ][DN];
     float m[NQ], l[NQ];
+    Column c[NQ];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-        const int q = n * 16 + i16, qc = min(q, p.Lq - 1);
-        const bool on = qvalid[qc] && q < p.Lq;
-        load_columns<T, KC>(p, (const T*)p.q + b * p.qs[0] + (int64_t)qc * p.qs[1] + h * p.qs[2], on, lane, qf[n]);
+        c[n] = column(p, n * 16 + i16);
+        const bool on = qvalid[c[n].q] && c[n].in;
+        load_columns<T, KC>(p, (const T*)p.q + b * p.qs[0] + (int64_t)c[n].q * p.qs[1] + (h + c[n].h) * p.qs[2], on, lane, qf[n]);
         m[n] = NEG_INF;
         l[n] = 0.f;
 #pragma unroll
@@ -533,10 +572,10 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd_few(const AttnP p) {
                 s[t] = bias[t];
 #pragma unroll
                 for (int kc = 0; kc < KC; ++kc) s[t] = mma<NP>(kf[t][kc], qf[n][kc], s[t]);
-                if (p.causal) hide_later(s[t], j0 + t * 16 + 4 * g, n * 16 + i16 + off);
+                if (p.causal) hide_later(s[t], j0 + t * 16 + 4 * g, c[n].q + off);
             }
             if (p.mask) {
-                const uint8_t* mask = p.mask + b * p.mask_s[0] + (int64_t)min(n * 16 + i16, p.Lq - 1) * p.mask_s[1];
+                const uint8_t* mask = p.mask + b * p.mask_s[0] + (int64_t)c[n].q * p.mask_s[1];
 #pragma unroll
                 for (int t = 0; t < 2; ++t) hide_masked(s[t], mask, j0 + t * 16 + 4 * g, jend);
             }
@@ -581,10 +620,8 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd_few(const AttnP p) {
         if (wave) return;
     }
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        const int q = n * 16 + i16;
-        if (q < p.Lq) finish<T, DN>(p, acc[n], m[n], l[n], b, h, q, split, g);
-    }
+    for (int n = 0; n < NQ; ++n)
+        if (c[n].in) finish<T, DN>(p, acc[n], m[n], l[n], b, h + c[n].h, c[n].q, split, g);
 }
 
 // dq of at most 16 NQ queries per tile: as above, K down its rows from the wave's LDS region
@@ -595,9 +632,10 @@ __global__ __launch_bounds__(256) void k_attn_dq_few(const AttnP p) {
     static_assert(NW / 2 * 16 * DP * 4 <= (int)sizeof(region), "the join fits");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, g = lane >> 4;
     int bh, split, tile;
-    if (!decode_few(p, p.B * p.H, NW, wave, bh, split, tile)) return;
+    const int per_b = p.H / p.pack;
+    if (!decode_few(p, p.B * per_b, NW, wave, bh, split, tile)) return;
     const int part = p.wpp > 1 ? wave : 0;
-    const int b = bh / p.H, h = bh % p.H, hk = h / p.G, off = p.Lk - p.Lq, qb = tile * 16 * NQ;
+    const int b = bh / per_b, h = bh % per_b * p.pack, hk = h / p.G, off = p.Lk - p.Lq, cb = tile * 16 * NQ;
     const T* kp = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
     const T* vp = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
     const Valid kvalid(p.key_valid, (int64_t)b * p.Lk), qvalid(p.query_valid, (int64_t)b * p.Lq);
@@ -605,7 +643,7 @@ __global__ __launch_bounds__(256) void k_attn_dq_few(const AttnP p) {
 
     const int first = split * p.split_len, step = 32 * p.wpp;
     int jend = min(p.Lk, first + p.split_len), j0 = first + part * 32;
-    if (p.causal) jend = min(jend, min(p.Lq, qb + 16 * NQ) + off);
+    if (p.causal) jend = min(jend, (p.pack > 1 ? p.Lq : min(p.Lq, cb + 16 * NQ)) + off);
     Held<T> rk[2][KC], rv[2][KC];
     Rows32 ok;
     if (j0 < jend) {
@@ -615,11 +653,12 @@ __global__ __launch_bounds__(256) void k_attn_dq_few(const AttnP p) {
     Frag<NP> qf[NQ][KC], gf[NQ][KC];
     f32x4 acc[NQ][DN];
     float nlse[NQ], delta[NQ];
+    Column c[NQ];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-        query_columns<T, KC>(p, qvalid, b, h, qb + n * 16 + i16, lane, qf[n], gf[n], nlse[n], delta[n]);
-        const int q = qb + n * 16 + i16;
-        if (q < p.Lq && g == 0 && split == 0 && part == 0) p.delta[((int64_t)b * p.H + h) * p.Lq + q] = delta[n];
+        c[n] = column(p, cb + n * 16 + i16);
+        query_columns<T, KC>(p, qvalid, b, h + c[n].h, c[n].in ? c[n].q : p.Lq, lane, qf[n], gf[n], nlse[n], delta[n]);
+        if (c[n].in && g == 0 && split == 0 && part == 0) p.delta[((int64_t)b * p.H + h + c[n].h) * p.Lq + c[n].q] = delta[n];
 #pragma unroll
         for (int d = 0; d < DN; ++d) acc[n][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
@@ -642,7 +681,6 @@ __global__ __launch_bounds__(256) void k_attn_dq_few(const AttnP p) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             f32x4 ds[2];
-            const int q = qb + n * 16 + i16;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 f32x4 s = bias[t], dp = {-delta[n], -delta[n], -delta[n], -delta[n]};
@@ -654,8 +692,8 @@ __global__ __launch_bounds__(256) void k_attn_dq_few(const AttnP p) {
                 const int j = j0 + t * 16 + 4 * g;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[e] = __builtin_fmaf(s[e], p.scale2, nlse[n]);
-                if (p.causal) hide_later(s, j, q + off);
-                if (p.mask) hide_masked(s, p.mask + b * p.mask_s[0] + (int64_t)min(q, p.Lq - 1) * p.mask_s[1], j, jend);
+                if (p.causal) hide_later(s, j, c[n].q + off);
+                if (p.mask) hide_masked(s, p.mask + b * p.mask_s[0] + (int64_t)c[n].q * p.mask_s[1], j, jend);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) ds[t][e] = __builtin_amdgcn_exp2f(s[e]) * dp[e];
             }
@@ -676,7 +714,7 @@ __global__ __launch_bounds__(256) void k_attn_dq_few(const AttnP p) {
     }
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
-        if (qb + n * 16 + i16 < p.Lq) store_dq<T, DN>(p, acc[n], b, h, qb + n * 16 + i16, split, g);
+        if (c[n].in) store_dq<T, DN>(p, acc[n], b, h + c[n].h, c[n].q, split, g);
 }
 
 // dk, dv of at most 16 NQ keys per tile: the walk goes over 32 queries at a time of every head of the group; dO, then Q pass through the region
@@ -810,7 +848,7 @@ __global__ __launch_bounds__(256) void k_attn_dkv_few(const AttnP p) {
 // hold 8 components of one row).  D_i = sum_j p_ij dp_ij is summed here, where a row's probabilities are all at hand: `out` is not read, and
 // its rounding does not enter.  K, dO and Q pass one after the other through the wave's LDS region to be read down their rows.
 template <typename T, int DP>
-__global__ __launch_bounds__(256, 2) void k_attn_bwd_small(const AttnP p) {
+__global__ __launch_bounds__(256, 3) void k_attn_bwd_small(const AttnP p) {
     constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, LD = DP + LDS_PAD;
     __shared__ __attribute__((aligned(16))) bf16 region[4 * NP * 32 * LD];
     __shared__ __attribute__((aligned(16))) float rowv[4][2][32];
@@ -898,17 +936,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_bwd_small(const AttnP p) {
             }
         }
         wave_fence();
-#pragma unroll
-        for (int d = 0; d < DN; ++d) {
-            Frag<NP> a;
-            frag_cols<NP, LD>(lds, (size_t)32 * LD, 4 * g, 16 + 4 * g, d * 16, lane, a);
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const int q = n * 16 + i16, col = d * 16 + 4 * g;
-                const f32x4 o = mma<NP>(a, df[n], zero) * p.scale;
-                if (q < p.Lq && col < p.D) store4((T*)p.dq + b * p.dqs[0] + q * p.dqs[1] + h * p.dqs[2] + col, p.D - col, o);
-            }
-        }
+        product<T, DP>(lds, lane, df, [&](int n, int d) { return (T*)p.dq + b * p.dqs[0] + (n * 16 + i16) * p.dqs[1] + h * p.dqs[2] + d * 16; }, p.Lq, p.D, [&](int, f32x4 o) { return o * p.scale; });
     }
     // keys as columns: dk, dv
     Frag<NP> pf[2], df[2];
@@ -944,17 +972,12 @@ __global__ __launch_bounds__(256, 2) void k_attn_bwd_small(const AttnP p) {
         wave_fence();
         rows32_to_lds<NP, KC, LD>(rows, lds, lane);
         wave_fence();
+        product<T, DP>(lds, lane, cols, [&](int n, int d) { return dst + b * st[0] + (n * 16 + i16) * st[1] + hk * st[2] + d * 16; }, p.Lk, p.D, [&](int n, f32x4 o) {
+            o = o * scale;
 #pragma unroll
-        for (int d = 0; d < DN; ++d) {
-            Frag<NP> a;
-            frag_cols<NP, LD>(lds, (size_t)32 * LD, 4 * g, 16 + 4 * g, d * 16, lane, a);
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const int key = n * 16 + i16, col = d * 16 + 4 * g;
-                const f32x4 o = mma<NP>(a, cols[n], zero) * scale;
-                if (key < p.Lk && col < p.D) store4(dst + b * st[0] + key * st[1] + hk * st[2] + col, p.D - col, kok.on(n, lane) ? o : zero);
-            }
-        }
+            for (int e = 0; e < 4; ++e) o[e] = kok.on(n, lane) ? o[e] : 0.f;
+            return o;
+        });
     };
     give(gf, pf, (T*)p.dv, p.dvs, 1.f);
     give(qf, df, (T*)p.dk, p.dks, p.scale);
@@ -963,7 +986,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_bwd_small(const AttnP p) {
 // ------------------------------------------------------------------------------------------------ backward: one tile
 // KT keys in LDS (bias `lb`: 0 or -inf), queries as columns: acc += K^T ds.  WHOLE: these are all the keys, and `delta` is the sum over p dp
 // taken here; otherwise it is given (D = do . out).
-template <int NP, int DP, int NQ, int KT, bool WHOLE = false>
+template <int NP, int DP, int NQ, int KT, bool HIDE, bool WHOLE = false>
 __device__ __forceinline__ void dq_tile(const AttnP& p, const bf16* lk, const bf16* lv, const float* lb, int lane, int b, int j0, int jend, bool diagonal, int off,
                                         const int (&qi)[NQ], const Frag<NP> (&qf)[NQ][DP / 32], const Frag<NP> (&gf)[NQ][DP / 32], const float (&nlse)[NQ],
                                         float (&delta)[NQ], f32x4 (&acc)[NQ][DP / 16]) {
@@ -999,8 +1022,10 @@ __device__ __forceinline__ void dq_tile(const AttnP& p, const bf16* lk, const bf
                 f32x4 x;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(s[n][e], p.scale2, nlse[n]);
-                if (diagonal) hide_later(x, j0 + t * 16 + 4 * g, qi[n] + off);
-                if (p.mask) hide_masked(x, p.mask + b * p.mask_s[0] + (int64_t)min(qi[n], p.Lq - 1) * p.mask_s[1], j0 + t * 16 + 4 * g, jend);
+                if constexpr (HIDE) {
+                    if (diagonal) hide_later(x, j0 + t * 16 + 4 * g, qi[n] + off);
+                    if (p.mask) hide_masked(x, p.mask + b * p.mask_s[0] + (int64_t)min(qi[n], p.Lq - 1) * p.mask_s[1], j0 + t * 16 + 4 * g, jend);
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) ds[n][u][e] = __builtin_amdgcn_exp2f(x[e]) * (WHOLE ? 1.f : dp[n][u][e]);
             }
@@ -1032,11 +1057,12 @@ __device__ __forceinline__ void dq_tile(const AttnP& p, const bf16* lk, const bf
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) acc[n][d] = mma<NP>(a, df[n], acc[n][d]);
             }
+            if constexpr (!HIDE) __builtin_amdgcn_sched_barrier(0);  // (32 rows at a time: more would not fit the registers)
         }
     }
 }
 // KT queries in LDS (-lse in powers of two, -inf where a query takes no part, and -D), keys as columns: dv += dO^T p, dk += Q^T ds
-template <int NP, int DP, int NQ, int KT>
+template <int NP, int DP, int NQ, int KT, bool HIDE>
 __device__ __forceinline__ void dkv_tile(const AttnP& p, const bf16* lq, const bf16* lg, const float* ll, const float* ld, int lane, int b, int q0, bool diagonal, int off,
                                          const int (&ki)[NQ], const Frag<NP> (&kf)[NQ][DP / 32], const Frag<NP> (&vf)[NQ][DP / 32], f32x4 (&dk)[NQ][DP / 16],
                                          f32x4 (&dv)[NQ][DP / 16]) {
@@ -1071,8 +1097,10 @@ __device__ __forceinline__ void dkv_tile(const AttnP& p, const bf16* lq, const b
                 f32x4 x;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(s[n][e], p.scale2, nl[e]);
-                if (diagonal) hide_earlier(x, q0 + tt * 16 + 4 * g, ki[n] - off);
-                if (p.mask) hide_masked_rows(x, p.mask + b * p.mask_s[0] + min(ki[n], p.Lk - 1), p.mask_s[1], q0 + tt * 16 + 4 * g, p.Lq);
+                if constexpr (HIDE) {
+                    if (diagonal) hide_earlier(x, q0 + tt * 16 + 4 * g, ki[n] - off);
+                    if (p.mask) hide_masked_rows(x, p.mask + b * p.mask_s[0] + min(ki[n], p.Lk - 1), p.mask_s[1], q0 + tt * 16 + 4 * g, p.Lq);
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     pr[n][u][e] = __builtin_amdgcn_exp2f(x[e]);
@@ -1097,14 +1125,19 @@ __device__ __forceinline__ void dkv_tile(const AttnP& p, const bf16* lq, const b
                 dk[n][d] = mma<NP>(v, df[n], dk[n][d]);
             }
         }
+        if constexpr (!HIDE) __builtin_amdgcn_sched_barrier(0);  // (32 rows at a time: more would not fit the registers)
     }
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dq
 // (bf16, D = 128: two column tiles fit 256 registers with tiles of 32 keys, and two waves per SIMD then hide each other's LDS reads: 495 us
 // instead of 700 with one wave per SIMD and 64 keys, 8192 x 8192 causal, 16 heads)
+// (bf16, D <= 64: steps without a mask and off the diagonal take a copy of the tile that has no branches, so that products, exponentials and LDS reads of
+// different rows overlap: D = 32 55 -> 51 us, 32 x 4 heads of 1024 x 1024; D = 64 85 -> 80, 8 x 16 heads; at D = 128 its registers spill, 525 -> 584)
+template <typename T, int DP, int NQ>
+constexpr int DQ_WAVES = sizeof(T) == 4 ? 1 : DP == 32 ? 5 - NQ : DP == 64 ? 4 - NQ : NQ;
 template <typename T, int DP, int NQ, int KT>
-__global__ __launch_bounds__(256, DP == 128 && NQ == 2 ? 2 : 1) void k_attn_dq(const AttnP p) {
+__global__ __launch_bounds__(256, (DQ_WAVES<T, DP, NQ>)) void k_attn_dq(const AttnP p) {
     constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, KN = KT / 16, NT = 256, LD = DP + LDS_PAD, QT = 64 * NQ;
     __shared__ __attribute__((aligned(16))) bf16 lk[NP * KT * LD];
     __shared__ __attribute__((aligned(16))) bf16 lv[NP * KT * LD];
@@ -1150,7 +1183,10 @@ __global__ __launch_bounds__(256, DP == 128 && NQ == 2 ? 2 : 1) void k_attn_dq(c
             sv.load(p, vp, p.vs[1], kvalid, j0 + KT, jend, tid);
         }
         const bool diagonal = p.causal && j0 + KT - 1 > q0 + off;
-        dq_tile<NP, DP, NQ, KT>(p, lk, lv, lb, lane, b, j0, jend, diagonal, off, qi, qf, gf, nlse, delta, acc);
+        if (DP == 128 || diagonal || p.mask)
+            dq_tile<NP, DP, NQ, KT, true>(p, lk, lv, lb, lane, b, j0, jend, diagonal, off, qi, qf, gf, nlse, delta, acc);
+        else
+            dq_tile<NP, DP, NQ, KT, false>(p, lk, lv, lb, lane, b, j0, jend, false, off, qi, qf, gf, nlse, delta, acc);
     }
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
@@ -1160,8 +1196,9 @@ __global__ __launch_bounds__(256, DP == 128 && NQ == 2 ? 2 : 1) void k_attn_dq(c
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
 // Columns are keys; the walk goes over the query tiles of every head of the key's group, so the gradients of shared heads are summed
 // in registers.  A split takes a contiguous part of that walk.
+// (the tile without branches, as above: D = 32 74 -> 63 us, D = 128 1010 -> 976, 8192 x 8192 causal; D = 64 112 both ways, and with a mask 39 -> 45)
 template <typename T, int DP, int NQ, int KT>
-__global__ __launch_bounds__(256) void k_attn_dkv(const AttnP p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 && DP == 32 ? 5 - NQ : 1) void k_attn_dkv(const AttnP p) {
     constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, KN = KT / 16, NT = 256, LD = DP + LDS_PAD, CT = 64 * NQ;
     __shared__ __attribute__((aligned(16))) bf16 lq[NP * KT * LD];
     __shared__ __attribute__((aligned(16))) bf16 lg[NP * KT * LD];
@@ -1225,7 +1262,10 @@ __global__ __launch_bounds__(256) void k_attn_dkv(const AttnP p) {
         const int q0 = (first + t % per_head) * KT;
         if (t + 1 < tend) load(t + 1);
         const bool diagonal = p.causal && k0 + 16 * NQ - 1 > q0 + off;
-        dkv_tile<NP, DP, NQ, KT>(p, lq, lg, ll, ld, lane, b, q0, diagonal, off, ki, kf, vf, dk, dv);
+        if (DP == 64 || (DP == 128 && NQ == 1) || diagonal || p.mask)
+            dkv_tile<NP, DP, NQ, KT, true>(p, lq, lg, ll, ld, lane, b, q0, diagonal, off, ki, kf, vf, dk, dv);
+        else
+            dkv_tile<NP, DP, NQ, KT, false>(p, lq, lg, ll, ld, lane, b, q0, false, off, ki, kf, vf, dk, dv);
     }
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
@@ -1249,10 +1289,9 @@ __global__ __launch_bounds__(256) void k_attn_bwd_mid(const AttnP p) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = lane & 15, g = lane >> 4;
     const Valid kvalid(p.key_valid, (int64_t)b * p.Lk), qvalid(p.query_valid, (int64_t)b * p.Lq);
     const int col[1] = {wave * 16 + i16};  // this lane's query, then its key
-    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     f32x4 dk[1][DN], dv[1][DN];
 #pragma unroll
-    for (int d = 0; d < DN; ++d) dk[0][d] = dv[0][d] = zero;
+    for (int d = 0; d < DN; ++d) dk[0][d] = dv[0][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
     Stage<T, DP, 256, L> sk, sv, sq, sg;
     sk.load(p, (const T*)p.k + b * p.ks[0] + hk * p.ks[2], p.ks[1], kvalid, 0, p.Lk, tid);
     sv.load(p, (const T*)p.v + b * p.vs[0] + hk * p.vs[2], p.vs[1], kvalid, 0, p.Lk, tid);
@@ -1281,14 +1320,10 @@ __global__ __launch_bounds__(256) void k_attn_bwd_mid(const AttnP p) {
                 frag_rows<NP, LD>(lg, (size_t)L * LD, wave * 16, kc * 32, lane, gf[0][kc]);
             }
 #pragma unroll
-            for (int d = 0; d < DN; ++d) acc[0][d] = zero;
-            dq_tile<NP, DP, 1, L, true>(p, lk, lv, lb, lane, b, 0, p.Lk, p.causal, off, col, qf, gf, nlse, delta, acc);
+            for (int d = 0; d < DN; ++d) acc[0][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            dq_tile<NP, DP, 1, L, true, true>(p, lk, lv, lb, lane, b, 0, p.Lk, p.causal, off, col, qf, gf, nlse, delta, acc);
             if (g == 0) ld[col[0]] = -delta[0];
-            if (col[0] < p.Lq) {
-#pragma unroll
-                for (int d = 0; d < DN; ++d)
-                    if (d * 16 + 4 * g < p.D) store4((T*)p.dq + b * p.dqs[0] + col[0] * p.dqs[1] + h * p.dqs[2] + d * 16 + 4 * g, p.D - d * 16 - 4 * g, acc[0][d] * p.scale);
-            }
+            if (col[0] < p.Lq) store_dq<T, DN>(p, acc[0], b, h, col[0], 0, g);
         }
         __syncthreads();  // every wave's D
         Frag<NP> kf[1][KC], vf[1][KC];
@@ -1297,18 +1332,9 @@ __global__ __launch_bounds__(256) void k_attn_bwd_mid(const AttnP p) {
             frag_rows<NP, LD>(lk, (size_t)L * LD, wave * 16, kc * 32, lane, kf[0][kc]);
             frag_rows<NP, LD>(lv, (size_t)L * LD, wave * 16, kc * 32, lane, vf[0][kc]);
         }
-        dkv_tile<NP, DP, 1, L>(p, lq, lg, ll, ld, lane, b, 0, p.causal, off, col, kf, vf, dk, dv);
+        dkv_tile<NP, DP, 1, L, true>(p, lq, lg, ll, ld, lane, b, 0, p.causal, off, col, kf, vf, dk, dv);
     }
-    if (col[0] < p.Lk) {
-        const bool on = lb[col[0]] == 0.f;
-#pragma unroll
-        for (int d = 0; d < DN; ++d) {
-            const int c = d * 16 + 4 * g;
-            if (c >= p.D) continue;
-            store4((T*)p.dk + b * p.dks[0] + col[0] * p.dks[1] + hk * p.dks[2] + c, p.D - c, on ? dk[0][d] * p.scale : zero);
-            store4((T*)p.dv + b * p.dvs[0] + col[0] * p.dvs[1] + hk * p.dvs[2] + c, p.D - c, on ? dv[0][d] : zero);
-        }
-    }
+    if (col[0] < p.Lk) store_dkv<T, DN>(p, dk[0], dv[0], lb[col[0]] == 0.f, b, hk, col[0], 0, g);
 }
 
 // sum of the splits' gradients, in split order, into a strided [B, L, H, D] tensor
@@ -1317,16 +1343,16 @@ __global__ __launch_bounds__(256) void k_attn_sum(const float* part, int n_split
     const int cols = (D + 3) / 4;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)B * L * H, row = id / cols;
     if (row >= rows) return;
-    const int col = (int)(id % cols) * 4;
+    const int col = min((int)(id % cols) * 4, D - 4);  // (the last columns perhaps twice)
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
     for (int s = 0; s < n_split; ++s) {
-        const float* src = part + (s * rows + row) * D + col;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (col + e < D) o[e] += src[e];
+        f32x4 x;
+        __builtin_memcpy(&x, part + (s * rows + row) * D + col, 16);
+        o += x;
     }
     const int64_t h = row % H, l = row / H % L, b = row / H / L;
-    store4(dst + b * sb + l * sl + h * sh + col, D - col, o);
+    store4(dst + b * sb + l * sl + h * sh + col, 4, o);
 }
 
 enum Pass { FWD, DQ, DKV };
@@ -1362,37 +1388,44 @@ Shape choose(Pass pass, int n_col, int walk, int64_t n_bh) {
             if (shared && n_col <= 16) return {32, 32, k_attn_fwd_few<T, DP, 1, 8>, 512, true, 8};
         return {32, 32, n_col <= 16 ? k_attn_fwd_few<T, DP, 1, 4> : k_attn_fwd_few<T, DP, 2, 4>, 256, true, wpp};
     }
+    // two column tiles per wave share each operand read from LDS, but a walk of one step is bound by the latency of its loads (10 queries, 1363 keys, D = 120,
+    // bf16, dk and dv: 50 us on two, 38 on one; 64 queries, 256 keys, D = 32, fp32: 10.6 and 9.3)
     if constexpr (wide)
-        if (n_col > 64 && n_bh * ((n_col + 127) / 128) >= 256) return tiles<T, DP, 2, KT>(pass);
+        if (n_col > 64 && !(pass == DKV && walk <= KT) && n_bh * ((n_col + 127) / 128) >= 256) return tiles<T, DP, 2, KT>(pass);
     return tiles<T, DP, 1, KT>(pass);
 }
 
+int heads_packed(const AttnP& p, Pass pass) { return pass != DKV && (int64_t)p.G * p.Lq <= 32 ? p.G : 1; }
+
 Shape choose(const AttnP& p, Pass pass) {
-    const int n_col = pass == DKV ? p.Lk : p.Lq, w = pass == DKV ? p.Lq : p.Lk;
-    const int64_t n = (int64_t)p.B * (pass == DKV ? p.Hkv : p.H);
+    const int pack = heads_packed(p, pass), n_col = pass == DKV ? p.Lk : p.Lq * pack, w = pass == DKV ? p.Lq : p.Lk;
+    const int64_t n = (int64_t)p.B * (pass == DKV ? p.Hkv : p.H / pack);
     if (p.dtype == 1) return p.D <= 32 ? choose<bf16, 32>(pass, n_col, w, n) : p.D <= 64 ? choose<bf16, 64>(pass, n_col, w, n) : choose<bf16, 128>(pass, n_col, w, n);
     return p.D <= 32 ? choose<float, 32>(pass, n_col, w, n) : p.D <= 64 ? choose<float, 64>(pass, n_col, w, n) : choose<float, 128>(pass, n_col, w, n);
 }
 
-// Few workgroups and a long walk: the walk is split over workgroups whose results a second kernel joins (about 5 us), until the chip has
-// about two workgroups per CU; a part keeps at least eight steps.
+// Few workgroups and a long walk: the walk is split over workgroups whose results a second kernel joins (4 us), until the chip has
+// about two workgroups per CU; a part keeps at least eight steps, where columns are few two (3 queries, 4090 keys, 16 heads on 4, D = 88, fp32:
+// parts of eight steps 51 us, of four 36, of two 24; a walk of less than eight steps in one part: one query, 1024 keys 12.4 us, in two parts 12.8 and one launch more).
 struct Plan {
     Shape s;
-    int n_col_tile, n_split, split_len, wpp;
+    int n_col_tile, n_split, split_len, wpp, pack;
     int64_t n_bh, blocks;
 };
 Plan plan(const AttnP& p, Pass pass) {
     Plan r;
     r.s = choose(p, pass);
-    const int n_col = pass == DKV ? p.Lk : p.Lq, walk = pass == DKV ? p.Lq : p.Lk;
+    r.pack = heads_packed(p, pass);
+    const int n_col = pass == DKV ? p.Lk : p.Lq * r.pack, walk = pass == DKV ? p.Lq : p.Lk;
     r.n_col_tile = (n_col + r.s.col_tile - 1) / r.s.col_tile;
-    r.n_bh = (int64_t)p.B * (pass == DKV ? p.Hkv : p.H);
+    r.n_bh = (int64_t)p.B * (pass == DKV ? p.Hkv : p.H / r.pack);
     const int64_t base = r.n_bh * r.n_col_tile;
     r.wpp = r.s.wpp;
     const int step = r.s.walk_tile * r.wpp;
     const int64_t steps = (int64_t)((walk + step - 1) / step) * (pass == DKV ? p.G : 1), slots = 512 * 4 / (r.s.few ? r.wpp : r.s.threads / 64);
     int64_t n = base * 2 <= slots ? slots / (base > 0 ? base : 1) : 1;
-    n = n < steps / 8 ? n : steps / 8;
+    const int64_t most = steps < 8 ? 1 : steps / (r.s.few ? 2 : 8);
+    n = n < most ? n : most;
     n = n < 1 ? 1 : n > 64 ? 64 : n;
     const int64_t len = (steps + n - 1) / n * step;  // (DKV: the kernel cuts its own walk, only n_split counts)
     r.split_len = len < step ? step : len > 0x7fffffff - step ? 0x7fffffff - step : (int)len;
@@ -1413,6 +1446,7 @@ const char* launch(AttnP p, const Plan& r, hipStream_t s) {
     p.n_split = r.n_split;
     p.split_len = r.split_len;
     p.wpp = r.wpp;
+    p.pack = r.pack;
     p.tile_major = p.causal && !r.s.few && r.n_bh * r.n_split < 64;
     int64_t blocks = r.blocks;
     if (blocks <= 0) return nullptr;
@@ -1436,8 +1470,9 @@ Short short_backward(const AttnP& p) {
     return NONE;
 }
 template <typename T>
-void launch_short(const AttnP& p, Short kind, hipStream_t s) {
+void launch_short(AttnP p, Short kind, hipStream_t s) {
     const int64_t n = (int64_t)p.B * p.Hkv;
+    p.n_split = 1;
     void (*kernel)(AttnP) = nullptr;
     if (kind == WAVE) {
         kernel = k_attn_bwd_small<T, 32>;

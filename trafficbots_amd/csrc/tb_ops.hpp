@@ -166,6 +166,43 @@ __device__ __forceinline__ void store4(bf16* p, int n, f32x4 v) {
     }
 }
 
+// A row of D results held in accumulator layout: group g of 16 lanes holds columns 16 d + 4 g .. + 3 of it in acc[d].  In bf16 two groups first
+// exchange halves of a pair of tiles (group 0 then has columns 0 .. 7 of the first tile, group 1 those of the second, groups 2 and 3 columns
+// 8 .. 15), so that a lane stores 16 bytes at once.
+template <typename T, int DN>
+__device__ __forceinline__ void store_row(T* row, int D, int g, const f32x4 (&acc)[DN]) {
+    static_assert(DN % 2 == 0);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int d = 0; d < DN; ++d)
+            if (d * 16 + 4 * g < D) store4(row + d * 16 + 4 * g, D - d * 16 - 4 * g, acc[d]);
+    } else {
+#pragma unroll
+        for (int d = 0; d < DN; d += 2) {
+            unsigned x[2], y[2], o[4];
+            const bf16x4 hx = __builtin_convertvector(acc[d], bf16x4), hy = __builtin_convertvector(acc[d + 1], bf16x4);
+            __builtin_memcpy(x, &hx, 8);
+            __builtin_memcpy(y, &hy, 8);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {  // odd groups of x change places with even groups of y
+                const auto r = __builtin_amdgcn_permlane16_swap(x[k], y[k], false, false);
+                o[k] = r[0];
+                o[2 + k] = r[1];
+            }
+            const int col = d * 16 + 16 * (g & 1) + 8 * (g >> 1), n = D - col;
+            if (n >= 8) {
+                __builtin_memcpy(row + col, o, 16);
+            } else {
+                bf16x8 v;
+                __builtin_memcpy(&v, o, 16);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j < n) row[col + j] = v[j];
+            }
+        }
+    }
+}
+
 __device__ __forceinline__ f32x4 load4(const float* p, int n) {
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     if (n >= 4) {

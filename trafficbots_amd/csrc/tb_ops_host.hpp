@@ -18,7 +18,7 @@ struct AttnP {
     void *out, *dq, *dk, *dv;
     float *lse, *delta;
     // of one launch
-    int n_col_tile, n_split, split_len, wpp, tile_major;
+    int n_col_tile, n_split, split_len, wpp, pack, tile_major;  // pack: heads whose queries are columns of one walk
     float *part, *part_lse;
 };
 int64_t attention_workspace(const AttnP& p, bool backward);

@@ -244,6 +244,11 @@ def _ptr(t: Optional[Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def _like(t: Tensor) -> Tensor:
+    """A contiguous tensor of t's shape and type (where t is contiguous itself: 1.2 us instead of 1.8)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 class HipEngine:
     """One `tb_ctx` on one device."""
 
@@ -946,7 +951,7 @@ class HipEngine:
         `attn_mask` [Lq, Lk] or [B, Lq, Lk]: True = may NOT attend (`attention.py:90-99`).  `causal`: key j for queries i >= j + Lq - Lk.
         `scale` defaults to 1 / sqrt(D).  Returns (out [B, Lq, H, D], lse [B, H, Lq] fp32); a query without a key gets 0 and -inf."""
         keep, args = self._attention_args("attention", q, k, v, query_valid, key_valid, attn_mask, causal, scale)
-        out = q.new_empty(q.shape)
+        out = _like(q)
         lse = q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)
         io = hip.TbAttentionIO()
         hip.PACK_ATTENTION.pack_into(io, 0, *args, out.data_ptr(), *out.stride()[:3], lse.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
@@ -964,7 +969,7 @@ class HipEngine:
             raise ValueError(f"{what}: d_out {tuple(d_out.shape)} and out {tuple(out.shape)} must have q's shape {tuple(q.shape)}")
         lse = self._f32(what, "lse", lse, (q.shape[0], q.shape[2], q.shape[1]))
         out, d_out = self._adjacent(out), self._adjacent(d_out)
-        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        dq, dk, dv = _like(q), _like(k), _like(v)
         io = hip.TbAttentionIO()
         hip.PACK_ATTENTION.pack_into(io, 0, *args, out.data_ptr(), *out.stride()[:3], lse.data_ptr(), d_out.data_ptr(), *d_out.stride()[:3], dq.data_ptr(),
                                      dk.data_ptr(), dv.data_ptr(), *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3], 0, 0)
@@ -988,8 +993,9 @@ class HipEngine:
                    ) -> Tuple[Tensor, Tensor, Tensor]:
         """`tb_layer_norm` over the last axis of x [..., C] (C <= 8192; fp32 or bf16): (y [..., C], mean [...], rstd [...], both fp32)."""
         dtype, n_row, x, weight, bias = self._norm_args("layer_norm", x, weight, bias)
-        y = x.new_empty(x.shape)
-        mean, rstd = x.new_empty(x.shape[:-1], dtype=torch.float32), x.new_empty(x.shape[:-1], dtype=torch.float32)
+        y = torch.empty_like(x)
+        mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+        rstd = torch.empty_like(mean)
         io = hip.TbLayerNormIO()
         hip.PACK_LAYER_NORM.pack_into(io, 0, dtype, x.shape[-1], n_row, float(eps), x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean.data_ptr(),
                                       rstd.data_ptr(), 0, 0, 0, 0, 0, 0)
@@ -1005,8 +1011,10 @@ class HipEngine:
             raise ValueError(f"{what}: d_out {tuple(d_out.shape)} must have x's shape {tuple(x.shape)}")
         d_out = d_out.contiguous()
         mean, rstd = self._f32(what, "mean", mean, x.shape[:-1]), self._f32(what, "rstd", rstd, x.shape[:-1])
-        dx = x.new_empty(x.shape) if want_dx else None
-        dw, db = (x.new_empty(x.shape[-1:]), x.new_empty(x.shape[-1:])) if want_dweight else (None, None)
+        dx, dw, db = torch.empty_like(x) if want_dx else None, None, None
+        if want_dweight:
+            dw = x.new_empty(x.shape[-1:])
+            db = torch.empty_like(dw)
         io = hip.TbLayerNormIO()
         hip.PACK_LAYER_NORM.pack_into(io, 0, dtype, x.shape[-1], n_row, 0.0, x.data_ptr(), _ptr(weight), 0, 0, mean.data_ptr(), rstd.data_ptr(), d_out.data_ptr(),
                                       _ptr(dx), _ptr(dw), _ptr(db), 0, 0)
@@ -1036,7 +1044,7 @@ class HipEngine:
                 raise ValueError(f"linear: {name} has shape {tuple(t.shape)}, expected {want}")
         bias, residual = None if bias is None else bias.contiguous(), None if residual is None else residual.contiguous()
         y = x.new_empty(shape)
-        act = x.new_empty(shape) if want_act and residual is not None else None
+        act = torch.empty_like(y) if want_act and residual is not None else None
         io = hip.TbLinearIO()
         hip.PACK_LINEAR.pack_into(io, 0, dtype, weight.shape[1], weight.shape[0], 1 if activation else 0, n_row, x.data_ptr(), weight.data_ptr(), _ptr(bias),
                                   _ptr(rv), _ptr(residual), y.data_ptr(), _ptr(act), 0, 0, 0, 0, 0, 0)
@@ -1053,8 +1061,8 @@ class HipEngine:
             if t is not None and t.shape != shape:
                 raise ValueError(f"linear_backward: {name} has shape {tuple(t.shape)}, expected {shape}")
         d_out, act = d_out.contiguous(), None if act is None else act.contiguous()
-        dx = x.new_empty(x.shape) if want_dx else None
-        dw = x.new_empty(weight.shape) if want_dweight else None
+        dx = torch.empty_like(x) if want_dx else None
+        dw = torch.empty_like(weight) if want_dweight else None
         db = x.new_empty(weight.shape[:1]) if want_dbias else None
         io = hip.TbLinearIO()
         hip.PACK_LINEAR.pack_into(io, 0, dtype, weight.shape[1], weight.shape[0], 0 if act is None else 1, n_row, x.data_ptr(), weight.data_ptr(), 0, _ptr(rv), 0, 0,
