@@ -1404,9 +1404,11 @@ Shape choose(const AttnP& p, Pass pass) {
     return p.D <= 32 ? choose<float, 32>(pass, n_col, w, n) : p.D <= 64 ? choose<float, 64>(pass, n_col, w, n) : choose<float, 128>(pass, n_col, w, n);
 }
 
-// Few workgroups and a long walk: the walk is split over workgroups whose results a second kernel joins (4 us), until the chip has
-// about two workgroups per CU; a part keeps at least eight steps, where columns are few two (3 queries, 4090 keys, 16 heads on 4, D = 88, fp32:
-// parts of eight steps 51 us, of four 36, of two 24; a walk of less than eight steps in one part: one query, 1024 keys 12.4 us, in two parts 12.8 and one launch more).
+// Few workgroups and a long walk: the walk is split over workgroups whose results a second kernel joins (4 us), until the chip has about two
+// workgroups per CU.  A part keeps at least four steps, where columns are few two, and a walk of less than eight is left whole.  900 x 900, D = 128,
+// 4 heads, bf16: parts of at least eight steps (here: no split) forward / dq / dkv 33 / 38 / 47 us, of four 17 / 20 / 24 and the join 4 / 3 / 3, of
+// two 15 / 18 / 22 and 5 / 3 / 3.  Few columns (3 queries, 4090 keys, 16 heads on 4, D = 88, fp32): of eight 51 us, of four 36, of two 24.  A short walk:
+// one query, 1024 keys 12.4 us whole, 12.8 and one launch more in two parts.
 struct Plan {
     Shape s;
     int n_col_tile, n_split, split_len, wpp, pack;
@@ -1424,7 +1426,7 @@ Plan plan(const AttnP& p, Pass pass) {
     const int step = r.s.walk_tile * r.wpp;
     const int64_t steps = (int64_t)((walk + step - 1) / step) * (pass == DKV ? p.G : 1), slots = 512 * 4 / (r.s.few ? r.wpp : r.s.threads / 64);
     int64_t n = base * 2 <= slots ? slots / (base > 0 ? base : 1) : 1;
-    const int64_t most = steps < 8 ? 1 : steps / (r.s.few ? 2 : 8);
+    const int64_t most = steps < 8 ? 1 : steps / (r.s.few ? 2 : 4);
     n = n < most ? n : most;
     n = n < 1 ? 1 : n > 64 ? 64 : n;
     const int64_t len = (steps + n - 1) / n * step;  // (DKV: the kernel cuts its own walk, only n_split counts)
