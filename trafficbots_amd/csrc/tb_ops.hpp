@@ -136,12 +136,15 @@ struct Held<bf16> {
 // where the chunk of columns col .. col + 7 of rows of `width` >= 8 elements is loaded from; fit()'s shift is what it lies behind `col`
 __device__ __forceinline__ int chunk_start(int col, int width) { return min(col, width - 8); }
 
-// a validity mask that may be absent: then one byte that says yes, read with stride 0 (no branch around the load)
+// a validity mask that may be absent: then one byte that says yes, read with stride 0 (no branch around the load).  The pointer says that it is
+// global memory: chosen between two sources it would be a flat one, whose loads count as LDS accesses too, and every LDS read of a step would
+// wait for the next step's prefetched mask.
 __device__ const uint8_t YES = 1;
 struct Valid {
-    const uint8_t* p;
+    typedef const __attribute__((address_space(1))) uint8_t* Global;
+    Global p;
     int64_t step;
-    __device__ __forceinline__ Valid(const uint8_t* mask, int64_t at) : p(mask ? mask + at : &YES), step(mask ? 1 : 0) {}
+    __device__ __forceinline__ Valid(const uint8_t* mask, int64_t at) : p((Global)(mask ? mask + at : &YES)), step(mask ? 1 : 0) {}
     __device__ __forceinline__ uint8_t operator[](int64_t i) const { return p[i * step]; }
 };
 
