@@ -710,3 +710,74 @@ def test_the_current_device_and_the_library_errors(eng):
     io.n_key, io.n_head, io.n_kv_head = 1 << 16, 1, 1
     io.q = io.k = io.v = io.out = io.lse = lse.data_ptr()
     assert eng.lib.tb_attention(eng._ctx, C.byref(io), None) != 0 and b"workspace" in eng.lib.tb_last_error(eng._ctx)
+
+
+@gpu
+def test_linear_gradients_need_their_operands(eng):
+    """The C entry refuses what its kernels would read through a null pointer."""
+    from trafficbots_amd import hip
+
+    t = torch.zeros(4, 16).cuda()
+    for fields, wish in ((("weight", "d_out"), "dbias"), (("weight", "d_out"), "dweight"), (("x", "d_out"), "dx"), (("x", "weight"), "dx"), (("x", "weight"), "dbias")):
+        io = hip.TbLinearIO()
+        io.n_in, io.n_out, io.n_row = 16, 16, 4
+        for f in fields + (wish,):
+            setattr(io, f, t.data_ptr())
+        assert eng.lib.tb_linear_backward(eng._ctx, C.byref(io), None) != 0 and b"NULL" in eng.lib.tb_last_error(eng._ctx)
+
+
+@gpu
+def test_forms_notice_operands_that_changed_before_the_gradient(eng):
+    from trafficbots_amd import functional as fn
+
+    g = torch.Generator().manual_seed(0)
+    q = torch.randn(2, 5, 2, 16, generator=g).cuda().requires_grad_()
+    x, w = torch.randn(6, 16, generator=g).cuda().requires_grad_(), torch.randn(8, 16, generator=g).cuda().requires_grad_()
+    kv, am, rv = torch.ones(2, 5, dtype=torch.bool).cuda(), torch.zeros(5, 5, dtype=torch.bool).cuda(), torch.ones(6, dtype=torch.bool).cuda()
+    for y, mask in ((fn.attention(eng, q, q, q, key_valid=kv), kv), (fn.attention(eng, q, q, q, attn_mask=am), am), (fn.linear(eng, x, w, row_valid=rv), rv)):
+        mask.logical_not_()
+        with pytest.raises(RuntimeError, match="modified"):
+            y.sum().backward()
+    y = fn.linear(eng, x, w, activation="relu")
+    y += 1  # ReLU's gradient needs it
+    with pytest.raises(RuntimeError, match="modified"):
+        y.sum().backward()
+
+
+@gpu
+def test_calls_of_two_threads(eng):
+    """Two threads on streams of their own, one context: the same bits as alone."""
+    import threading
+
+    inputs = [_step_inputs(s, F32) for s in (1, 2)]
+    want = [_step(eng, t) for t in inputs]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(20):
+                    got[i] = _step(eng, inputs[i])
+            s.synchronize()
+        except Exception as e:  # noqa: BLE001 (reported below)
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@gpu
+def test_an_engine_on_the_device_without_an_index(eng):
+    from trafficbots_amd.runtime import HipEngine
+
+    e = HipEngine(eng.cfg, "cuda")
+    x = torch.randn(3, 16, generator=torch.Generator().manual_seed(0)).cuda()
+    assert e.device == x.device and torch.equal(e.linear(x, x), eng.linear(x, x))

@@ -81,12 +81,21 @@ __device__ __forceinline__ void to_planes(const float (&x)[8], bf16x8 (&p)[NP]) 
 // load of a walk.  The caller clamps a row or column that is out of range or masked to one that is there (chunk_start), and what does not
 // belong is dropped where the data is used: fit() moves the end of a row that is no multiple of 8 (`ragged`, uniform over the launch) to
 // the chunk's front, keep(false) makes the chunk zero.  Rows of fewer than 8 elements take single loads (load_narrow).
+// 16 bytes from any element's address.  Said to be global memory: a pointer that the compiler cannot trace to an argument makes a load flat, and
+// LDS reads then wait for it.
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+__device__ __forceinline__ u32x4 load16(const void* p) { return *(const __attribute__((address_space(1))) u32x4_any*)p; }
 template <typename T>
 struct Held;
 template <>
 struct Held<float> {
     float x[8];
-    __device__ __forceinline__ void load(const float* p) { __builtin_memcpy(x, p, 32); }
+    __device__ __forceinline__ void load(const float* p) {
+        const u32x4 a = load16(p), b = load16(p + 4);
+        __builtin_memcpy(x, &a, 16);
+        __builtin_memcpy(x + 4, &b, 16);
+    }
     __device__ __forceinline__ void load_narrow(const float* p, int n) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = j < n ? p[j] : 0.f;
@@ -107,9 +116,8 @@ struct Held<float> {
 };
 template <>
 struct Held<bf16> {
-    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
     u32x4 u;
-    __device__ __forceinline__ void load(const bf16* p) { __builtin_memcpy(&u, p, 16); }
+    __device__ __forceinline__ void load(const bf16* p) { u = load16(p); }
     __device__ __forceinline__ void load_narrow(const bf16* p, int n) {
         bf16x8 v;
 #pragma unroll

@@ -190,7 +190,7 @@ extern "C" int tb_linear_backward(tb_ctx* ctx, const tb_linear_io* io, tb_stream
     if (!ctx || !io) return 1;
     return call(ctx, "tb_linear_backward", [&]() -> const char* {
         if (const char* e = sizes(*io)) return e;
-        if ((io->dx && !io->weight) || (io->n_row && (!io->d_out || (io->dweight && !io->x)))) return "a required buffer pointer is NULL";
+        if ((io->dx && !io->weight) || (io->n_row && (!io->d_out || ((io->dweight || io->dbias) && !io->x)))) return "a required buffer pointer is NULL";
         if (io->activation == 1 && io->n_row && !io->act) return "ReLU's gradient needs act (what tb_linear wrote there)";
         LinearP p = params(*io);
         p.act = io->activation == 1 ? io->act : nullptr;

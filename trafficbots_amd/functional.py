@@ -17,23 +17,23 @@ from torch.autograd.function import once_differentiable
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, engine, q, k, v, masks):
-        out, lse = engine.attention(q, k, v, **masks)
-        ctx.engine, ctx.masks = engine, masks
-        ctx.save_for_backward(q, k, v, out, lse)
+    def forward(ctx, engine, q, k, v, query_valid, key_valid, attn_mask, causal, scale):
+        out, lse = engine.attention(q, k, v, query_valid, key_valid, attn_mask, causal, scale)
+        ctx.engine, ctx.causal, ctx.scale = engine, causal, scale
+        ctx.save_for_backward(q, k, v, out, lse, query_valid, key_valid, attn_mask)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out):
-        dq, dk, dv = ctx.engine.attention_backward(d_out, *ctx.saved_tensors, **ctx.masks)
-        return None, dq, dk, dv, None
+        dq, dk, dv = ctx.engine.attention_backward(d_out, *ctx.saved_tensors, ctx.causal, ctx.scale)
+        return None, dq, dk, dv, None, None, None, None, None
 
 
 def attention(engine, q: Tensor, k: Tensor, v: Tensor, query_valid: Optional[Tensor] = None, key_valid: Optional[Tensor] = None,
               attn_mask: Optional[Tensor] = None, causal: bool = False, scale: Optional[float] = None) -> Tensor:
     """:meth:`HipEngine.attention` with gradients of q, k and v: [B, Lq, H, D]."""
-    return _Attention.apply(engine, q, k, v, dict(query_valid=query_valid, key_valid=key_valid, attn_mask=attn_mask, causal=causal, scale=scale))
+    return _Attention.apply(engine, q, k, v, query_valid, key_valid, attn_mask, causal, scale)
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -61,20 +61,20 @@ def layer_norm(engine, x: Tensor, weight: Optional[Tensor] = None, bias: Optiona
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, engine, x, weight, bias, residual, activation, row_valid):
-        y, act = engine.linear(x, weight, bias, activation=activation, row_valid=row_valid, residual=residual, want_act=activation is not None) \
-            if activation is not None else (engine.linear(x, weight, bias, row_valid=row_valid, residual=residual), None)
-        ctx.engine, ctx.row_valid = engine, row_valid
-        ctx.save_for_backward(x, weight, act)
+        y, act = engine.linear(x, weight, bias, activation, row_valid, residual, want_act=True) if activation else \
+            (engine.linear(x, weight, bias, activation, row_valid, residual), None)
+        ctx.engine = engine
+        ctx.save_for_backward(x, weight, act, row_valid)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out):
-        x, weight, act = ctx.saved_tensors
+        x, weight, act, row_valid = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dw = db = None
         if any(need[1:4]):
-            dx, dw, db = ctx.engine.linear_backward(d_out, x, weight, act=act, row_valid=ctx.row_valid, want_dx=need[1], want_dweight=need[2], want_dbias=need[3])
+            dx, dw, db = ctx.engine.linear_backward(d_out, x, weight, act=act, row_valid=row_valid, want_dx=need[1], want_dweight=need[2], want_dbias=need[3])
         return None, dx, dw, db, d_out if need[4] else None, None, None
 
 

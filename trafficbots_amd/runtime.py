@@ -258,6 +258,8 @@ class HipEngine:
         self.lib = hip.load()
         self.cfg = cfg
         self.device = torch.device(device)
+        if self.device.index is None:
+            self.device = torch.device(self.device.type, torch.cuda.current_device())
         torch.cuda.set_device(self.device)
         self._ctx = C.c_void_p()
         c = hip.make_config(cfg)
