@@ -465,6 +465,45 @@ def test_linear_backward_of_narrow_layers(eng, dtype, m, k, n, relu, pad):
 
 @gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m,k,n", [(16, 2100, 3), (5, 4096, 37), (130, 1500, 9), (1, 1040, 200)])
+def test_linear_of_few_rows_and_long_sums(eng, dtype, m, k, n):
+    """Few tiles and a long contraction: split and joined, forward and dx, narrower and wider than 16 bytes."""
+    g = torch.Generator().manual_seed(m + k + n)
+    x, w, b, res, do = (torch.randn(*s, generator=g).to(dtype) for s in ((m, k), (n, k), (n,), (m, n), (m, k)))
+    rv = torch.rand(m, generator=g) < 0.7
+    x[~rv] = float("nan")
+    ref = oo.linear(x, w, b, True, rv, res)
+    y, act = eng.linear(x.cuda(), w.cuda(), b.cuda(), activation="relu", row_valid=rv.cuda(), residual=res.cuda(), want_act=True)
+    _near("y", y, ref["y"], ref["y_bound"])
+    _near("act", act, ref["act"], ref["act_bound"])
+    x = torch.randn(m, n, generator=g).to(dtype)  # the other way round: dx contracts over k
+    wt = w.t().contiguous()
+    ref = oo.linear_backward(do, x, wt)
+    for name, t in zip(("dx", "dw", "db"), eng.linear_backward(do.cuda(), x.cuda(), wt.cuda())):
+        _near(name, t, ref[name], ref[name + "_bound"])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m,k,n", [(4096, 8, 8), (5001, 128, 70), (4099, 33, 128)])
+def test_linear_backward_of_narrow_layers_over_fewer_rows(eng, dtype, m, k, n):
+    g = torch.Generator().manual_seed(m + k + n)
+    x, w, do = (torch.randn(*s, generator=g).to(dtype) for s in ((m, k), (n, k), (m, n)))
+    ref = oo.linear_backward(do, x, w)
+    for name, t in zip(("dx", "dw", "db"), eng.linear_backward(do.cuda(), x.cuda(), w.cuda())):
+        _near(name, t, ref[name], ref[name + "_bound"])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("b,lq,lk,h,d", [(160, 1, 70, 4, 32), (600, 3, 66, 1, 16), (130, 9, 300, 4, 64)])
+def test_attention_of_many_problems_with_few_rows(eng, dtype, b, lq, lk, h, d):
+    """More problems than workgroups that would share a walk: one wave each."""
+    _check_attention(eng, *_attention_inputs(b, lq, lk, h, h, d, dtype, seed=b, pad=True))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_linear_over_many_rows(eng, dtype):
     """The long contraction of the weight's gradient is split and joined; big tiles with ragged edges."""
     g = torch.Generator().manual_seed(0)

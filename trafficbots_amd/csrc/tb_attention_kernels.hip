@@ -194,6 +194,10 @@ __device__ __forceinline__ void finish(const AttnP& p, const f32x4 (&acc)[DN], f
 }
 
 // ------------------------------------------------------------------------------------------------ forward
+// Keys and values pass through LDS in tiles of KT, the next tile's loads under way while this one is worked on.  Bound by what stands next to the
+// products: per pair an exponential and four more VALU operations, and every operand read from LDS serves two column tiles (NQ = 2).
+// 1024 x 1024, D = 32, 32 x 4 heads, bf16: 47 us (17.2 GFLOP, 365 TFLOP/s; its exponentials alone 14 us); 8192 x 8192 causal, D = 128, 16 heads on 4, bf16:
+// 436 us (630 TFLOP/s); 64 x 256, D = 32, 32 x 4 heads, fp32: 10.8 us (latency).
 template <typename T, int DP, int NQ, int KT>
 __global__ __launch_bounds__(256) void k_attn_fwd(const AttnP p) {
     constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, KN = KT / 16, NT = 256, LD = DP + LDS_PAD, QT = 64 * NQ;
@@ -295,7 +299,7 @@ __global__ __launch_bounds__(256) void k_attn_fwd(const AttnP p) {
     }
 }
 
-// join of the splits: o = sum_s 2^(lse_s - lse) o_s.  One thread per 4 columns of a row.
+// join of the splits: o = sum_s 2^(lse_s - lse) o_s.  One thread per 4 columns of a row (4 - 5 us: a launch and the latency of two rounds of loads).
 template <typename T>
 __global__ __launch_bounds__(256) void k_attn_join(const AttnP p) {
     const int cols = (p.D + 3) / 4;
@@ -409,7 +413,9 @@ __device__ __forceinline__ void product(const bf16* lds, int lane, const Frag<Pl
 // With at most 32 columns a workgroup has nothing to share: each wave walks 32 rows at a time on its own.  The rows it needs as A operand it
 // loads straight into that layout; only what the second product reads down its rows goes through LDS, a region of the wave's own, so
 // there is no barrier in the walk.  One wave takes one problem; with `wpp` = NW (a single query over a long cache) the waves of a workgroup
-// share the walk of one problem and join at its end.
+// share the walk of one problem and join at its end.  Long caches are bound by HBM (one query, 4096 keys, 16 x 32 heads on 8, D = 128, bf16: 45 us, 6.0
+// TB/s), short ones by the latency of a step (one query, 1024 keys, 4 heads, fp32: 12.4 us), many short problems by how few a SIMD holds
+// (8192 x 4 heads of 20 x 20, D = 32, fp32: 110 us, 3.1 TB/s: two waves of 178 registers; held to three, 168 registers, it spilled and took the same).
 // wave -> (row of the (batch, head) list, split, column tile); with wpp > 1 all waves of a workgroup get the same, and none is beyond the list
 __device__ __forceinline__ bool decode_few(const AttnP& p, int n_bh, int n_wave, int wave, int& bh, int& split, int& tile) {
     const int64_t id = p.wpp > 1 ? blockIdx.x : (int64_t)blockIdx.x * n_wave + wave, rest = id / n_bh;
@@ -1130,8 +1136,10 @@ __device__ __forceinline__ void dkv_tile(const AttnP& p, const bf16* lq, const b
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dq
-// (bf16, D = 128: two column tiles fit 256 registers with tiles of 32 keys, and two waves per SIMD then hide each other's LDS reads: 495 us
-// instead of 700 with one wave per SIMD and 64 keys, 8192 x 8192 causal, 16 heads)
+// Three products per pair of the forward's two, the same structure.  1024 x 1024, D = 32, 32 x 4 heads, bf16: 49 us (525 TFLOP/s); 8192 x 8192 causal,
+// D = 128, 16 heads on 4, bf16: 508 us (810 TFLOP/s).
+// (bf16, D = 128: two column tiles fit 256 registers with tiles of 32 keys, and two waves per SIMD then hide each other's LDS reads: 508 us
+// instead of 700 with one wave per SIMD and 64 keys)
 // (bf16, D <= 64: steps without a mask and off the diagonal take a copy of the tile that has no branches, so that products, exponentials and LDS reads of
 // different rows overlap: D = 32 55 -> 51 us, 32 x 4 heads of 1024 x 1024; D = 64 85 -> 80, 8 x 16 heads; at D = 128 its registers spill, 525 -> 584)
 template <typename T, int DP, int NQ>
@@ -1195,7 +1203,10 @@ __global__ __launch_bounds__(256, (DQ_WAVES<T, DP, NQ>)) void k_attn_dq(const At
 
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
 // Columns are keys; the walk goes over the query tiles of every head of the key's group, so the gradients of shared heads are summed
-// in registers.  A split takes a contiguous part of that walk.
+// in registers.  A split takes a contiguous part of that walk.  Four products per pair.  1024 x 1024, D = 32, 32 x 4 heads, bf16: 62 us (550 TFLOP/s);
+// 8192 x 8192 causal, D = 128, 16 heads on 4, bf16: 1005 us (547 TFLOP/s): there dk, dv and the column operands take 192 registers, one wave per SIMD is left, and
+// matrix (23 % of the cycles), LDS (28 %) and VALU work (34 %) follow each other.  One column tile per wave and two waves: 1470 (LDS reads double); tiles
+// of 32 queries held to 256 registers: 2760 (spills).
 // (the tile without branches, as above: D = 32 74 -> 63 us, D = 128 1010 -> 976, 8192 x 8192 causal; D = 64 112 both ways, and with a mask 39 -> 45)
 template <typename T, int DP, int NQ, int KT>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && DP == 32 ? 5 - NQ : 1) void k_attn_dkv(const AttnP p) {
@@ -1274,7 +1285,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP == 32 ? 5 - NQ : 1) void 
 
 // ------------------------------------------------------------------------------------------------ backward of at most 64 x 64
 // One workgroup per key / value head, one launch, no scratch: K, V, Q and dO are staged once, each wave takes 16 queries for dq, then 16 keys
-// for dk and dv.  The operands of a wave's columns are rows of the same LDS tiles.
+// for dk and dv.  The operands of a wave's columns are rows of the same LDS tiles.  61 x 61, D = 32, 33 x 4 heads, bf16: 7 us, latency.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void k_attn_bwd_mid(const AttnP p) {
     constexpr int NP = Planes<T>::N, KC = DP / 32, DN = DP / 16, LD = DP + LDS_PAD, L = 64;
@@ -1337,7 +1348,7 @@ __global__ __launch_bounds__(256) void k_attn_bwd_mid(const AttnP p) {
     if (col[0] < p.Lk) store_dkv<T, DN>(p, dk[0], dv[0], lb[col[0]] == 0.f, b, hk, col[0], 0, g);
 }
 
-// sum of the splits' gradients, in split order, into a strided [B, L, H, D] tensor
+// sum of the splits' gradients, in split order, into a strided [B, L, H, D] tensor (4 us: a launch and the latency of its loads)
 template <typename T>
 __global__ __launch_bounds__(256) void k_attn_sum(const float* part, int n_split, int B, int L, int H, int D, T* dst, int64_t sb, int64_t sl, int64_t sh) {
     const int cols = (D + 3) / 4;
@@ -1377,9 +1388,10 @@ Shape choose(Pass pass, int n_col, int walk, int64_t n_bh) {
     constexpr bool wide = sizeof(T) == 2 || DP == 32;  // two column tiles per wave fit the registers
     constexpr int KT = sizeof(T) == 2 || DP == 32 ? 64 : 32;
     if (n_col <= 32) {
-        // one problem per workgroup below 2048 problems (with a walk to share), one per wave above; the forward on eight waves where their
+        // one problem per workgroup below 512 problems (with a walk to share), one per wave above (shared | not, with the join: one query, 512 keys, fp32, 256
+        // problems 9.9 | 13.2 us, 512 19.2 | 18.1, 1024 33.9 | 28.8; 8 queries, 100 keys, bf16, 2048 problems 22.4 | 12.2); the forward on eight waves where their
         // tiles fit LDS (one query, 1024 keys, fp32: 14.2 us on four, 12.4 on eight)
-        const bool shared = walk > 64 && n_bh < 2048;
+        const bool shared = walk > 64 && n_bh < 512;
         const int wpp = shared ? 4 : 1;
         constexpr int NQ = wide ? 2 : 1;
         if (pass == DQ) return n_col <= 16 ? Shape{16, 32, k_attn_dq_few<T, DP, 1>, 256, true, wpp} : Shape{16 * NQ, 32, k_attn_dq_few<T, DP, NQ>, 256, true, wpp};
@@ -1388,7 +1400,9 @@ Shape choose(Pass pass, int n_col, int walk, int64_t n_bh) {
             if (shared && n_col <= 16) return {32, 32, k_attn_fwd_few<T, DP, 1, 8>, 512, true, 8};
         return {32, 32, n_col <= 16 ? k_attn_fwd_few<T, DP, 1, 4> : k_attn_fwd_few<T, DP, 2, 4>, 256, true, wpp};
     }
-    // two column tiles per wave share each operand read from LDS, but a walk of one step is bound by the latency of its loads (10 queries, 1363 keys, D = 120,
+    // two column tiles per wave share each operand read from LDS, where they leave a workgroup for every CU (forward / dq / dk, dv on one | two: 64 heads of 256 x
+    // 256, D = 64, bf16, 128 workgroups of two 9.1 / 9.6 / 10.5 | 10.4 / 11.1 / 13.4 us; 128 heads 11.4 / 12.7 / 13.6 | 10.8 / 11.7 / 14.4; 128 heads of 1024 x
+    // 1024, D = 32: 58 / 56 / 76 | 47 / 48 / 62), but a walk of one step is bound by the latency of its loads (10 queries, 1363 keys, D = 120,
     // bf16, dk and dv: 50 us on two, 38 on one; 64 queries, 256 keys, D = 32, fp32: 10.6 and 9.3)
     if constexpr (wide)
         if (n_col > 64 && !(pass == DKV && walk <= KT) && n_bh * ((n_col + 127) / 128) >= 256) return tiles<T, DP, 2, KT>(pass);

@@ -369,6 +369,8 @@ __device__ __forceinline__ void load_to_lds(const bf16* src, bf16* dst) {
 // at place c ^ (r % 8), which spreads a 16-row read over all banks.  A 256 x 256 tile on eight waves (128 x 64 each) reads LDS 768 cycles
 // for 1024 cycles of matrix work per 32 steps; 128 x 128 on four waves is balanced and serves what would not fill the chip otherwise.
 // Rows and columns beyond the matrix repeat its last one: they reach only results that are not stored.  Invalid rows too.
+// Bound by the matrix cores' feed: 16384 x 2048 -> 2048 with a residual 131 us (1050 TFLOP/s) on 256 x 256 tiles, 159 on 128 x 128, 187 through registers (k_linear);
+// 16384 x 512 -> 512: 18.6 us on 128 x 128, 21.6 through registers.
 template <int TR, int TC, int WR, int WC>
 __global__ __launch_bounds__(64 * WR * WC) void k_linear_direct(const LinearP p) {
     constexpr int NW = WR * WC, MR = TR / WR / 16, MC = TC / WC / 16, KB = 64;
@@ -455,7 +457,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear_direct(const LinearP p)
 // Both gradient products of a layer of at most 128 x 128 over many rows, in one walk: dy (and what gates it) and x are read once, where the
 // two products of their own read dy twice.  A workgroup of eight waves keeps W in LDS, walks tiles of RT rows in steps of the grid, and
 // holds its part of dW (64 x 32 of 128 x 128 per wave) in registers; dx of a tile leaves at once.  HBM-bound: 163840 rows of 128 fp32,
-// 336 MB in 65 us.
+// 336 MB in 79 us and 7 for the sum of the parts (4.2 TB/s; the two kernels, dx then dW, 120).
 template <typename T, bool GATED>
 __global__ __launch_bounds__(512) void k_linear_bwd_rows(const LinearP p) {
     constexpr int NP = Planes<T>::N, NT = 512, RT = NP == 3 ? 32 : 64, F = 128, LD = F + LDS_PAD, CR = RT / 16;
@@ -592,14 +594,22 @@ __global__ __launch_bounds__(256) void k_linear_finish(const LinearP p) {
     const int chunks = (p.N + VEC<T> - 1) / VEC<T>;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, m = id / chunks;
     if (m >= p.M) return;
-    const int n0 = (int)(id % chunks) * VEC<T>, n = p.N - n0;
+    const int n0 = max(min((int)(id % chunks) * VEC<T>, p.N - VEC<T>), 0), n = p.N - n0;  // (the last columns perhaps twice)
     Row16<T> a;
 #pragma unroll
     for (int j = 0; j < VEC<T>; ++j) a.v[j] = 0.f;
-    for (int s = 0; s < p.n_split; ++s) {
-        const float* src = p.part + (s * p.M + m) * p.N + n0;
+    if (n >= VEC<T>) {
+#pragma unroll 8
+        for (int s = 0; s < p.n_split; ++s) {
+            f32x4 v[VEC<T> / 4];
+            __builtin_memcpy(v, p.part + (s * p.M + m) * p.N + n0, sizeof(v));
 #pragma unroll
-        for (int j = 0; j < VEC<T>; ++j) a.v[j] += src[j < n ? j : 0];
+            for (int j = 0; j < VEC<T>; ++j) a.v[j] += v[j / 4][j % 4];
+        }
+    } else {
+        for (int s = 0; s < p.n_split; ++s)
+#pragma unroll
+            for (int j = 0; j < VEC<T>; ++j) a.v[j] += p.part[(s * p.M + m) * p.N + min(j, n - 1)];
     }
     const int64_t at = m * p.N + n0;
     if (p.bias) add_row<T>(a, (const T*)p.bias + n0, n);
@@ -618,7 +628,8 @@ Shape shape() {
 template <typename T, Kind KIND, bool GATED>
 Shape choose(const LinearP& p, int64_t r, int64_t c) {
     if (p.K < 8 || (KIND != FWD && p.N < 8)) return shape<T, KIND, GATED, 64, 64, 2, 2, true>();
-    // 128 x 128 tiles feed the matrix cores best; below one such tile per CU the smaller ones spread the work
+    // 128 x 128 tiles feed the matrix cores best; below one such tile per CU the smaller ones spread the work.  With one to two per CU both are near each other
+    // (128 | 64 wide: 8200 x 600 -> 600 fp32 61.6 | 63.5 us; dx of 14336 x 512 -> 512 bf16 22.2 | 24.8; 12000 x 333 -> 500 bf16 25.4 | 23.2).
     if (KIND == DW ? r > 64 || c > 64 : (r + 127) / 128 * ((c + 127) / 128) >= 256) return shape<T, KIND, GATED, 128, 128, 2, 2, false>();
     return shape<T, KIND, GATED, 64, 64, 2, 2, false>();
 }
@@ -655,7 +666,8 @@ Plan plan(const LinearP& p) {
     r.p.n_rt = (int)((R + r.s.tr - 1) / r.s.tr);
     r.p.n_ct = (C + r.s.tc - 1) / r.s.tc;
     // Splits of the contraction.  dW: about two workgroups per CU, a part keeps at least four steps.  The others only where the tiles leave CUs
-    // idle and the contraction is long: the join is a launch of its own (14 x 818 x 56 fp32, dx: 26 steps on one CU).
+    // idle and the contraction is long: the join is a launch of its own (whole | split and join: 14 x 818 -> 56 fp32, dx 26 | 7.9 + 1.7 us; 64 x 2048 -> 512 bf16 17.7 |
+    // 5.3 + 3.8; 1024 x 1024 -> 256 11.3 | 6.4 + 3.3).
     const int64_t K = KIND == FWD ? p.K : KIND == DX ? p.N : p.M, steps = (K + r.s.kb - 1) / r.s.kb, base = (int64_t)r.p.n_rt * r.p.n_ct;
     int64_t n = 1;
     if (KIND == DW)
@@ -685,8 +697,9 @@ void launch_sum(const float* part, int n_split, int64_t n_w, int n_b, void* dw, 
 
 }  // namespace
 
-// both gradients of a narrow layer over many rows: k_linear_bwd_rows
-bool rows_backward(const LinearP& p) { return p.N >= 8 && p.K >= 8 && p.N <= 128 && p.K <= 128 && p.M >= 16384; }
+// both gradients of a narrow layer over many rows: k_linear_bwd_rows (against dx, dW and their sum: 163840 x 128 -> 128 fp32 86 and 127 us; 16384 22 and 30; 4096 x 64
+// -> 128 bf16 15 and 19; below 4096 rows its 256 parts cost what it saves: 2048 x 64 -> 32 bf16 13.6 and 12.1)
+bool rows_backward(const LinearP& p) { return p.N >= 8 && p.K >= 8 && p.N <= 128 && p.K <= 128 && p.M >= 4096; }
 constexpr int ROWS_BLOCKS = 256;  // one per CU: its LDS holds the weight
 
 int64_t linear_workspace(const LinearP& p, bool backward) {  // (whichever gradients are wanted)
