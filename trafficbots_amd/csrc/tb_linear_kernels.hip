@@ -629,8 +629,12 @@ template <typename T, Kind KIND, bool GATED>
 Shape choose(const LinearP& p, int64_t r, int64_t c) {
     if (p.K < 8 || (KIND != FWD && p.N < 8)) return shape<T, KIND, GATED, 64, 64, 2, 2, true>();
     // 128 x 128 tiles feed the matrix cores best; below one such tile per CU the smaller ones spread the work.  With one to two per CU both are near each other
-    // (128 | 64 wide: 8200 x 600 -> 600 fp32 61.6 | 63.5 us; dx of 14336 x 512 -> 512 bf16 22.2 | 24.8; 12000 x 333 -> 500 bf16 25.4 | 23.2).
-    if (KIND == DW ? r > 64 || c > 64 : (r + 127) / 128 * ((c + 127) / 128) >= 256) return shape<T, KIND, GATED, 128, 128, 2, 2, false>();
+    // (128 | 64 wide: 8200 x 600 -> 600 fp32 61.6 | 63.5 us; dx of 14336 x 512 -> 512 bf16 22.2 | 24.8; 12000 x 333 -> 500 bf16 25.4 | 23.2; dW of 3000 x 256 -> 128 fp32, 46
+    // workgroups against 188, 14.4 | 7.5).  Small ones too where the large would work on 30 % more beside the matrix (35466 x 512 -> 150 fp32 94 | 63 us, 60000 x
+    // 300 -> 40 bf16 17.4 | 14.8; dx and dW of 35466 x 150 -> 150 fp32 39 and 39 | 36 and 29).
+    const int64_t big = (r + 127) / 128 * ((c + 127) / 128), small = (r + 63) / 64 * ((c + 63) / 64);  // tiles
+    const int64_t groups = KIND == DW ? big * (p.M / (sizeof(T) == 2 ? 256 : 128)) : big;  // (dW: with the splits, of four steps or more)
+    if (40 * big <= 13 * small && groups >= 256) return shape<T, KIND, GATED, 128, 128, 2, 2, false>();
     return shape<T, KIND, GATED, 64, 64, 2, 2, false>();
 }
 template <typename T, Kind KIND>
